@@ -36,6 +36,8 @@ enum {
 
 /* Cache element type = element size in bytes. */
 enum { SF37KV_F16 = 2, SF37KV_F32 = 4 };
+/* int8 caches (below): accepted by the calls that name it, refused elsewhere. */
+enum { SF37KV_I8 = 1 };
 /* Query element type for prefill. */
 enum { SF37KV_Q_F32 = 0, SF37KV_Q_BF16 = 1 };
 /* Snapshot KV row formats. */
@@ -179,6 +181,99 @@ int sf37kv_prefill(const sf37kv_cache *cache, const void *q, int q_type,
                    uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
                    int dtype, void *stream);
 
+/* ---- int8 caches: quantised as they are written, and read back ----
+ * An I8 cache of K (or V) takes sf37kv_i8_cache_bytes(cap, kv_heads, 128) bytes
+ * (132 for each head of a row; a multiple of 256): bytes c + 128 as
+ * [cap][kv_heads][128], then f32 scales [kv_heads][cap].  A head of a row has
+ * one scale s = max|x| / 127 (f32; 0 where that is below 2^-126), c is the
+ * integer nearest to x / s, ties to even, and the value read is c * s, so an
+ * element is off by at most s / 2.  A head with an element that is not finite
+ * gets the scale NaN: it reads back, and attends, as NaN.  head_dim is 128;
+ * the reference has no counterpart (its caches are f32).  Slots are pos % cap
+ * as in the other caches; caches and rows 16-byte aligned; positions < 2^31.
+ * sf37kv_decode, _prefill, _append and the snapshot calls do not take I8 caches:
+ * a chunked prefill appends its chunk, reads the attended rows back into an
+ * f16 cache that all layers share, and runs sf37kv_prefill on that. */
+uint64_t sf37kv_i8_cache_bytes(uint32_t cap, uint32_t kv_heads, uint32_t head_dim);
+
+/* Quantises n_tok rows per layer into slots (pos0 + t) % cap.  row_type:
+ * SF37KV_Q_F32 or SF37KV_Q_BF16.  With n_tok > cap the last cap rows stay.  A
+ * cache given twice in one call is refused. */
+typedef struct {
+    sf37kv_cache cache;
+    uint32_t pos0;
+    uint32_t n_tok;
+    const void *k;         /* [n_tok][kv_heads][128] */
+    const void *v;
+} sf37kv_append_i8_layer;
+int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n_layers, uint32_t kv_heads,
+                     uint32_t head_dim, int row_type, void *stream);
+
+/* Reads positions first_pos .. first_pos + rows - 1 of I8 caches back into
+ * f16 (rounded to nearest even) or f32 caches, position p to slot p % dst.cap.
+ * rows <= both caps; other slots of dst are left as they were. */
+typedef struct {
+    sf37kv_cache src;      /* I8 */
+    sf37kv_cache dst;      /* dst_dtype: SF37KV_F16 or SF37KV_F32 */
+    uint32_t first_pos;
+    uint32_t rows;
+} sf37kv_read_i8_layer;
+int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_layers, uint32_t kv_heads,
+                   uint32_t head_dim, int dst_dtype, void *stream);
+
+/* ---- batched decode: int8 caches, shared prefixes ----
+ * One query token of one sequence (or layer).  q, out, k_new and v_new are of
+ * io_type: SF37KV_Q_F32, or SF37KV_Q_BF16 (out is then rounded once from f32). */
+typedef struct {
+    sf37kv_cache cache;    /* this sequence's own rows */
+    uint32_t pos;          /* position of this token */
+    uint32_t reserved;
+    const void *q;         /* [q_heads][128] */
+    const float *gate;     /* [q_heads] or NULL (no gate) */
+    void *out;             /* [q_heads][128] */
+    const void *k_new;     /* [kv_heads][128] stored at pos first, or NULL */
+    const void *v_new;
+} sf37kv_decode_seq;
+
+/* sf37kv_decode() over I8 caches: the new rows are quantised into the caches
+ * and each query attends to its cache's rows.  head_dim 128, q_heads/kv_heads
+ * <= 16 and any number of sequences.  A cache that one sequence appends to
+ * may not be another's in the same call.
+ * workspace: device memory of sf37kv_decode_i8_workspace() bytes, 256-byte
+ * aligned, zero-filled once before its first use (sf37kv_dev_alloc does) and
+ * left reusable by every call.  Calls that may overlap on the GPU (other
+ * streams, graphs replayed side by side) need a workspace each.  Nothing is
+ * allocated, so the calls can be captured into a graph. */
+uint64_t sf37kv_decode_i8_workspace(uint32_t n_seqs, uint32_t q_heads, uint32_t kv_heads);
+int sf37kv_decode_i8(const sf37kv_decode_seq *seqs, uint32_t n_seqs, uint32_t q_heads, uint32_t kv_heads,
+                     uint32_t head_dim, int io_type, void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* Decode for sequences that share a prefix.  A group's prefix cache (f16)
+ * holds positions 0 .. prefix_len-1 at slot = position (prefix_len <= cap);
+ * each of its sequences keeps its later rows in its own cache (dtype
+ * SF37KV_F16 or SF37KV_I8; position p at slot p % cap), with the prefix's
+ * positions counted in pos, and pos >= prefix_len - 1 (at prefix_len - 1 the
+ * sequence has no row of its own yet).  The attention over the prefix is
+ * computed for all sequences of the group at once, on the tensor cores, and
+ * joined with each one's own rows; a sliding window covers both.  An own
+ * cache must still hold every own row of the window (else EINVAL), and prefix rows that
+ * any sequence of the group attends to must be finite.  prefix_len may be 0.  An I8 prefix is
+ * read back once with sf37kv_read_i8.
+ * io_type F32 computes to f32 accuracy (queries and weights in two f16 parts);
+ * BF16 rounds the weights to f16, which its output's rounding covers.
+ * Workspace and limits as sf37kv_decode_i8; n_seqs in the workspace query is
+ * the total over the groups. */
+typedef struct {
+    sf37kv_cache prefix;
+    uint32_t prefix_len;
+    uint32_t n_seqs;
+    const sf37kv_decode_seq *seqs;   /* host array */
+} sf37kv_shared_group;
+uint64_t sf37kv_decode_shared_workspace(uint32_t n_groups, uint32_t n_seqs, uint32_t q_heads, uint32_t kv_heads);
+int sf37kv_decode_shared(const sf37kv_shared_group *groups, uint32_t n_groups, uint32_t q_heads,
+                         uint32_t kv_heads, uint32_t head_dim, int dtype, int io_type, void *workspace,
+                         uint64_t workspace_bytes, void *stream);
+
 /* ---- snapshot KV sections (bit-exact with the reference formats) ----
  * Byte size of one encoded row. */
 uint64_t sf37kv_row_bytes(uint32_t kv_dim, int fmt, uint32_t group);
@@ -233,7 +328,7 @@ int sf37kv_unpack_slice_from_host(const void *host_src, const sf37kv_pack_layer 
                                   uint32_t col0, int dtype, int fmt, uint32_t group);
 
 /* Synchronizes the device and returns the library's device error flag: 1
- * when a prefill kernel's bounded wait gave up, 2 when a multi-GPU gather or
+ * when a prefill or shared-prefix kernel's bounded wait gave up, 2 when a multi-GPU gather or
  * reduce wait did (the kernel then stopped early and its output is
  * invalid), 0 otherwise, -1 if it cannot be read.  clear != 0 resets it. */
 int sf37kv_device_error(int clear);

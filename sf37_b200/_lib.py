@@ -6,6 +6,8 @@ every call raises.  Build it with ``python -m sf37_b200.build``.
 import ctypes
 import os
 
+import numpy as np
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsf37kv.so")
 
@@ -73,6 +75,19 @@ class CachePlan(ctypes.Structure):
                 ("full_layers", c_u32), ("sliding_layers", c_u32), ("cap", c_u32 * 64), ("sliding", c_u32 * 64),
                 ("kv_cache_bytes", c_u64)]
 
+
+# Descriptors of the batched calls, as numpy records with the C structs' layout:
+# arrays of them are filled by column (kv.decode_seqs_desc and the like).
+def _cache_fields(prefix=""):
+    return [(prefix + "k_cache", "u8"), (prefix + "v_cache", "u8"), (prefix + "cap", "u4"), (prefix + "sliding", "u4"),
+            (prefix + "window", "u4"), (prefix + "reserved", "u4")]
+
+
+APPEND_I8_LAYER = np.dtype(_cache_fields() + [("pos0", "u4"), ("n_tok", "u4"), ("k", "u8"), ("v", "u8")])
+READ_I8_LAYER = np.dtype(_cache_fields("src_") + _cache_fields("dst_") + [("first_pos", "u4"), ("rows", "u4")])
+DECODE_SEQ = np.dtype(_cache_fields() + [("pos", "u4"), ("pad", "u4"), ("q", "u8"), ("gate", "u8"), ("out", "u8"),
+                                         ("k_new", "u8"), ("v_new", "u8")])
+SHARED_GROUP = np.dtype(_cache_fields("prefix_") + [("prefix_len", "u4"), ("n_seqs", "u4"), ("seqs", "u8")])
 
 TP = ctypes.POINTER(Tensor)
 SP = ctypes.POINTER(Session)
@@ -151,6 +166,13 @@ SIGNATURES = {
     "sf37kv_sliding_prefill_cap": (c_u32, [c_u32, c_u32]),
     "sf37kv_kv_cache_bytes": (c_u64, [c_u32, c_u32, c_u32, c_int]),
     "sf37kv_prefill_default_chunk": (c_u32, [c_u64]),
+    "sf37kv_i8_cache_bytes": (c_u64, [c_u32, c_u32, c_u32]),
+    "sf37kv_append_i8": (c_int, [c_vp, c_u32, c_u32, c_u32, c_int, c_vp]),
+    "sf37kv_read_i8": (c_int, [c_vp, c_u32, c_u32, c_u32, c_int, c_vp]),
+    "sf37kv_decode_i8_workspace": (c_u64, [c_u32, c_u32, c_u32]),
+    "sf37kv_decode_i8": (c_int, [c_vp, c_u32, c_u32, c_u32, c_u32, c_int, c_vp, c_u64, c_vp]),
+    "sf37kv_decode_shared_workspace": (c_u64, [c_u32, c_u32, c_u32, c_u32]),
+    "sf37kv_decode_shared": (c_int, [c_vp, c_u32, c_u32, c_u32, c_u32, c_int, c_int, c_vp, c_u64, c_vp]),
     "sf37kv_plan_caches": (c_int, [c_u32, c_u32, c_u32, c_u32, c_u32, c_int, ctypes.POINTER(CachePlan)]),
     "sf37kv_managed_kv_policy": (c_int, [c_u64, c_u64, c_u64, c_u64]),
     # include/sf37kv_session.h

@@ -1,0 +1,1002 @@
+// Batched decode over int8 caches and over shared prefixes: the kernel for a
+// sequence's own rows, the merge, the split planning and the entry points.
+// The attention over a shared prefix itself is in prefix_tc05.cu.
+//
+// For query head h of KV head h / G over rows r (log2 domain, base-2 exps):
+//   s_r = (q[h] . K[r]) log2(e) / sqrt(128),  out = sum_r 2^(s_r - m) V[r] / l,
+// one pass with a running reference m that is raised only when a score exceeds
+// it by more than 8.  I8 rows enter as their integer codes (exact in f16):
+// a key's scale multiplies its score, a value's scale its weight.
+//
+// One CTA serves one KV head of one sequence over a run of rows (a split), so
+// each K/V byte is read once for all G query heads.  Four warps stream
+// interleaved 16-row blocks through private rings of cp.async stages; S = qK^T
+// and O += PV are mma.sync m16n8k16 tiles on fragments that the lanes load
+// straight from the stage.  The bytes bound it, not the products: 16 rows of I8
+// are 4224 bytes and about 270 warp instructions, and an SM receives those
+// bytes in 180 cycles, in which it could issue 720.  The CTAs of a (sequence,
+// KV head) leave unnormalised partials; the last one to finish (an atomic
+// counter) joins them, and the shared prefix's, in a fixed order, so results do
+// not depend on which CTA is last.
+//
+// Sixteen M rows of a tile hold, by MODE:
+//   kPair  G <= 8:  eight heads twice, f16 "hi" and remainder "lo" of q and of
+//          the weights, 22 bits at no extra cost;
+//   kWide  G <= 16 and bf16 outputs: sixteen heads, weights rounded to f16 (half a step is 2^-11 of
+//          a weight; the output's own rounding has 2^-8);
+//   kTwo   G <= 16 and f32 outputs: two kPair tiles on the same K/V fragments.
+#include <algorithm>
+#include <climits>
+
+#include "batch_internal.cuh"
+
+namespace sf37kv {
+
+extern unsigned long long g_launches;
+
+enum { kPair = 0, kWide = 1, kTwo = 2 };
+
+constexpr float kSlack = 8.0f;
+constexpr int kWarps = 4;
+constexpr uint32_t kThreads = kWarps * 32;
+constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
+constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
+constexpr uint32_t kMergePass = 32;    // partials joined per pass
+// Range of the weights' power of two (kernel below): the ratio of two is finite.
+constexpr int kFMin = -86, kFMax = 40;
+
+struct SeqDev {
+    const void *k, *v, *q;
+    const float *gate;
+    void *out;
+    const void *k_new, *v_new;
+    uint32_t start, end, cap;            // own rows [start, end)
+    uint32_t split_rows, n_splits, cta_begin;
+    // partials of the shared prefix: tile pre_tile + kvh * pre_kvh + split, row pre_row on
+    uint32_t pre_tile, pre_kvh, pre_splits, pre_row;
+};
+__host__ __device__ constexpr uint32_t part_stride(uint32_t g) { return g * 128u + ((2u * g + 3u) & ~3u); }
+
+template <int NJ>
+struct BatchParams {
+    SeqDev seq[NJ];
+    uint32_t n, group, kv_heads, bf16;
+    float *part;          // [cta][part_stride(G)]: O [G][128], then (m, l) [G]
+    uint32_t *counters;   // [sequence][kv head]
+    const float *pre_part, *pre_ml;
+};
+
+// ------------------------------------------------------------ device helpers
+namespace bd {
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ float2 lds64f(uint32_t addr) {
+    float2 r;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4 &u, int w) {
+    return w == 0 ? u.x : w == 1 ? u.y : w == 2 ? u.z : u.w;
+}
+// Two bytes u (in the low and high half's low byte of an 0x64uu pair) to f16
+// u - 128: 0x6400 + u is the f16 1024 + u, and 1152 is subtracted exactly.
+__device__ __forceinline__ uint32_t unbias(uint32_t h) {
+    const uint32_t bias = 0x64806480u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2 *>(&h), *reinterpret_cast<const __half2 *>(&bias));
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) { return unbias(prmt(w, 0x64646464u, 0x4140u)); }
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return unbias(prmt(w, 0x64646464u, 0x4342u)); }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint64_t pol) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 2^-e for a positive f32 x in [2^e, 2^(e+1)), e clamped to [-126, 126].
+__device__ __forceinline__ float pow2_below(float x, int &e) {
+    e = (int)((__float_as_uint(x) >> 23) & 255u) - 127;
+    e = max(-126, min(126, e));
+    return __int_as_float((127 - e) << 23);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+
+// Float index of dimension d of row `row` in the merge buffer: 16-byte chunks
+// permuted so that the fragment stores spread over the banks and float4 reads
+// stay whole.
+__device__ __forceinline__ uint32_t os_at(uint32_t row, uint32_t d) {
+    const uint32_t c = d >> 2;
+    return row * 128u + ((c ^ (row & 7u) ^ ((c >> 3) & 3u)) << 2) + (d & 3u);
+}
+__device__ __forceinline__ void store_out4(void *out, uint64_t i, float4 x, bool bf16) {
+    if (!bf16) {
+        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(out) + i) = x;
+        return;
+    }
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+    uint2 w;
+    w.x = *reinterpret_cast<const uint32_t *>(&a);
+    w.y = *reinterpret_cast<const uint32_t *>(&b);
+    *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(out) + i) = w;
+}
+__device__ __forceinline__ float4 normalise(float4 a, float l, float g) {
+    if (l == 0.f) return make_float4(0.f, 0.f, 0.f, 0.f);  // no row attended to
+    return make_float4(a.x / l * g, a.y / l * g, a.z / l * g, a.w / l * g);
+}
+
+}  // namespace bd
+
+// ------------------------------------------------------------ the stage
+// One stage: 16 rows of K, 16 of V (I8: then 16 + 16 scales).  16-byte chunk ch
+// of row r sits at ch ^ k_swz(r) (K) or ch ^ v_swz(r) (V), which keeps the
+// eight lanes of a load phase on distinct banks:
+//   K: lane (g, t) reads row g (+8), chunk t + 4c; V: rows 2t + {0,1,8,9}, chunk g (+8).
+template <bool I8>
+struct Stage {
+    static constexpr uint32_t kRow = I8 ? 128 : 256;
+    static constexpr uint32_t kV = 16 * kRow;
+    static constexpr uint32_t kScales = 32 * kRow;
+    static constexpr uint32_t kBytes = 32 * kRow + (I8 ? 128 : 0);
+    static constexpr int kStages = I8 ? 6 : 3;
+    static __device__ __forceinline__ uint32_t k_swz(uint32_t r) {
+        return I8 ? (r & 1u) << 2 : ((r & 1u) << 2) ^ (((r >> 1) & 3u) << 1);
+    }
+    static __device__ __forceinline__ uint32_t v_swz(uint32_t r) {
+        return I8 ? ((r >> 1) & 3u) << 1 : ((r & 1u) << 2) ^ (((r >> 1) & 3u) << 1);
+    }
+    // Dimension of element e (0..3) that lane t holds in k-step kk: the order
+    // inside a head is permuted so that the loaded words are the fragments.
+    static __device__ __forceinline__ uint32_t k_dim(uint32_t kk, uint32_t t, uint32_t e) {
+        if (I8) return 64u * (kk >> 2) + 16u * t + 4u * (kk & 3u) + e;
+        const uint32_t w = 2u * kk + (e >> 1);
+        return (4u * (w >> 2) + t) * 8u + 2u * (w & 3u) + (e & 1u);
+    }
+    // Dimension of column c (0..7) of output tile jt.
+    static __device__ __forceinline__ uint32_t v_dim(uint32_t jt, uint32_t c) {
+        return I8 ? 16u * c + jt : jt < 8 ? 8u * c + jt : 64u + 8u * c + jt - 8u;
+    }
+};
+
+template <bool I8>
+constexpr size_t batch_smem(int tiles) {
+    return (size_t)kWarps * Stage<I8>::kStages * Stage<I8>::kBytes + (size_t)tiles * 8 * 32 * 16;
+}
+
+template <int MODE, bool I8, int NJ>
+__global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_constant__ BatchParams<NJ> P) {
+    using namespace bd;
+    using St = Stage<I8>;
+    constexpr int NT = MODE == kTwo ? 2 : 1;   // M tiles
+    constexpr int NH = MODE == kPair ? 1 : 2;  // heads of a lane
+    constexpr int S = St::kStages;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float qfac[16], gate_s[16];
+    __shared__ float mw[kMergePass * 16], mM[16], mScale[16], mL[16];
+    __shared__ uint32_t s_last;
+
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
+    uint32_t lo = 0, hi = P.n;  // the sequence whose CTAs hold blockIdx.x
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (P.seq[mid].cta_begin <= blockIdx.x) lo = mid;
+        else hi = mid;
+    }
+    const SeqDev &J = P.seq[lo];
+    const uint32_t G = P.group, local = blockIdx.x - J.cta_begin;
+    const uint32_t kvh = local / J.n_splits, split = local - kvh * J.n_splits;
+    const uint32_t row0 = J.start + split * J.split_rows;
+    const uint32_t row1 = min(row0 + J.split_rows, J.end);
+    const uint64_t row_bytes = (uint64_t)P.kv_heads * St::kRow;
+    const uint8_t *kbase = reinterpret_cast<const uint8_t *>(J.k), *vbase = reinterpret_cast<const uint8_t *>(J.v);
+    const float *sbase = reinterpret_cast<const float *>((lane < 16 ? kbase : vbase) + row_bytes * J.cap) +
+                         (uint64_t)kvh * J.cap;
+    const uint32_t wbuf = (uint32_t)__cvta_generic_to_shared(smem) + warp * S * St::kBytes;
+    uint4 *Qs = reinterpret_cast<uint4 *>(smem + kWarps * S * St::kBytes);  // [tile][kk][lane]
+
+    // The CTA that covers the last row stores the appended one first: K by
+    // warp 0, V by warp 1.
+    if (J.k_new && row0 < row1 && row1 == J.end) {
+        if (warp < 2) {
+            uint8_t *cache = const_cast<uint8_t *>(warp ? vbase : kbase);
+            const float4 x = load_row4(warp ? J.v_new : J.k_new, kvh * 128u + lane * 4u, P.bf16);
+            const uint32_t slot = (J.end - 1u) % J.cap;
+            if (I8) {
+                store_i8_head(cache, J.cap, P.kv_heads, kvh, slot, lane, x);
+            } else {
+                uint2 w;
+                w.x = h2_bits(x.x, x.y);
+                w.y = h2_bits(x.z, x.w);
+                *reinterpret_cast<uint2 *>(cache + slot * row_bytes + kvh * 256u + lane * 8u) = w;
+            }
+        }
+        __syncthreads();
+    }
+
+    const uint32_t b_first = row0 + warp * 16u;
+    constexpr uint32_t kStep = kWarps * 16;
+    const uint32_t nblk = b_first < row1 ? (row1 - b_first + kStep - 1) / kStep : 0u;
+    uint64_t pol;  // a step reads more than L2 holds: the stream is marked to leave first
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
+    auto issue = [&](uint32_t it) {
+        if (it < nblk) {
+            const uint32_t bb = b_first + it * kStep, sb = bb % J.cap, st = wbuf + (it % S) * St::kBytes;
+            constexpr uint32_t kCh = St::kRow / 16;
+#pragma unroll
+            for (uint32_t i = 0; i < kCh / 2; i++) {
+                const uint32_t c = lane + 32u * i, r = c / kCh, ch = c % kCh;
+                uint32_t slot = sb + r;
+                if (slot >= J.cap) slot %= J.cap;
+                if (bb + r >= row1) slot = sb;  // past the end: a row that is read anyway, masked below
+                const uint64_t go = slot * row_bytes + kvh * St::kRow + ch * 16u;
+                cp16(st + r * St::kRow + ((ch ^ St::k_swz(r)) << 4), kbase + go, pol);
+                cp16(st + St::kV + r * St::kRow + ((ch ^ St::v_swz(r)) << 4), vbase + go, pol);
+            }
+            if (I8) {
+                const uint32_t r = lane & 15u;
+                uint32_t slot = sb + r;
+                if (slot >= J.cap) slot %= J.cap;
+                if (bb + r >= row1) slot = sb;
+                cp4(st + St::kScales + lane * 4u, sbase + slot);
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < S - 1; s++) issue(s);
+
+    // q: scaled by a power of two for each head so that its largest element is
+    // in [1, 2) (f16 then holds a bf16 q exactly, and 22 bits of an f32 one).
+    if (warp < NT) {
+        const uint32_t h0 = warp * 8u + g;
+        float qv[MODE == kWide ? 2 : 1][8][4];
+#pragma unroll
+        for (int x = 0; x < (MODE == kWide ? 2 : 1); x++) {
+            const uint32_t h = h0 + 8u * x;
+            float top = 0.f;
+#pragma unroll
+            for (uint32_t kk = 0; kk < 8; kk++)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) {
+                    const uint64_t i = (uint64_t)(kvh * G + min(h, G - 1u)) * 128u + St::k_dim(kk, t, e);
+                    const float q = P.bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(J.q)[i] << 16)
+                                           : reinterpret_cast<const float *>(J.q)[i];
+                    qv[x][kk][e] = h < G ? q : 0.f;
+                    top = fmaxf(top, fabsf(qv[x][kk][e]));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e2;
+            const float f = pow2_below(top, e2);
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) qv[x][kk][e] *= f;
+            if (t == 0 && h < 16) qfac[h] = pow2(e2) * (1.4426950408889634f * 0.08838834764831845f);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++) {
+            uint32_t a[4];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const float x0 = qv[0][kk][2 * half], x1 = qv[0][kk][2 * half + 1];
+                const __half2 hv = __floats2half2_rn(x0, x1);
+                a[2 * half] = *reinterpret_cast<const uint32_t *>(&hv);
+                if (MODE == kWide) {
+                    constexpr int kB = MODE == kWide ? 1 : 0;
+                    a[2 * half + 1] = h2_bits(qv[kB][kk][2 * half], qv[kB][kk][2 * half + 1]);
+                } else {
+                    const float2 f = __half22float2(hv);
+                    a[2 * half + 1] = h2_bits(x0 - f.x, x1 - f.y);
+                }
+            }
+            Qs[(warp * 8 + kk) * 32 + lane] = make_uint4(a[0], a[1], a[2], a[3]);
+        }
+    }
+    if (tid < 16) gate_s[tid] = tid < G && J.gate ? sigmoid_dev(J.gate[kvh * G + tid]) : 1.f;
+    __syncthreads();
+    float qf[NH];
+#pragma unroll
+    for (int h = 0; h < NH; h++) qf[h] = qfac[g + 8u * h];
+    const uint32_t qaddr = (uint32_t)__cvta_generic_to_shared(Qs + lane);
+
+    float o[NT][16][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    // Per head: reference m, sum l, and f, a power of two that brings the
+    // weights p * (value scale) into f16's range: the largest is kept in
+    // [2^7, 2^15], so weights down to 2^-32 of it are held (value scales from
+    // 2^-40 to 2^100; smaller ones lose bits, larger ones overflow).
+    float m[NH], l[NH], f[NH];
+#pragma unroll
+    for (int h = 0; h < NH; h++) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+        f[h] = I8 ? pow2(kFMax) : 128.f;
+    }
+
+    for (uint32_t it = 0; it < nblk; it++) {
+        cp_wait<S - 2>();
+        __syncwarp();
+        issue(it + S - 1);
+        const uint32_t b = b_first + it * kStep, st = wbuf + (it % S) * St::kBytes;
+
+        float s[NT][2][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < (I8 ? 2 : 4); c++) {
+            uint4 u[2];
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) {
+                const uint32_t r = 8u * i + g;
+                u[i] = lds128(st + r * St::kRow + (((4u * c + t) ^ St::k_swz(r)) << 4));
+            }
+#pragma unroll
+            for (int w = 0; w < (I8 ? 4 : 2); w++) {
+                const int kk = c * (I8 ? 4 : 2) + w;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const uint4 q4 = lds128(qaddr + (n * 8 + kk) * 512);
+                    const uint32_t a[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (I8) mma(s[n][i], a, codes_lo(word(u[i], w)), codes_hi(word(u[i], w)));
+                        else mma(s[n][i], a, word(u[i], 2 * w), word(u[i], 2 * w + 1));
+                    }
+                }
+            }
+        }
+
+        // scores of the lane's keys 8i + 2t + e; the value scales of the same
+        float sc[NH][2][2], vs[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float2 ks = make_float2(1.f, 1.f), v2 = make_float2(1.f, 1.f);
+            if (I8) {
+                ks = lds64f(st + St::kScales + (8u * i + 2u * t) * 4u);
+                v2 = lds64f(st + St::kScales + 64u + (8u * i + 2u * t) * 4u);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const bool live = b + 8u * i + 2u * t + e < row1;
+                const float k = e ? ks.y : ks.x;
+                vs[i][e] = live ? (e ? v2.y : v2.x) : 0.f;
+#pragma unroll
+                for (int h = 0; h < NH; h++) {
+                    const float x = MODE == kWide ? s[0][i][e + 2 * h] : s[h % NT][i][e] + s[h % NT][i][e + 2];
+                    sc[h][i][e] = live ? x * (qf[h] * k) : -INFINITY;
+                }
+            }
+        }
+        float p[NH][2][2], w[NH][2][2];
+        bool need[NH];
+        auto weigh = [&](int h) {
+            const float mu = m[h] == -INFINITY ? 0.f : m[h];
+            float xm = -INFINITY, wm = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float x = sc[h][i][e] - mu;
+                    xm = fmaxf(xm, x);
+                    p[h][i][e] = fast_exp2(x);
+                    w[h][i][e] = I8 ? p[h][i][e] * (vs[i][e] * f[h]) : p[h][i][e] * f[h];
+                    wm = fmaxf(wm, w[h][i][e]);
+                }
+            need[h] = xm > kSlack || (m[h] == -INFINITY && xm > -INFINITY) || (I8 && wm > 32768.f);
+        };
+        bool any = false;
+#pragma unroll
+        for (int h = 0; h < NH; h++) {
+            weigh(h);
+            any |= need[h];
+        }
+        if (__any_sync(0xffffffffu, any)) {
+            float fac[NH];
+#pragma unroll
+            for (int h = 0; h < NH; h++) {
+                uint32_t nd = need[h];
+                nd |= __shfl_xor_sync(0xffffffffu, nd, 1);
+                nd |= __shfl_xor_sync(0xffffffffu, nd, 2);
+                float mx = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                fac[h] = 1.f;
+                const float mn = nd ? fmaxf(m[h], mx) : m[h];
+                if (nd) {
+                    const float alpha = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - mn);
+                    l[h] *= alpha;
+                    fac[h] = alpha;
+                    m[h] = mn;
+                }
+                if (I8) {
+                    const float mu = mn == -INFINITY ? 0.f : mn;
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) top = fmaxf(top, fast_exp2(sc[h][i][e] - mu) * vs[i][e]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (nd) {
+                        int e2;
+                        pow2_below(top, e2);
+                        const float fn = pow2(max(kFMin, min(kFMax, 7 - e2)));
+                        fac[h] *= fn / f[h];
+                        f[h] = fn;
+                    }
+                }
+                weigh(h);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[n][i][e] *= MODE == kWide ? fac[(e >> 1) % NH] : fac[n % NH];
+        }
+        uint32_t pa[NT][4];
+#pragma unroll
+        for (int h = 0; h < NH; h++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                l[h] += p[h][i][0] + p[h][i][1];
+                const __half2 hv = __floats2half2_rn(w[h][i][0], w[h][i][1]);
+                const uint32_t hb = *reinterpret_cast<const uint32_t *>(&hv);
+                if (MODE == kWide) {
+                    pa[0][2 * i + h] = hb;
+                } else {
+                    const float2 b2 = __half22float2(hv);
+                    pa[h % NT][2 * i] = hb;
+                    pa[h % NT][2 * i + 1] = h2_bits(w[h][i][0] - b2.x, w[h][i][1] - b2.y);
+                }
+            }
+
+        // O += P V: rows 2t, 2t+1 (B register 0) and 2t+8, 2t+9 (B register 1)
+        const uint32_t vt = st + St::kV;
+        if (I8) {
+            uint4 v[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const uint32_t r = 2u * t + (x & 1) + (x >> 1) * 8u;
+                v[x] = lds128(vt + r * St::kRow + ((g ^ St::v_swz(r)) << 4));
+            }
+#pragma unroll
+            for (int wd = 0; wd < 4; wd++) {
+#pragma unroll
+                for (int hf = 0; hf < 2; hf++) {
+                    const uint32_t sel = hf ? 0x7362u : 0x5140u;  // {a2,b2,a3,b3} or {a0,b0,a1,b1}
+                    const uint32_t x = prmt(word(v[0], wd), word(v[1], wd), sel);
+                    const uint32_t y = prmt(word(v[2], wd), word(v[3], wd), sel);
+                    const uint32_t x0 = codes_lo(x), x1 = codes_hi(x), y0 = codes_lo(y), y1 = codes_hi(y);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        mma(o[n][4 * wd + 2 * hf], pa[n], x0, y0);
+                        mma(o[n][4 * wd + 2 * hf + 1], pa[n], x1, y1);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                uint4 v[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const uint32_t r = 2u * t + (x & 1) + (x >> 1) * 8u;
+                    v[x] = lds128(vt + r * St::kRow + (((g + 8u * u) ^ St::v_swz(r)) << 4));
+                }
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+                    const uint32_t b0 = prmt(word(v[0], e >> 1), word(v[1], e >> 1), sel);
+                    const uint32_t b1 = prmt(word(v[2], e >> 1), word(v[3], e >> 1), sel);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) mma(o[n][8 * u + e], pa[n], b0, b1);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    cp_wait<0>();
+    __syncthreads();  // the stages become the merge buffer
+
+    // ---- the four warps' states to one ----
+    float *Os = reinterpret_cast<float *>(smem);  // [warp*16 + head][128]
+    float *Ms = Os + kWarps * 16 * 128, *Ls = Ms + kWarps * 16, *W = Ls + kWarps * 16, *PM = W + kWarps * 16,
+          *PL = PM + 16;
+#pragma unroll
+    for (int h = 0; h < NH; h++) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const uint32_t row = warp * 16u + g + 8u * h;
+        const float inv = 1.f / f[h];
+#pragma unroll
+        for (uint32_t jt = 0; jt < 16; jt++)
+#pragma unroll
+            for (uint32_t e = 0; e < 2; e++) {
+                const float x = MODE == kWide ? o[0][jt][e + 2 * h] : o[h % NT][jt][e] + o[h % NT][jt][e + 2];
+                Os[os_at(row, St::v_dim(jt, 2u * t + e))] = x * inv;
+            }
+        if (t == 0) {
+            Ms[row] = m[h];
+            Ls[row] = l[h];
+        }
+    }
+    __syncthreads();
+    if (tid < G) {
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) M = fmaxf(M, Ms[s * 16 + tid]);
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) {
+            // a state whose only scores were NaN has m = -inf and l = NaN: its weight is 1, so that NaN stays
+            const float ms = Ms[s * 16 + tid], ls = Ls[s * 16 + tid];
+            const float w = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : fast_exp2(ms - M);
+            W[s * 16 + tid] = w;
+            L += ls * w;
+        }
+        PM[tid] = M;
+        PL[tid] = L;
+    }
+    __syncthreads();
+    const bool single = J.n_splits == 1 && J.pre_splits == 0;
+    const uint32_t stride = part_stride(G);
+    float *part = P.part + (uint64_t)blockIdx.x * stride;
+    const uint64_t out0 = (uint64_t)kvh * G * 128u;
+    for (uint32_t idx = tid; idx < G * 32u; idx += kThreads) {
+        const uint32_t h = idx >> 5, d4 = (idx & 31u) * 4u;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int s = 0; s < kWarps; s++) {
+            const float w = W[s * 16 + h];
+            const float4 x = *reinterpret_cast<const float4 *>(Os + os_at(s * 16u + h, d4));
+            a.x = fmaf(x.x, w, a.x);
+            a.y = fmaf(x.y, w, a.y);
+            a.z = fmaf(x.z, w, a.z);
+            a.w = fmaf(x.w, w, a.w);
+        }
+        if (single) store_out4(J.out, out0 + idx * 4u, normalise(a, PL[h], gate_s[h]), P.bf16);
+        else __stcg(reinterpret_cast<float4 *>(part + idx * 4u), a);
+    }
+    // A shared prefix's partials come from the launch before this one, which
+    // this kernel may overlap until here (programmatic dependent launch).
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (single) return;
+    if (tid < G) __stcg(reinterpret_cast<float2 *>(part + G * 128u + 2u * tid), make_float2(PM[tid], PL[tid]));
+    __syncthreads();
+    uint32_t *ctr = P.counters + (uint64_t)lo * P.kv_heads + kvh;
+    if (tid == 0) {
+        uint32_t prev;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(prev) : "l"(ctr) : "memory");
+        s_last = prev == J.n_splits - 1u;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    if (tid == 0) *ctr = 0u;  // ready for the next call
+
+    // ---- the last CTA joins all partials of (sequence, KV head) ----
+    const uint32_t n_src = J.n_splits + J.pre_splits;
+    const float *own = P.part + (uint64_t)(J.cta_begin + kvh * J.n_splits) * stride;
+    const uint64_t tile0 = (uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh;
+    // the partials land in the stages, their (m, l) pairs where q was
+    const uint32_t land = (uint32_t)__cvta_generic_to_shared(smem), ml_land = (uint32_t)__cvta_generic_to_shared(Qs);
+    const float *ml_s = reinterpret_cast<const float *>(Qs);
+    static_assert(kMergePass * 32 * 4 <= 8 * 32 * 16, "(m, l) pairs of a pass");
+    constexpr uint32_t kStageArea = kWarps * S * St::kBytes;
+    const uint32_t per = min(kMergePass, kStageArea / (G * 512u));
+    if (tid < 16) {
+        mM[tid] = -INFINITY;
+        mL[tid] = 0.f;
+    }
+    constexpr int kPer = 4;  // float4 outputs of a thread, G <= 16
+    float4 acc[kPer];
+#pragma unroll
+    for (int k = 0; k < kPer; k++) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < n_src; s0 += per) {
+        const uint32_t cnt = min(per, n_src - s0);
+        for (uint32_t s = 0; s < cnt; s++) {
+            const uint32_t x = s0 + s;
+            const float *po, *pm;
+            if (x < J.n_splits) {
+                po = own + (uint64_t)x * stride;
+                pm = po + G * 128u;
+            } else {
+                const uint64_t row = (tile0 + (x - J.n_splits)) * 128u + J.pre_row;
+                po = P.pre_part + row * 128u;
+                pm = P.pre_ml + row * 2u;
+            }
+            for (uint32_t idx = tid; idx < G * 32u; idx += kThreads) cp16(land + s * G * 512u + idx * 16u, po + idx * 4u);
+            if (tid < 2u * G) cp4(ml_land + (s * 32u + tid) * 4u, pm + tid);
+        }
+        cp_commit();
+        cp_wait<0>();
+        __syncthreads();
+        for (uint32_t h = warp; h < G; h += kWarps) {
+            float ms = -INFINITY, ls = 0.f;
+            if (lane < cnt) {
+                ms = ml_s[lane * 32u + 2u * h];
+                ls = ml_s[lane * 32u + 2u * h + 1u];
+            }
+            const float mo = mM[h];
+            float M = fmaxf(ms, mo);
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+            const float w = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : fast_exp2(ms - M);
+            float L = ls * w;
+#pragma unroll
+            for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
+            mw[lane * 16u + h] = w;
+            __syncwarp();
+            if (lane == 0) {
+                const float sc = mo == -INFINITY ? (mL[h] == 0.f ? 0.f : 1.f) : fast_exp2(mo - M);
+                mScale[h] = sc;
+                mL[h] = mL[h] * sc + L;
+                mM[h] = M;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kPer; k++) {
+            const uint32_t idx = tid + (uint32_t)k * kThreads;
+            if (idx < G * 32u) {
+                const uint32_t h = idx >> 5;
+                const float sc = mScale[h];
+                float4 a = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
+#pragma unroll 4
+                for (uint32_t s = 0; s < cnt; s++) {
+                    const float w = mw[s * 16u + h];
+                    const float4 x = *reinterpret_cast<const float4 *>(smem + (s * G * 32u + idx) * 16u);
+                    a.x = fmaf(x.x, w, a.x);
+                    a.y = fmaf(x.y, w, a.y);
+                    a.z = fmaf(x.z, w, a.z);
+                    a.w = fmaf(x.w, w, a.w);
+                }
+                acc[k] = a;
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; k++) {
+        const uint32_t idx = tid + (uint32_t)k * kThreads;
+        if (idx < G * 32u) store_out4(J.out, out0 + idx * 4u, normalise(acc[k], mL[idx >> 5], gate_s[idx >> 5]), P.bf16);
+    }
+}
+
+// ------------------------------------------------------------ planning
+// Rows of a split.  Two CTAs fit an SM, so 296 run at once.  A launch whose
+// CTAs can each take all of their share in one wave of at most kWaveRows rows does so
+// (fewest partials); more work is cut into about kWaves waves, whose ends even out.
+constexpr uint32_t kResident = 2 * kPlanSms, kWaves = 8;
+constexpr uint32_t kUnit = kWarps * 16;  // rows that the warps of a CTA take at once
+
+static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint32_t rows) {
+    uint64_t c = 0;
+    for (uint32_t i = 0; i < n; i++) c += std::max(1u, (seqs[i].end - seqs[i].start + rows - 1) / rows);
+    return c;
+}
+
+static uint32_t plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads) {
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < n; i++) total += seqs[i].end - seqs[i].start;
+    const uint64_t per_wave = (total * kv_heads + kResident - 1) / kResident;  // rows of a CTA in one wave
+    uint64_t rows;
+    if (per_wave <= 2048) {
+        rows = std::max<uint64_t>(1, (per_wave + kUnit - 1) / kUnit) * kUnit;
+        if ((uint64_t)n * kv_heads <= kResident)
+            while (plan_ctas(seqs, n, (uint32_t)rows) * kv_heads > kResident) rows += std::max<uint64_t>(1, rows / (16 * kUnit)) * kUnit;
+    } else {
+        rows = std::max<uint64_t>(1024, (total * kv_heads + kResident * kWaves - 1) / (kResident * kWaves));
+        rows = (rows + kUnit - 1) / kUnit * kUnit;
+    }
+    uint32_t ctas = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        SeqDev &J = seqs[i];
+        const uint32_t len = J.end - J.start;
+        J.n_splits = std::max<uint32_t>(1u, (uint32_t)((len + rows - 1) / rows));
+        // even splits, whole units
+        J.split_rows = std::max<uint32_t>(kUnit, ((len + J.n_splits - 1) / J.n_splits + kUnit - 1) / kUnit * kUnit);
+        J.cta_begin = ctas;
+        ctas += J.n_splits * kv_heads;
+    }
+    return ctas;
+}
+
+// Sequences of a launch: the counters bound them with many KV heads.
+static uint32_t seqs_per_launch(uint32_t kv_heads) {
+    return (uint32_t)std::min<uint64_t>(kMaxSeqs, kCounters / kv_heads);
+}
+
+// Workspace: counters, own partials, prefix partial tiles, their (max, sum) pairs.
+struct Layout {
+    uint64_t part, pre, ml, bytes;
+};
+static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads, bool shared) {
+    const uint64_t n = std::min<uint64_t>(n_seqs, seqs_per_launch(kv_heads)), g = std::min<uint64_t>(n_groups, kPrefixGroups);
+    // plan_splits() cuts at most kResident * kWaves CTAs beyond one for each (sequence, KV head)
+    const uint64_t ctas = n * kv_heads + kResident * kWaves;
+    const uint64_t tiles = shared ? prefix_tiles_bound(g, n, q_heads, kv_heads) : 0;
+    Layout w;
+    w.part = kCounters * 4u;
+    w.pre = (w.part + ctas * part_stride(q_heads / kv_heads) * 4u + 255u) / 256u * 256u;
+    w.ml = w.pre + tiles * 128u * 128u * 4u;
+    w.bytes = w.ml + tiles * 128u * 2u * 4u;
+    return w;
+}
+
+// ------------------------------------------------------------ launches
+template <int MODE, bool I8, int NJ>
+static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
+                  cudaStream_t stream) {
+    constexpr size_t smem = batch_smem<I8>(MODE == kTwo ? 2 : 1);
+    static bool ready[64];
+    int dev = 0;
+    if (int rc = check_cuda(cudaGetDevice(&dev), "decode get device")) return rc;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        if (int rc = check_cuda(cudaFuncSetAttribute(batch_decode_kernel<MODE, I8, NJ>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                "decode shared memory"))
+            return rc;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    BatchParams<NJ> P;
+    std::copy(seqs, seqs + n, P.seq);
+    P.n = n;
+    P.group = head.group;
+    P.kv_heads = head.kv_heads;
+    P.bf16 = head.bf16;
+    P.part = head.part;
+    P.counters = head.counters;
+    P.pre_part = head.pre_part;
+    P.pre_ml = head.pre_ml;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    // After a prefix launch the CTAs start as its CTAs leave, and stream their own
+    // rows meanwhile; every CTA waits for that launch before it reads its
+    // partials.  This kernel lets nothing start before its own end.
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = after_prefix ? 1 : 0;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, NJ>, P);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    g_launches++;
+    return check_cuda(e, "decode launch");
+}
+
+template <int MODE, bool I8>
+static int launch_n(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
+                    cudaStream_t stream) {
+    // The descriptors travel as kernel parameters; a small launch carries few.
+    return n <= kSmallSeqs ? launch<MODE, I8, kSmallSeqs>(seqs, n, ctas, head, after_prefix, stream)
+                           : launch<MODE, I8, kMaxSeqs>(seqs, n, ctas, head, after_prefix, stream);
+}
+
+template <bool I8>
+static int launch_mode(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
+                       cudaStream_t stream) {
+    if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, ctas, head, after_prefix, stream);
+    if (head.bf16) return launch_n<kWide, I8>(seqs, n, ctas, head, after_prefix, stream);
+    return launch_n<kTwo, I8>(seqs, n, ctas, head, after_prefix, stream);
+}
+
+static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, uint32_t prefix_len, bool ring_clamp) {
+    if (int rc = check_cache(what, i, L.cache)) return rc;
+    if (!L.q || !L.out || !aligned16(L.q) || !aligned16(L.out))
+        return set_error(SF37KV_EINVAL, "%s: sequence %u q and out must be non-NULL and 16-byte aligned", what, i);
+    if ((L.k_new != nullptr) != (L.v_new != nullptr))
+        return set_error(SF37KV_EINVAL, "%s: sequence %u has only one of k_new/v_new", what, i);
+    if (!aligned16(L.k_new) || !aligned16(L.v_new) || ((uintptr_t)L.gate & 3u))
+        return set_error(SF37KV_EINVAL, "%s: sequence %u k_new/v_new must be 16-byte and gate 4-byte aligned", what, i);
+    if (L.pos >= kMaxPos) return set_error(SF37KV_EINVAL, "%s: sequence %u position %u exceeds %u", what, i, L.pos, kMaxPos);
+    if (ring_clamp) return SF37KV_OK;
+    const uint32_t have = L.pos + 1u;
+    if (have < prefix_len)
+        return set_error(SF37KV_EINVAL, "%s: sequence %u position %u is inside the prefix of %u", what, i, L.pos, prefix_len);
+    if (L.k_new && have == prefix_len)
+        return set_error(SF37KV_EINVAL, "%s: sequence %u appends at position %u, which is the prefix's", what, i, L.pos);
+    uint32_t first = L.cache.sliding && have > L.cache.window ? have - L.cache.window : 0u;
+    if (first < prefix_len) first = prefix_len;
+    if (have > first && have - first > L.cache.cap)
+        return set_error(SF37KV_EINVAL, "%s: sequence %u attends to %u own rows, its cache holds %u", what, i, have - first,
+                         L.cache.cap);
+    return SF37KV_OK;
+}
+
+// A cache that is appended to and given twice, among n sequences.
+static bool append_conflict(const sf37kv_decode_seq *const *seqs, uint32_t n) {
+    struct Item {
+        const void *p;
+        bool writes;
+    } items[2 * kMaxSeqs];
+    bool any = false;
+    for (uint32_t i = 0; i < n; i++) {
+        const bool w = seqs[i]->k_new != nullptr;
+        any |= w;
+        items[2 * i] = Item{seqs[i]->cache.k_cache, w};
+        items[2 * i + 1] = Item{seqs[i]->cache.v_cache, w};
+    }
+    if (!any) return false;
+    std::sort(items, items + 2 * n, [](const Item &a, const Item &b) { return a.p != b.p ? a.p < b.p : a.writes > b.writes; });
+    for (uint32_t i = 1; i < 2 * n; i++)
+        if (items[i].p == items[i - 1].p && items[i - 1].writes) return true;
+    return false;
+}
+
+// Decode of all groups; ring_clamp (sf37kv_decode_i8): no prefixes, and a full cache's
+// oldest rows drop out as in sf37kv_decode.
+static int decode_groups(const char *what, const sf37kv_shared_group *groups, uint32_t n_groups, uint32_t q_heads,
+                         uint32_t kv_heads, uint32_t head_dim, int dtype, int io_type, void *workspace,
+                         uint64_t workspace_bytes, bool ring_clamp, cudaStream_t stream) {
+    if (int rc = check_heads(what, q_heads, kv_heads, head_dim)) return rc;
+    if (dtype != SF37KV_F16 && dtype != SF37KV_I8)
+        return set_error(SF37KV_EUNSUPPORTED, "%s: cache dtype %d is neither f16 nor i8", what, dtype);
+    if (io_type != SF37KV_Q_F32 && io_type != SF37KV_Q_BF16)
+        return set_error(SF37KV_EINVAL, "%s: unknown io type %d", what, io_type);
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < n_groups; i++) {
+        const sf37kv_shared_group &Gr = groups[i];
+        if (Gr.n_seqs == 0) continue;
+        if (!Gr.seqs) return set_error(SF37KV_EINVAL, "%s: group %u has no sequences array", what, i);
+        if (Gr.prefix_len) {
+            if (int rc = check_cache(what, i, Gr.prefix)) return rc;
+            if (Gr.prefix_len > Gr.prefix.cap)
+                return set_error(SF37KV_EINVAL, "%s: group %u prefix of %u rows exceeds its cache of %u", what, i,
+                                 Gr.prefix_len, Gr.prefix.cap);
+        }
+        for (uint32_t k = 0; k < Gr.n_seqs; k++) {
+            const sf37kv_decode_seq &L = Gr.seqs[k];
+            if (int rc = check_seq(what, k, L, Gr.prefix_len, ring_clamp)) return rc;
+            if (Gr.prefix_len && L.k_new &&
+                (L.cache.k_cache == Gr.prefix.k_cache || L.cache.v_cache == Gr.prefix.v_cache))
+                return set_error(SF37KV_EINVAL, "%s: sequence %u appends to its prefix's cache", what, k);
+        }
+        total += Gr.n_seqs;
+    }
+    if (total == 0) return SF37KV_OK;
+    const Layout W = layout(n_groups, total, q_heads, kv_heads, !ring_clamp);
+    if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < W.bytes)
+        return set_error(SF37KV_EINVAL, "%s: the workspace must be 256-byte aligned and hold %llu bytes", what,
+                         (unsigned long long)W.bytes);
+    char *ws = (char *)workspace;
+    BatchParams<1> head;
+    head.group = q_heads / kv_heads;
+    head.kv_heads = kv_heads;
+    head.bf16 = io_type == SF37KV_Q_BF16;
+    head.counters = (uint32_t *)ws;
+    head.part = (float *)(ws + W.part);
+    head.pre_part = (const float *)(ws + W.pre);
+    head.pre_ml = (const float *)(ws + W.ml);
+    const uint32_t most = seqs_per_launch(kv_heads), T = prefix_seqs_per_tile(head.group);
+    // Pass 0 forms the launches and checks them, pass 1 runs them.
+    for (int pass = 0; pass < 2; pass++) {
+        uint32_t gi = 0, k0 = 0;  // next group, and its next sequence
+        while (gi < n_groups) {
+            PrefixGroup pg[kPrefixGroups];
+            PrefixSeq ps[kMaxSeqs];
+            SeqDev sd[kMaxSeqs];
+            const sf37kv_decode_seq *src[kMaxSeqs];
+            uint32_t owner[kMaxSeqs];  // the sequence's prefix group, or n_pg
+            uint32_t n = 0, n_pg = 0;
+            while (gi < n_groups && n < most && n_pg < (uint32_t)kPrefixGroups) {
+                const sf37kv_shared_group &Gr = groups[gi];
+                const uint32_t take = std::min(Gr.n_seqs - k0, most - n);
+                PrefixGroup &X = pg[n_pg];
+                X = PrefixGroup{Gr.prefix.k_cache, Gr.prefix.v_cache, Gr.prefix_len, Gr.prefix_len, Gr.prefix.cap, n, take};
+                for (uint32_t k = 0; k < take; k++, n++) {
+                    const sf37kv_decode_seq &L = Gr.seqs[k0 + k];
+                    const uint32_t have = L.pos + 1u;
+                    uint32_t first = L.cache.sliding && have > L.cache.window ? have - L.cache.window : 0u;
+                    if (ring_clamp) first = start_at(L.pos, L.cache.cap, (int)L.cache.sliding, L.cache.window);
+                    ps[n] = PrefixSeq{L.q, std::min(first, Gr.prefix_len), 0};
+                    X.lo = std::min(X.lo, ps[n].start);
+                    SeqDev &J = sd[n];
+                    J = SeqDev{L.cache.k_cache, L.cache.v_cache, L.q, L.gate, L.out, L.k_new, L.v_new};
+                    J.start = std::min(std::max(first, Gr.prefix_len), have);
+                    J.end = have;
+                    J.cap = L.cache.cap;
+                    src[n] = &L;
+                    owner[n] = n_pg;
+                }
+                if (X.lo < X.len) n_pg++;
+                else for (uint32_t k = n - take; k < n; k++) owner[k] = UINT32_MAX;
+                k0 += take;
+                if (k0 == Gr.n_seqs) {
+                    gi++;
+                    k0 = 0;
+                }
+            }
+            if (n == 0) continue;
+            if (pass == 0) {
+                if (append_conflict(src, n))
+                    return set_error(SF37KV_EINVAL, "%s: a cache that one sequence appends to is given twice", what);
+                continue;
+            }
+            if (n_pg) prefix_plan(pg, n_pg, q_heads, kv_heads, !head.bf16);
+            for (uint32_t k = 0; k < n; k++) {
+                SeqDev &J = sd[k];
+                J.pre_tile = J.pre_kvh = J.pre_splits = J.pre_row = 0;
+                if (owner[k] == UINT32_MAX || ps[k].start >= pg[owner[k]].len) continue;
+                const PrefixGroup &X = pg[owner[k]];
+                const uint32_t i = k - X.seq0;
+                J.pre_tile = X.part0 + i / T * X.splits;
+                J.pre_kvh = X.m_tiles * X.splits;
+                J.pre_splits = X.splits;
+                J.pre_row = i % T * head.group;
+            }
+            const uint32_t ctas = plan_splits(sd, n, kv_heads);
+            if (n_pg)
+                if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
+                                              (float *)(ws + W.ml), stream))
+                    return rc;
+            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, ctas, head, n_pg > 0, stream)
+                                              : launch_mode<false>(sd, n, ctas, head, n_pg > 0, stream);
+            if (rc) return rc;
+        }
+    }
+    return SF37KV_OK;
+}
+
+}  // namespace sf37kv
+
+using namespace sf37kv;
+
+extern "C" uint64_t sf37kv_decode_i8_workspace(uint32_t n_seqs, uint32_t q_heads, uint32_t kv_heads) {
+    if (check_heads("decode_i8_workspace", q_heads, kv_heads, 128)) return 0;
+    return layout(1, n_seqs, q_heads, kv_heads, false).bytes;
+}
+
+extern "C" int sf37kv_decode_i8(const sf37kv_decode_seq *seqs, uint32_t n_seqs, uint32_t q_heads, uint32_t kv_heads,
+                                uint32_t head_dim, int io_type, void *workspace, uint64_t workspace_bytes,
+                                void *stream) {
+    if (!seqs && n_seqs) return set_error(SF37KV_EINVAL, "decode_i8: seqs is NULL");
+    sf37kv_shared_group one = {};
+    one.n_seqs = n_seqs;
+    one.seqs = seqs;
+    return decode_groups("decode_i8", &one, 1, q_heads, kv_heads, head_dim, SF37KV_I8, io_type, workspace,
+                         workspace_bytes, true, stream ? (cudaStream_t)stream : current_stream());
+}
+
+extern "C" uint64_t sf37kv_decode_shared_workspace(uint32_t n_groups, uint32_t n_seqs, uint32_t q_heads,
+                                                   uint32_t kv_heads) {
+    if (check_heads("decode_shared_workspace", q_heads, kv_heads, 128)) return 0;
+    return layout(n_groups, n_seqs, q_heads, kv_heads, true).bytes;
+}
+
+extern "C" int sf37kv_decode_shared(const sf37kv_shared_group *groups, uint32_t n_groups, uint32_t q_heads,
+                                    uint32_t kv_heads, uint32_t head_dim, int dtype, int io_type, void *workspace,
+                                    uint64_t workspace_bytes, void *stream) {
+    if (!groups && n_groups) return set_error(SF37KV_EINVAL, "decode_shared: groups is NULL");
+    return decode_groups("decode_shared", groups, n_groups, q_heads, kv_heads, head_dim, dtype, io_type, workspace,
+                         workspace_bytes, false, stream ? (cudaStream_t)stream : current_stream());
+}

@@ -1,0 +1,116 @@
+// Declarations shared by the int8 cache and the batched decode kernels
+// (cache_i8.cu, batch_decode.cu, prefix_tc05.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "kv_internal.cuh"
+
+namespace sf37kv {
+
+// Positions stay below 2^31 so that pos + 1 and slot sums fit 32 bits.
+constexpr uint32_t kMaxPos = 0x7fffffffu;
+constexpr uint64_t kMaxUnits = 0x7fffff00ull;  // grid size bound
+
+static inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
+
+// Head counts and head_dim that the kernels of this file family take.
+static inline int check_heads(const char *what, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim) {
+    if (kv_heads == 0 || q_heads == 0 || q_heads % kv_heads)
+        return set_error(SF37KV_EINVAL, "%s: %u query heads do not divide over %u KV heads", what, q_heads, kv_heads);
+    if (head_dim != 128) return set_error(SF37KV_EUNSUPPORTED, "%s: head_dim must be 128", what);
+    if (kv_heads > 4096) return set_error(SF37KV_EUNSUPPORTED, "%s: more than 4096 KV heads", what);
+    if (q_heads / kv_heads > 16)
+        return set_error(SF37KV_EUNSUPPORTED, "%s: more than 16 query heads for each KV head", what);
+    return SF37KV_OK;
+}
+
+static inline int check_cache(const char *what, uint32_t i, const sf37kv_cache &c) {
+    if (!c.k_cache || !c.v_cache || !aligned16(c.k_cache) || !aligned16(c.v_cache))
+        return set_error(SF37KV_EINVAL, "%s: cache %u must be non-NULL and 16-byte aligned", what, i);
+    if (c.cap == 0 || c.cap > kMaxPos) return set_error(SF37KV_EINVAL, "%s: cache %u has cap %u", what, i, c.cap);
+    if (c.k_cache == c.v_cache) return set_error(SF37KV_EINVAL, "%s: cache %u has one buffer for K and V", what, i);
+    return SF37KV_OK;
+}
+
+__device__ __forceinline__ uint32_t h2_bits(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Four consecutive elements of an f32 or bf16 array (16- or 8-byte aligned).
+__device__ __forceinline__ float4 load_row4(const void *p, uint64_t i, bool bf16) {
+    if (!bf16) return __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i));
+    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i));
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xffff0000u));
+}
+
+// The integer nearest to x / s, ties to even, decided exactly: x * (1/s) is at
+// most one off, and the remainder x - c*s is an exact f32 (a multiple of the
+// smaller of ulp(x), ulp(s) and at most 1.5 s), so comparing 2r with s is too.
+__device__ __forceinline__ int i8_code(float x, float s, float inv) {
+    int c = __float2int_rn(x * inv);
+    const float r = fmaf(-(float)c, s, x), r2 = r + r;
+    if (r2 > s || (r2 == s && (c & 1))) c++;
+    else if (-r2 > s || (-r2 == s && (c & 1))) c--;
+    return c;
+}
+
+// Quantises one head (four elements a lane, all 32 lanes) and stores its codes
+// and scale in slot `slot` of an I8 cache.
+__device__ __forceinline__ void store_i8_head(uint8_t *cache, uint32_t cap, uint32_t heads, uint32_t head, uint32_t slot,
+                                              uint32_t lane, float4 x) {
+    const bool finite = fabsf(x.x) <= 3.402823466e38f && fabsf(x.y) <= 3.402823466e38f &&
+                        fabsf(x.z) <= 3.402823466e38f && fabsf(x.w) <= 3.402823466e38f;
+    float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    float s = __fdiv_rn(a, 127.0f);
+    if (s < 1.17549435e-38f) s = 0.f;
+    if (!__all_sync(0xffffffffu, finite)) s = __int_as_float(0x7fc00000);
+    uint32_t w = 0x80808080u;  // zeros: also the codes of a NaN scale
+    if (s > 0.f) {
+        const float inv = __frcp_rn(s);
+        w = (uint32_t)(i8_code(x.x, s, inv) + 128) | ((uint32_t)(i8_code(x.y, s, inv) + 128) << 8) |
+            ((uint32_t)(i8_code(x.z, s, inv) + 128) << 16) | ((uint32_t)(i8_code(x.w, s, inv) + 128) << 24);
+    }
+    const uint64_t kv_dim = (uint64_t)heads * 128u;
+    *reinterpret_cast<uint32_t *>(cache + slot * kv_dim + head * 128u + lane * 4u) = w;
+    if (lane == 0) reinterpret_cast<float *>(cache + cap * kv_dim)[(uint64_t)head * cap + slot] = s;
+}
+
+// ------------------------------------------------------------ shared prefix
+constexpr int kPrefixGroups = 8;    // groups per prefix launch
+constexpr int kPrefixSeqs = 256;    // sequences per prefix launch
+constexpr uint32_t kPlanSms = 148;  // B200
+
+struct PrefixSeq {
+    const void *q;     // [q_heads][128]
+    uint32_t start;    // first prefix row that the sequence attends to
+    uint32_t pad;
+};
+// One group: all sequences over the rows [lo, len) of one f16 prefix cache.
+struct PrefixGroup {
+    const void *k, *v;
+    uint32_t lo, len, cap;
+    uint32_t seq0, n_seqs;      // its sequences in the launch's list
+    // filled by prefix_plan()
+    uint32_t m_tiles, splits, tiles_per_split;
+    uint32_t unit0;             // first (kv head, m tile) unit of the group
+    uint32_t part0;             // first partial tile of the group
+};
+
+// Sequences of one 128-row tile: row sl * G + hl holds head hl of sequence sl.
+static inline uint32_t prefix_seqs_per_tile(uint32_t group) { return 128u / group; }
+
+// Splits each group's rows over CTAs; returns the number of 128-row partial
+// tiles, each 128 x 128 f32 (unnormalised outputs) and 128 (max, sum) pairs.
+// Partial of (kv head h, m tile t, split s): part0 + (h * m_tiles + t) * splits + s.
+uint64_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32);
+// Partial tiles that prefix_plan() stays within.
+uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads);
+int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
+                     uint32_t kv_heads, bool f32, float *part, float *ml, cudaStream_t stream);
+
+}  // namespace sf37kv

@@ -1,0 +1,236 @@
+// int8 KV caches: rows are quantised as they are written and read back into
+// f16 or f32 caches.
+//
+// Layout of one I8 cache of K (or V): cap * kv_heads * 128 bytes c + 128,
+// [cap][kv_heads][128], then f32 scales [kv_heads][cap]; position p lives in
+// slot p % cap as in the other caches.  One scale serves one head of one row:
+//   s = max|x| / 127 rounded to f32 (0 when below 2^-126, NaN when an element
+//   is not finite), c = the integer nearest to x / s (ties to even), value c*s.
+// A head is the unit that attention multiplies, so a key's scale is one factor
+// of its score and a value's scale one factor of its weight.  The scales of
+// a head lie side by side over the rows: a decode warp reads 16 of them as
+// 64 contiguous bytes (row-major scales would cost it a 32-byte sector each).
+//
+// Both kernels move bytes and compute a few operations for each; HBM bounds
+// them, at (2 or 4) + 1.03 bytes for each element in either direction.
+#include <algorithm>
+
+#include "batch_internal.cuh"
+
+namespace sf37kv {
+
+extern unsigned long long g_launches;
+
+// ------------------------------------------------------------ append
+struct AppendI8Job {
+    uint8_t *k_cache, *v_cache;
+    const void *k, *v;   // [n_tok][heads][128], f32 or bf16
+    uint32_t pos0, cap;  // the rows that stay: at most cap
+};
+struct AppendI8Params {
+    AppendI8Job job[kMaxJobs];
+    uint32_t row_begin[kMaxJobs + 1];
+    uint32_t n_jobs, heads, bf16;
+};
+
+// One warp per head of one row, K and V together: four elements a lane, so
+// a head's maximum is five shuffles and its codes one 128-byte store.
+__global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t unit = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
+    const uint32_t row = (uint32_t)(unit / P.heads), head = (uint32_t)(unit - (uint64_t)row * P.heads);
+    if (row >= P.row_begin[P.n_jobs]) return;
+    uint32_t j = 0;
+    while (j + 1 < P.n_jobs && P.row_begin[j + 1] <= row) j++;
+    const AppendI8Job &J = P.job[j];
+    const uint32_t t = row - P.row_begin[j];
+    const uint32_t slot = (uint32_t)(((uint64_t)J.pos0 + t) % J.cap);
+    const uint64_t src = ((uint64_t)t * P.heads + head) * 128u + lane * 4u;
+    const float4 k = load_row4(J.k, src, P.bf16), v = load_row4(J.v, src, P.bf16);
+    store_i8_head(J.k_cache, J.cap, P.heads, head, slot, lane, k);
+    store_i8_head(J.v_cache, J.cap, P.heads, head, slot, lane, v);
+}
+
+// ------------------------------------------------------------ read back
+struct ReadI8Job {
+    const uint8_t *k_src, *v_src;
+    void *k_dst, *v_dst;
+    uint32_t first, rows, src_cap, dst_cap;
+};
+struct ReadI8Params {
+    ReadI8Job job[kMaxJobs];
+    uint32_t blk_begin[kMaxJobs + 1];
+    uint32_t n_jobs, heads;
+};
+
+// One CTA per kReadRows rows of one job's K (blockIdx.y 0) or V (1).  A thread
+// writes 16 bytes at a time, so stores are coalesced and loads are 4 (f32) or
+// 8 (f16) contiguous codes; 32 or 16 neighbouring threads share a scale.
+constexpr uint32_t kReadRows = 16;
+
+template <bool F16>
+__global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ ReadI8Params P) {
+    constexpr uint32_t E = F16 ? 8u : 4u;  // elements a thread and step
+    uint32_t j = 0;
+    while (j + 1 < P.n_jobs && P.blk_begin[j + 1] <= blockIdx.x) j++;
+    const ReadI8Job &J = P.job[j];
+    const uint32_t r0 = (blockIdx.x - P.blk_begin[j]) * kReadRows;
+    const uint32_t nr = min(kReadRows, J.rows - r0);
+    const uint8_t *src = blockIdx.y ? J.v_src : J.k_src;
+    void *dst = blockIdx.y ? J.v_dst : J.k_dst;
+    const uint64_t kv_dim = (uint64_t)P.heads * 128u;
+    const float *scales = reinterpret_cast<const float *>(src + kv_dim * J.src_cap);
+    const uint32_t per_row = P.heads * (128u / E);
+    const uint64_t first = (uint64_t)J.first + r0;
+    const uint32_t s_src = (uint32_t)(first % J.src_cap), s_dst = (uint32_t)(first % J.dst_cap);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < nr * per_row; i += 256u) {
+        const uint32_t r = i / per_row, c = i - r * per_row;
+        uint32_t a = s_src + r, b = s_dst + r;
+        if (a >= J.src_cap) a %= J.src_cap;
+        if (b >= J.dst_cap) b %= J.dst_cap;
+        const float s = __ldg(scales + (uint64_t)(c / (128u / E)) * J.src_cap + a);
+        const uint8_t *p = src + a * kv_dim + c * E;
+        float x[E];
+        if (F16) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(p);
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) x[e] = (float)((int)(((e < 4 ? w.x : w.y) >> (8u * (e & 3u))) & 255u) - 128) * s;
+            uint4 h;
+            h.x = h2_bits(x[0], x[1]);
+            h.y = h2_bits(x[2], x[3]);
+            h.z = h2_bits(x[4 % E], x[5 % E]);
+            h.w = h2_bits(x[6 % E], x[7 % E]);
+            *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(dst) + b * kv_dim + c * E) = h;
+        } else {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++) x[e] = (float)((int)((w >> (8u * e)) & 255u) - 128) * s;
+            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + b * kv_dim + c * E) =
+                make_float4(x[0], x[1], x[2], x[3]);
+        }
+    }
+}
+
+// Whether two of n pointers are equal (n <= kMaxJobs).
+static bool any_twice(const void **p, uint32_t n) {
+    std::sort(p, p + n);
+    return std::adjacent_find(p, p + n) != p + n;
+}
+
+}  // namespace sf37kv
+
+using namespace sf37kv;
+
+extern "C" uint64_t sf37kv_i8_cache_bytes(uint32_t cap, uint32_t kv_heads, uint32_t head_dim) {
+    if (head_dim != 128) return 0;
+    return ((uint64_t)cap * kv_heads * 132u + 255u) / 256u * 256u;
+}
+
+extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n_layers, uint32_t kv_heads,
+                                uint32_t head_dim, int row_type, void *stream) {
+    if (!layers && n_layers) return set_error(SF37KV_EINVAL, "append_i8: layers is NULL");
+    if (int rc = check_heads("append_i8", kv_heads, kv_heads, head_dim)) return rc;
+    if (row_type != SF37KV_Q_F32 && row_type != SF37KV_Q_BF16)
+        return set_error(SF37KV_EINVAL, "append_i8: unknown row type %d", row_type);
+    cudaStream_t s = stream ? (cudaStream_t)stream : current_stream();
+    // All checks run before the first launch, so a refused call changes nothing.
+    for (uint32_t i = 0; i < n_layers; i++) {
+        const sf37kv_append_i8_layer &L = layers[i];
+        if (int rc = check_cache("append_i8", i, L.cache)) return rc;
+        if (L.n_tok == 0) continue;
+        if (!L.k || !L.v || !aligned16(L.k) || !aligned16(L.v))
+            return set_error(SF37KV_EINVAL, "append_i8: layer %u rows must be non-NULL and 16-byte aligned", i);
+        if ((uint64_t)L.pos0 + L.n_tok > kMaxPos)
+            return set_error(SF37KV_EINVAL, "append_i8: layer %u positions exceed %u", i, kMaxPos);
+        if ((uint64_t)(L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap) * kv_heads > kMaxUnits)
+            return set_error(SF37KV_EINVAL, "append_i8: layer %u has too many rows for one call", i);
+    }
+    // Pass 0 forms the launches and checks them, pass 1 runs them.
+    for (int pass = 0; pass < 2; pass++) {
+        for (uint32_t base = 0; base < n_layers;) {
+            AppendI8Params P;
+            P.n_jobs = 0;
+            P.heads = kv_heads;
+            P.bf16 = row_type == SF37KV_Q_BF16;
+            uint64_t rows = 0;
+            uint32_t i = base;
+            const void *seen[2 * kMaxJobs];
+            for (; i < n_layers && P.n_jobs < (uint32_t)kMaxJobs; i++) {
+                const sf37kv_append_i8_layer &L = layers[i];
+                if (L.n_tok == 0) continue;
+                // With n_tok > cap only the last cap rows stay, as in a sequential append.
+                const uint32_t keep = L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap, skip = L.n_tok - keep;
+                if ((rows + keep) * kv_heads > kMaxUnits) break;
+                const uint64_t off = (uint64_t)skip * kv_heads * 128u * (P.bf16 ? 2u : 4u);
+                P.job[P.n_jobs] = AppendI8Job{(uint8_t *)L.cache.k_cache, (uint8_t *)L.cache.v_cache,
+                                              (const char *)L.k + off, (const char *)L.v + off, L.pos0 + skip,
+                                              L.cache.cap};
+                seen[2 * P.n_jobs] = L.cache.k_cache;
+                seen[2 * P.n_jobs + 1] = L.cache.v_cache;
+                P.row_begin[P.n_jobs++] = (uint32_t)rows;
+                rows += keep;
+            }
+            base = i;
+            if (P.n_jobs == 0) continue;
+            if (pass == 0) {
+                if (any_twice(seen, 2 * P.n_jobs))
+                    return set_error(SF37KV_EINVAL, "append_i8: one cache is written twice in one call");
+                continue;
+            }
+            P.row_begin[P.n_jobs] = (uint32_t)rows;
+            append_i8_kernel<<<(unsigned)((rows * kv_heads + 7u) / 8u), 256, 0, s>>>(P);
+            g_launches++;
+            if (int rc = check_cuda(cudaGetLastError(), "append_i8 launch")) return rc;
+        }
+    }
+    return SF37KV_OK;
+}
+
+extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_layers, uint32_t kv_heads,
+                              uint32_t head_dim, int dst_dtype, void *stream) {
+    if (!layers && n_layers) return set_error(SF37KV_EINVAL, "read_i8: layers is NULL");
+    if (int rc = check_heads("read_i8", kv_heads, kv_heads, head_dim)) return rc;
+    if (dst_dtype != SF37KV_F16 && dst_dtype != SF37KV_F32)
+        return set_error(SF37KV_EINVAL, "read_i8: destination dtype %d is neither f16 nor f32", dst_dtype);
+    cudaStream_t s = stream ? (cudaStream_t)stream : current_stream();
+    for (uint32_t i = 0; i < n_layers; i++) {
+        const sf37kv_read_i8_layer &L = layers[i];
+        if (int rc = check_cache("read_i8", i, L.src)) return rc;
+        if (int rc = check_cache("read_i8", i, L.dst)) return rc;
+        if (L.rows > L.src.cap || L.rows > L.dst.cap)
+            return set_error(SF37KV_EINVAL, "read_i8: layer %u has %u rows for caches of %u and %u", i, L.rows,
+                             L.src.cap, L.dst.cap);
+        if ((uint64_t)L.first_pos + L.rows > kMaxPos)
+            return set_error(SF37KV_EINVAL, "read_i8: layer %u positions exceed %u", i, kMaxPos);
+        if (L.src.k_cache == L.dst.k_cache || L.src.v_cache == L.dst.v_cache || L.src.k_cache == L.dst.v_cache ||
+            L.src.v_cache == L.dst.k_cache)
+            return set_error(SF37KV_EINVAL, "read_i8: layer %u reads and writes the same cache", i);
+    }
+    for (uint32_t base = 0; base < n_layers;) {
+        ReadI8Params P;
+        P.n_jobs = 0;
+        P.heads = kv_heads;
+        uint64_t blks = 0;
+        uint32_t i = base;
+        for (; i < n_layers && P.n_jobs < (uint32_t)kMaxJobs; i++) {
+            const sf37kv_read_i8_layer &L = layers[i];
+            if (L.rows == 0) continue;
+            const uint32_t nb = (L.rows + kReadRows - 1u) / kReadRows;
+            if (blks + nb > kMaxUnits) break;
+            P.job[P.n_jobs] = ReadI8Job{(const uint8_t *)L.src.k_cache, (const uint8_t *)L.src.v_cache, L.dst.k_cache,
+                                        L.dst.v_cache, L.first_pos, L.rows, L.src.cap, L.dst.cap};
+            P.blk_begin[P.n_jobs++] = (uint32_t)blks;
+            blks += nb;
+        }
+        base = i;
+        if (P.n_jobs == 0) continue;
+        P.blk_begin[P.n_jobs] = (uint32_t)blks;
+        const dim3 grid((unsigned)blks, 2);
+        if (dst_dtype == SF37KV_F16) read_i8_kernel<true><<<grid, 256, 0, s>>>(P);
+        else read_i8_kernel<false><<<grid, 256, 0, s>>>(P);
+        g_launches++;
+        if (int rc = check_cuda(cudaGetLastError(), "read_i8 launch")) return rc;
+    }
+    return SF37KV_OK;
+}

@@ -26,6 +26,8 @@ int check_cuda(cudaError_t err, const char *what);
 
 cudaStream_t current_stream();
 int *device_error_flag();
+// The current device's error flag of the shared-prefix kernel (prefix_tc05.cu).
+int prefix_device_error(int clear);
 int num_sms();
 
 // ---------------------------------------------------------------- scratch

@@ -1,0 +1,522 @@
+// Attention of a batch of decode queries over one shared f16 prefix, on the
+// tcgen05 tensor cores: each K/V tile is read once for up to 32 sequences.
+//
+// M folds the batch and the GQA group: row sl * G + hl of a 128-row Q tile is
+// query head hl of sequence sl (128 / G sequences a tile), so one UMMA serves
+// all of a KV head's queries.  A CTA takes one KV head, a run of 128-key tiles
+// (a split) and one or two Q tiles, and leaves its unnormalised O with a
+// (reference, sum) pair for each row; batch_decode.cu joins the splits with each
+// sequence's own rows.
+//
+// Two streams of a CTA ping-pong, so that one's softmax overlaps the other's
+// MMAs.  With two Q tiles (pair) each stream is a Q tile and both use every
+// K/V tile; with one (solo) the streams take alternate K/V tiles of the same
+// Q tile and are joined through shared memory at the end.
+//
+// Warps 0-7 and 8-15 are the softmax of stream 0 and 1, two threads for each
+// row (64 score columns each); warp 16 issues the MMAs, warp 17 the TMA loads,
+// as in prefill_tc05.cu.  TMEM: S_0, S_1, O_0, O_1 (128 columns each); P
+// (f16) overwrites its S.  F32 (f32 queries and outputs): q and P are two
+// f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits: twice the MMAs; P_lo
+// takes the second half of S's columns.
+//
+// Weights are 2^(x - m) with the reference m 7 below a running row maximum,
+// raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
+// the largest.  S and O accumulate in f32 (TMEM), m and l in f32 registers.
+#include <algorithm>
+
+#include "batch_internal.cuh"
+#include "tc05.cuh"
+
+namespace sf37kv {
+
+extern unsigned long long g_launches;
+
+static __device__ int g_prefix_error;  // 1: a bounded wait gave up
+
+struct PrefixDev {
+    CUtensorMap kmap, vmap;  // rows [0, len): later rows read as zeros
+    uint32_t lo, len, seq0, n_seqs, m_tiles, splits, tps, part0, cta0, pairs;
+};
+template <int NS>
+struct PrefixParams {
+    PrefixDev group[kPrefixGroups];
+    PrefixSeq seq[NS];
+    float *part, *ml;
+    uint32_t n_groups, heads_per_kv, kv_heads, tpt;
+};
+
+constexpr float kHead = 7.0f, kRaise = 15.0f;
+
+template <bool F32, int NS>
+__global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
+    using namespace tc05;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_SFULL = 8, B_PFULL = 10, B_ODONE = 12, N_BARS = 14 };
+    enum { T_Q = 0, T_K = 2, T_V = 4 };  // 32 KB tiles; Q: two tiles (pair) or hi and lo (F32)
+    __shared__ __align__(8) uint64_t bars[N_BARS];
+    __shared__ uint32_t tmem_base_sh;
+    __shared__ volatile int abort_sh;
+    __shared__ float xch[2][2][2][128];  // [parity][stream][half][row]
+    __shared__ float qscale_sh[2][128];
+
+    const uint32_t sraw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t s0 = (sraw + 1023u) & ~1023u;
+    uint8_t *gsm = smem_raw + (s0 - sraw);
+    auto tile = [&](uint32_t i) { return s0 + i * kTile; };
+    auto bar = [&](uint32_t i) { return (uint32_t)__cvta_generic_to_shared(&bars[i]); };
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+
+    uint32_t gi = 0;
+    while (gi + 1 < P.n_groups && P.group[gi + 1].cta0 <= blockIdx.x) gi++;
+    const PrefixDev &Gr = P.group[gi];
+    const uint32_t local = blockIdx.x - Gr.cta0;
+    const uint32_t pr = local % Gr.pairs, kvh = (local / Gr.pairs) % P.kv_heads, split = local / (Gr.pairs * P.kv_heads);
+    const uint32_t mt0 = F32 ? pr : 2u * pr;
+    const bool solo = F32 || mt0 + 1u >= Gr.m_tiles;
+    const uint32_t G = P.heads_per_kv, T = P.tpt;
+    const uint32_t kbeg = Gr.lo + split * Gr.tps * 128u;
+    const uint32_t kend = min(kbeg + Gr.tps * 128u, Gr.len);
+    const uint32_t nt = (kend - kbeg + 127u) / 128u;
+    const uint32_t steps = solo ? nt : 2u * nt;
+
+    if (tid == 0) {
+        for (uint32_t t = 0; t < 2; t++) {
+            bar_init(bar(B_KFULL + t), 1);
+            bar_init(bar(B_KEMPTY + t), 1);
+            bar_init(bar(B_VFULL + t), 1);
+            bar_init(bar(B_VEMPTY + t), 1);
+            bar_init(bar(B_SFULL + t), 1);
+            bar_init(bar(B_PFULL + t), 256);
+            bar_init(bar(B_ODONE + t), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;");
+        abort_sh = 0;
+    }
+    if (warp == 0) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&tmem_base_sh);
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // Nothing but workspace partials is written here, and the kernel launched
+    // next waits before it reads them: it may start as SMs become free.
+    asm volatile("griddepcontrol.launch_dependents;");
+
+    const uint32_t st = warp >> 3;               // stream of a softmax warp
+    const uint32_t hh = (warp >> 2) & 1u;        // column half
+    const uint32_t r = ((warp & 3u) << 5) | lane;
+    const uint32_t sl = r / G, hl = r - sl * G;
+    const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
+    const uint32_t si = mt * T + sl;             // sequence within the group
+    const bool valid = sl < T && si < Gr.n_seqs;
+    const PrefixSeq &Q = P.seq[Gr.seq0 + min(si, Gr.n_seqs - 1u)];
+    // Q tiles: scaled by a power of two for each row so that its largest element
+    // is in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.
+    const bool loads_q = warp < 16 && (!solo || st == 0);
+    float qv[64];
+    if (loads_q) {
+        const uint64_t at = (uint64_t)(kvh * G + min(hl, G - 1u)) * 128u + 64u * hh;
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float4 x = load_row4(Q.q, at + 4u * i, !F32);
+            qv[4 * i] = x.x;
+            qv[4 * i + 1] = x.y;
+            qv[4 * i + 2] = x.z;
+            qv[4 * i + 3] = x.w;
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        }
+        xch[0][st][hh][r] = top;
+    }
+    __syncthreads();
+    if (loads_q) {
+        const float top = fmaxf(xch[0][st][0][r], xch[0][st][1][r]);
+        const int e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
+        const float f = __int_as_float((127 - e) << 23);
+        if (hh == 0) qscale_sh[st][r] = __int_as_float((127 + e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
+        uint8_t *qt = gsm + (T_Q + (F32 ? 0u : st)) * kTile;
+#pragma unroll
+        for (uint32_t c = 0; c < 8; c++) {
+            uint4 hv, lv;
+            uint32_t *ho = &hv.x, *lo = &lv.x;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float a = qv[8 * c + 2 * i] * f, b = qv[8 * c + 2 * i + 1] * f;
+                ho[i] = pack_h2(a, b);
+                if (F32) {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&ho[i]));
+                    lo[i] = pack_h2(a - h.x, b - h.y);
+                }
+            }
+            *reinterpret_cast<uint4 *>(qt + tile_off(r, 8u * hh + c)) = hv;
+            if (F32) *reinterpret_cast<uint4 *>(qt + kTile + tile_off(r, 8u * hh + c)) = lv;
+        }
+        fence_async_smem();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_base_sh;
+
+    if (warp == 17) {
+        // ---------------- TMA loader: K and V double-buffered ----------------
+        if (lane == 0) {
+            const int32_t x0 = (int32_t)(kvh * 128u);
+            auto load = [&](uint32_t which, uint32_t j) {  // which: 0 = K, 1 = V
+                const uint32_t b = j & 1u;
+                const int32_t y = (int32_t)(kbeg + j * 128u);
+                const uint32_t full = bar((which ? B_VFULL : B_KFULL) + b);
+                const uint32_t dst = tile((which ? T_V : T_K) + b);
+                const CUtensorMap *map = which ? &Gr.vmap : &Gr.kmap;
+                bar_expect_tx(full, kTile);
+                tma_load_2d(dst, map, x0, y, full);
+                tma_load_2d(dst + kHalf, map, x0 + 64, y, full);
+            };
+            for (uint32_t j = 0; j < 2 && j < nt; j++) {
+                load(0, j);
+                load(1, j);
+            }
+            for (uint32_t j = 0; j + 2 < nt && !abort_sh; j++) {
+                if (!wait_bar(bar(B_KEMPTY + (j & 1u)), (j >> 1) & 1u)) { abort_sh = 1; break; }
+                load(0, j + 2);
+                if (!wait_bar(bar(B_VEMPTY + (j & 1u)), (j >> 1) & 1u)) { abort_sh = 1; break; }
+                load(1, j + 2);
+            }
+        }
+    } else if (warp == 16) {
+        // ---------------- MMA issuer ----------------
+        // Step i belongs to stream i & 1 and key tile i (solo) or i / 2 (pair).
+        // S of step i + 2 overwrites the columns from which PV of step i reads P:
+        // MMAs issued by one thread execute in order.
+        if (lane == 0) {
+            auto issue_s = [&](uint32_t i) -> bool {
+                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
+                if ((solo || t == 0) && !wait_bar(bar(B_KFULL + (j & 1u)), (j >> 1) & 1u)) return false;
+                const uint32_t kt = tile(T_K + (j & 1u)), qt = tile(T_Q + (solo ? 0u : t));
+                fence_after();
+#pragma unroll
+                for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++) {
+                    const uint32_t off = ((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u;
+                    mma(tmem + t * 128u, sdesc(qt + (kk >> 3) * kTile + off, 16, 1024), sdesc(kt + off, 16, 1024),
+                        idesc(0), kk > 0);
+                }
+                commit(bar(B_SFULL + t));
+                if (solo || t == 1) commit(bar(B_KEMPTY + (j & 1u)));
+                return true;
+            };
+            auto issue_pv = [&](uint32_t i) -> bool {
+                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
+                if (!wait_bar(bar(B_PFULL + t), (i >> 1) & 1u)) return false;
+                if ((solo || t == 0) && !wait_bar(bar(B_VFULL + (j & 1u)), (j >> 1) & 1u)) return false;
+                const uint32_t vt = tile(T_V + (j & 1u));
+                fence_after();
+#pragma unroll
+                for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++)
+                    mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, sdesc(vt + (kk & 7u) * 2048u, kHalf, 1024),
+                           idesc(1), (i > 1 || kk > 0) ? 1u : 0u);
+                commit(bar(B_ODONE + t));
+                if (solo || t == 1) commit(bar(B_VEMPTY + (j & 1u)));
+                return true;
+            };
+            bool ok = issue_s(0) && (steps < 2 || issue_s(1));
+            for (uint32_t i = 0; i < steps && ok && !abort_sh; i++)
+                ok = issue_pv(i) && (i + 2 >= steps || issue_s(i + 2));
+            if (!ok) abort_sh = 1;
+        }
+    } else {
+        // ---------------- softmax of stream st, column half hh ----------------
+        const uint32_t lane_off = ((warp & 3u) * 32u) << 16;
+        const uint32_t cb = 64u * hh;
+        const uint32_t t_s = tmem + st * 128u + lane_off, t_o = tmem + 256u + st * 128u + lane_off;
+        const uint32_t pair_bar = 1u + st * 4u + (warp & 3u);  // the two warps that share these rows
+        // Pair barrier that also ORs a flag, so both warps take the same exit.
+        auto pair_any = [&](bool v) -> bool {
+            uint32_t rr;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                "bar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                : "=r"(rr)
+                : "r"((uint32_t)v), "r"(pair_bar)
+                : "memory");
+            return rr != 0;
+        };
+        const uint32_t s_row = max(Q.start, kbeg);
+        const float qs = qscale_sh[solo ? 0 : st][r];
+        const uint32_t n_steps = solo ? (nt + 1u - st) >> 1 : nt;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        // One pass over this thread's 64 scores with reference mu: weights (f16 pairs,
+        // and their remainders) into w and wl, their sum, the largest x - mu.
+        auto pass = [&](uint32_t k0, bool full, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la, float &xm) {
+            float lb = 0.f, xa = -INFINITY, xb = -INFINITY;
+            la = 0.f;
+#pragma unroll
+            for (int q2 = 0; q2 < 2; q2++) {
+                float v[32];
+                tmem_ld32(t_s + cb + q2 * 32u, v);
+                tmem_wait_ld();
+                const uint32_t kb = k0 + cb + (uint32_t)(q2 * 32);
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float x0 = fmaf(v[2 * i], qs, -mu), x1 = fmaf(v[2 * i + 1], qs, -mu);
+                    if (!full) {
+                        const uint32_t kp = kb + 2u * i;
+                        if (kp < s_row || kp >= kend) x0 = -INFINITY;
+                        if (kp + 1u < s_row || kp + 1u >= kend) x1 = -INFINITY;
+                    }
+                    xa = fmaxf(xa, x0);
+                    xb = fmaxf(xb, x1);
+                    const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                    la += p0;
+                    lb += p1;
+                    w[q2][i] = pack_h2(p0, p1);
+                    if (F32) {
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[q2][i]));
+                        wl[q2][i] = pack_h2(p0 - h.x, p1 - h.y);
+                    }
+                }
+            }
+            la += lb;
+            xm = fmaxf(xa, xb);
+        };
+        for (uint32_t s = 0; s < n_steps; s++) {
+            const uint32_t k0 = kbeg + (solo ? 2u * s + st : s) * 128u;
+            __syncwarp();
+            const bool got = !abort_sh && wait_bar_warp(bar(B_SFULL + st), s & 1u);
+            fence_after();
+            const bool full = __all_sync(0xffffffffu, k0 >= s_row && k0 + 128u <= kend);
+            uint32_t w[2][16], wl[2][16];
+            float la = 0.f, xm = -INFINITY;
+            const float mu0 = m == -INFINITY ? 0.f : m;
+            if (got) pass(k0, full, mu0, w, wl, la, xm);
+            if (pair_any(!got)) { abort_sh = 1; ok = false; break; }
+            const bool need = (m == -INFINITY && xm > -INFINITY) || xm > kRaise;
+            if (pair_any(need)) {
+                // raise the rows' references: exchange the maximum with the other half, rescale O, redo P
+                xch[s & 1u][st][hh][r] = xm + mu0;
+                pair_any(false);
+                const float mx = fmaxf(xch[s & 1u][st][0][r], xch[s & 1u][st][1][r]) - kHead;
+                const bool raise = mx > -INFINITY && (m == -INFINITY || mx > m + (kRaise - kHead));
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float alpha = !raise ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - mx);
+                    if (s > 0) {
+#pragma unroll
+                        for (int q2 = 0; q2 < 2; q2++) {
+                            float v[32];
+                            tmem_ld32(t_o + cb + q2 * 32u, v);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) v[i] *= alpha;
+                            tmem_st32(t_o + cb + q2 * 32u, v);
+                        }
+                        tmem_wait_st();
+                    }
+                    if (raise) {
+                        l *= alpha;
+                        m = mx;
+                    }
+                    pass(k0, full, m == -INFINITY ? 0.f : m, w, wl, la, xm);
+                }
+                pair_any(false);  // both halves have re-read S
+            }
+            // (both halves have read S: P overwrites columns of either)
+            l += la;
+            tmem_st16u(t_s + cb / 2u, w[0]);
+            tmem_st16u(t_s + cb / 2u + 16u, w[1]);
+            if (F32) {
+                tmem_st16u(t_s + 64u + cb / 2u, wl[0]);
+                tmem_st16u(t_s + 64u + cb / 2u + 16u, wl[1]);
+            }
+            tmem_wait_st();
+            fence_before();
+            bar_arrive(bar(B_PFULL + st));
+        }
+        const bool got_e = n_steps == 0 || (ok && !abort_sh && wait_bar_warp(bar(B_ODONE + st), (n_steps - 1) & 1u));
+        if (ok) {
+            xch[0][st][hh][r] = l;
+            if (pair_any(!got_e)) ok = false;
+        }
+        if (!ok) abort_sh = 1;
+        if (ok) l = xch[0][st][0][r] + xch[0][st][1][r];
+        // Partial tile of (kv head, m tile, split).
+        const uint64_t row = ((uint64_t)Gr.part0 + ((uint64_t)kvh * Gr.m_tiles + mt) * Gr.splits + split) * 128u + r;
+        float4 *op = reinterpret_cast<float4 *>(P.part + row * 128u + cb);
+        float wA = 1.f;
+        const float *ob = reinterpret_cast<const float *>(gsm + T_K * kTile);  // stream 1's O, [128 columns][128 rows]
+        if (solo) {
+            // Join the streams: stream 1 leaves (m, l) and its O, scaled, in the K tiles (all MMAs on them are done).
+            if (hh == 0) {
+                xch[1][st][0][r] = m;
+                xch[1][st][1][r] = l;
+            }
+            asm volatile("bar.sync 9, 512;" ::: "memory");
+            const float m0 = xch[1][0][0][r], m1 = xch[1][1][0][r], l0 = xch[1][0][1][r], l1 = xch[1][1][1][r];
+            const float mj = fmaxf(m0, m1);
+            wA = m0 == -INFINITY ? (l0 == 0.f ? 0.f : 1.f) : fast_exp2(m0 - mj);
+            const float wB = m1 == -INFINITY ? (l1 == 0.f ? 0.f : 1.f) : fast_exp2(m1 - mj);
+            if (st == 1 && n_steps > 0 && !abort_sh) {
+                fence_after();
+#pragma unroll
+                for (int q2 = 0; q2 < 2; q2++) {
+                    float v[32];
+                    tmem_ld32(t_o + cb + q2 * 32u, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) const_cast<float *>(ob)[(cb + q2 * 32u + i) * 128u + r] = v[i] * wB;
+                }
+            }
+            asm volatile("bar.sync 9, 512;" ::: "memory");
+            m = mj;
+            l = l0 * wA + l1 * wB;
+        }
+        if (!abort_sh && (!solo || st == 0)) {
+            fence_after();
+#pragma unroll
+            for (int q2 = 0; q2 < 2; q2++) {
+                float v[32];
+                tmem_ld32(t_o + cb + q2 * 32u, v);
+                tmem_wait_ld();
+                if (solo) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        v[i] *= wA;
+                        if (nt > 1) v[i] += ob[(cb + q2 * 32u + i) * 128u + r];
+                    }
+                }
+                if (valid)
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        op[q2 * 8 + i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            }
+            if (valid && hh == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (abort_sh && tid == 0) atomicExch(&g_prefix_error, 1);
+    fence_after();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// ------------------------------------------------------------ planning
+// Every CTA takes the same number of key tiles (splits of a group differ by its
+// last): the fewest that fit w waves of one CTA an SM, w the smallest possible or one
+// more, whichever costs less with kFixed tiles' time for a CTA's start and end.
+constexpr uint64_t kFixed = 4;
+
+uint64_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32) {
+    const uint32_t T = prefix_seqs_per_tile(q_heads / kv_heads);
+    uint64_t units = 0, work = 0, most = 1;
+    for (uint32_t i = 0; i < n; i++) {
+        PrefixGroup &X = groups[i];
+        X.m_tiles = (X.n_seqs + T - 1) / T;
+        const uint64_t ctas = (uint64_t)kv_heads * (f32 ? X.m_tiles : (X.m_tiles + 1) / 2);
+        const uint64_t nt = (X.len - X.lo + 127) / 128;
+        units += ctas;
+        work += ctas * nt;
+        most = std::max(most, nt);
+    }
+    auto ctas_at = [&](uint64_t tps) {
+        uint64_t c = 0;
+        for (uint32_t i = 0; i < n; i++) {
+            const PrefixGroup &X = groups[i];
+            c += (uint64_t)kv_heads * (f32 ? X.m_tiles : (X.m_tiles + 1) / 2) * (((X.len - X.lo + 127) / 128 + tps - 1) / tps);
+        }
+        return c;
+    };
+    uint64_t best_tps = most, best_cost = UINT64_MAX;
+    const uint64_t w0 = (units + kPlanSms - 1) / kPlanSms;
+    for (uint64_t w = w0; w <= w0 + 1; w++) {
+        uint64_t tps = std::max<uint64_t>(1, (work + w * kPlanSms - 1) / (w * kPlanSms));
+        while (tps < most && ctas_at(tps) > w * kPlanSms) tps += std::max<uint64_t>(1, tps / 32);
+        tps = std::min(tps, most);
+        const uint64_t cost = (ctas_at(tps) + kPlanSms - 1) / kPlanSms * (tps + kFixed);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best_tps = tps;
+        }
+    }
+    uint64_t tiles = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        PrefixGroup &X = groups[i];
+        X.tiles_per_split = (uint32_t)best_tps;
+        X.splits = (uint32_t)(((X.len - X.lo + 127) / 128 + best_tps - 1) / best_tps);
+        X.part0 = (uint32_t)tiles;
+        tiles += (uint64_t)kv_heads * X.m_tiles * X.splits;
+    }
+    return tiles;
+}
+
+// CTAs stay within units + 2 * kPlanSms, a CTA has at most two tiles, and
+// 2 * (KV heads x tile pairs) within KV heads x (m tiles + groups).
+uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads) {
+    const uint64_t m_tiles = n_seqs / prefix_seqs_per_tile(q_heads / kv_heads) + n_groups;
+    return (uint64_t)kv_heads * (m_tiles + n_groups) + 4u * kPlanSms;
+}
+
+template <bool F32, int NS>
+static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
+                  uint32_t kv_heads, float *part, float *ml, cudaStream_t stream) {
+    constexpr size_t smem = 6 * tc05::kTile + 1024;
+    static bool ready[64];
+    int dev = 0;
+    if (int rc = check_cuda(cudaGetDevice(&dev), "prefix get device")) return rc;
+    if (dev < 0 || dev >= 64 || !ready[dev]) {
+        if (int rc = check_cuda(cudaFuncSetAttribute(prefix_tc05_kernel<F32, NS>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                "prefix shared memory"))
+            return rc;
+        if (dev >= 0 && dev < 64) ready[dev] = true;
+    }
+    PrefixParams<NS> P;
+    uint32_t ctas = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        const PrefixGroup &X = groups[i];
+        PrefixDev &D = P.group[i];
+        if (!tc05::make_map(&D.kmap, X.k, kv_heads * 128u, X.len) || !tc05::make_map(&D.vmap, X.v, kv_heads * 128u, X.len))
+            return set_error(SF37KV_ECUDA, "prefix: tensor map encoding failed");
+        D.lo = X.lo;
+        D.len = X.len;
+        D.seq0 = X.seq0;
+        D.n_seqs = X.n_seqs;
+        D.m_tiles = X.m_tiles;
+        D.splits = X.splits;
+        D.tps = X.tiles_per_split;
+        D.part0 = X.part0;
+        D.pairs = F32 ? X.m_tiles : (X.m_tiles + 1) / 2;
+        D.cta0 = ctas;
+        ctas += D.pairs * kv_heads * X.splits;
+    }
+    std::copy(seqs, seqs + n_seqs, P.seq);
+    P.part = part;
+    P.ml = ml;
+    P.n_groups = n;
+    P.heads_per_kv = q_heads / kv_heads;
+    P.kv_heads = kv_heads;
+    P.tpt = prefix_seqs_per_tile(P.heads_per_kv);
+    prefix_tc05_kernel<F32, NS><<<ctas, 576, smem, stream>>>(P);
+    g_launches++;
+    return check_cuda(cudaGetLastError(), "prefix launch");
+}
+
+int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
+                     uint32_t kv_heads, bool f32, float *part, float *ml, cudaStream_t stream) {
+    if (n_seqs <= 32)
+        return f32 ? launch<true, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream)
+                   : launch<false, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream);
+    return f32 ? launch<true, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream)
+               : launch<false, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream);
+}
+
+int prefix_device_error(int clear) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_prefix_error, sizeof(int)) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return -1;
+    }
+    const int zero = 0;
+    if (clear && v) (void)cudaMemcpyToSymbol(g_prefix_error, &zero, sizeof(int));
+    return v;
+}
+
+}  // namespace sf37kv

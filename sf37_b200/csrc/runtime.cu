@@ -124,7 +124,8 @@ int sf37kv_device_error(int clear) {
         return -1;
     }
     if (clear && v) cudaMemset(f, 0, sizeof(int));
-    return v;
+    const int p = prefix_device_error(clear);
+    return v ? v : p;
 }
 
 void *sf37kv_host_alloc(uint64_t bytes) {

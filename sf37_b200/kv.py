@@ -8,11 +8,13 @@ on error).
 """
 import ctypes
 
+import numpy as np
 import torch
 
-from ._lib import AppendLayer, Cache, DecodeLayer, PackLayer, Tensor, check, lib
+from ._lib import (APPEND_I8_LAYER, DECODE_SEQ, READ_I8_LAYER, SHARED_GROUP, AppendLayer, Cache, DecodeLayer, PackLayer,
+                   Tensor, check, lib)
 
-F16, F32 = 2, 4
+I8, F16, F32 = 1, 2, 4
 Q_F32, Q_BF16 = 0, 1
 FMT_RAW, FMT_I8G = 0, 1
 _DT = {torch.float16: F16, torch.float32: F32}
@@ -206,3 +208,154 @@ def device_error(clear=False) -> int:
 def oproj(layers, in_dim, out_dim, stream=None):
     """Q8_0 o_proj matvec of every layer in one launch (sf37kv_oproj_q8_0)."""
     check(lib().sf37kv_oproj_q8_0(layers, len(layers), in_dim, out_dim, _sp(stream)), "sf37kv_oproj_q8_0")
+
+
+# ------------------------------------------- int8 caches and batched decode
+# The *_desc functions fill a descriptor array once; a decode loop keeps it and
+# writes what changes (``seqs["pos"] = positions``).  They take tensors with a
+# leading dimension of n layers or sequences, or lists of n tensors; the tensors
+# have to outlive the descriptors.
+_IO = {torch.float32: Q_F32, torch.bfloat16: Q_BF16}
+
+
+def _addresses(name, x, n, dtypes=None, inner=None):
+    """Addresses of the n items of a stacked tensor or a list of tensors."""
+    items = [x] if isinstance(x, torch.Tensor) else list(x)
+    for t in items:
+        if not t.is_cuda or t.device != items[0].device or t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name}: tensors on the current CUDA device are needed, got {t.device}")
+        if dtypes is not None and t.dtype not in dtypes:
+            raise ValueError(f"{name}: dtype {t.dtype} is not one of {dtypes}")
+    if isinstance(x, torch.Tensor):
+        if x.dim() < 1 or x.shape[0] != n:
+            raise ValueError(f"{name}: a leading dimension of {n} is needed, got shape {tuple(x.shape)}")
+        items, first = [x[0]] if n else [], x.data_ptr()
+        at = first + np.arange(n, dtype=np.uint64) * np.uint64(x.stride(0) * x.element_size() if n > 1 else 0)
+    else:
+        if len(items) != n:
+            raise ValueError(f"{name}: {n} tensors are needed, got {len(items)}")
+        at = np.array([t.data_ptr() for t in items], dtype=np.uint64)
+    for t in items:
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: each item has to be contiguous")
+        if inner is not None and tuple(t.shape) != tuple(inner):
+            raise ValueError(f"{name}: items of shape {tuple(inner)} are needed, got {tuple(t.shape)}")
+    return at
+
+
+def _count(x):
+    return x.shape[0] if isinstance(x, torch.Tensor) else len(x)
+
+
+def _item(x):
+    return x[0]
+
+
+def i8_cache_bytes(cap, kv_heads, head_dim=128) -> int:
+    """Bytes of one int8 cache of K (or V); allocate it as uint8 (zero-filled or not)."""
+    return int(lib().sf37kv_i8_cache_bytes(cap, kv_heads, head_dim))
+
+
+def append_i8_desc(k_cache, v_cache, cap, pos0, k, v):
+    """k, v: [n][n_tok][kv_heads][128] f32 or bf16 (or lists of [n_tok][kv_heads][128])."""
+    n, rows = _count(k), tuple(_item(k).shape)
+    d = np.zeros(n, APPEND_I8_LAYER)
+    d["k_cache"], d["v_cache"] = (_addresses("k_cache", k_cache, n, (torch.uint8,)),
+                                  _addresses("v_cache", v_cache, n, (torch.uint8,)))
+    d["cap"], d["pos0"], d["n_tok"] = cap, pos0, rows[0] if isinstance(k, torch.Tensor) else [t.shape[0] for t in k]
+    inner = rows if isinstance(k, torch.Tensor) else None
+    d["k"], d["v"] = _addresses("k", k, n, tuple(_IO), inner), _addresses("v", v, n, (_item(k).dtype,), inner)
+    return d
+
+
+def append_i8(layers, kv_heads, head_dim, dtype, stream=None):
+    """Quantises the rows of append_i8_desc() into their caches; dtype: the rows' torch dtype."""
+    check(lib().sf37kv_append_i8(layers.ctypes.data, len(layers), kv_heads, head_dim, _IO[dtype], _sp(stream)),
+          "sf37kv_append_i8")
+
+
+def read_i8_desc(k_cache, v_cache, cap, dst_k, dst_v, dst_cap, first_pos, rows):
+    """dst_k, dst_v: f16 or f32 caches of dst_cap rows, [n][dst_cap][kv_heads][128]."""
+    n = _count(dst_k)
+    d = np.zeros(n, READ_I8_LAYER)
+    d["src_k_cache"], d["src_v_cache"] = (_addresses("k_cache", k_cache, n, (torch.uint8,)),
+                                          _addresses("v_cache", v_cache, n, (torch.uint8,)))
+    d["dst_k_cache"] = _addresses("dst_k", dst_k, n, tuple(_DT))
+    d["dst_v_cache"] = _addresses("dst_v", dst_v, n, (_item(dst_k).dtype,))
+    d["src_cap"], d["dst_cap"], d["first_pos"], d["rows"] = cap, dst_cap, first_pos, rows
+    return d
+
+
+def read_i8(layers, kv_heads, head_dim, dtype, stream=None):
+    """Reads the rows of read_i8_desc() back; dtype: the destinations' torch dtype."""
+    check(lib().sf37kv_read_i8(layers.ctypes.data, len(layers), kv_heads, head_dim, _DT[dtype], _sp(stream)),
+          "sf37kv_read_i8")
+
+
+def decode_seqs_desc(k_cache, v_cache, cap, pos, q, out, gate=None, k_new=None, v_new=None, sliding=False,
+                     window=512):
+    """q, out: [n][q_heads][128] f32 or bf16; gate: [n][q_heads] f32; k_new, v_new: [n][kv_heads][128] like q;
+    caches: uint8 (int8 caches) or f16."""
+    n = _count(q)
+    d = np.zeros(n, DECODE_SEQ)
+    cache = (torch.uint8, torch.float16)
+    d["k_cache"], d["v_cache"] = _addresses("k_cache", k_cache, n, cache), _addresses("v_cache", v_cache, n, cache)
+    d["cap"], d["sliding"], d["window"], d["pos"] = cap, np.asarray(sliding, dtype=bool), window, pos
+    heads, dtype = _item(q).shape[0], (_item(q).dtype,)
+    d["q"], d["out"] = _addresses("q", q, n, tuple(_IO), (heads, 128)), _addresses("out", out, n, dtype, (heads, 128))
+    if gate is not None:
+        d["gate"] = _addresses("gate", gate, n, (torch.float32,), (heads,))
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None:
+        inner = tuple(_item(k_new).shape)
+        d["k_new"], d["v_new"] = _addresses("k_new", k_new, n, dtype, inner), _addresses("v_new", v_new, n, dtype, inner)
+    return d
+
+
+def decode_i8_workspace(n_seqs, q_heads, kv_heads) -> int:
+    """Bytes of a workspace for decode_i8(): allocate it zero-filled (torch.zeros, uint8)."""
+    return int(lib().sf37kv_decode_i8_workspace(n_seqs, q_heads, kv_heads))
+
+
+def decode_i8(seqs, q_heads, kv_heads, head_dim, dtype, workspace, stream=None):
+    """One decode step over int8 caches; dtype: torch dtype of q and out."""
+    check(lib().sf37kv_decode_i8(seqs.ctypes.data, len(seqs), q_heads, kv_heads, head_dim, _IO[dtype],
+                                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), _sp(stream)),
+          "sf37kv_decode_i8")
+
+
+def shared_groups_desc(groups):
+    """groups: list of dicts k_cache, v_cache (f16 [cap][kv_heads][128], or None), prefix_len, seqs (an array of
+    decode_seqs_desc(), which the result refers to: later changes of it count)."""
+    d = np.zeros(len(groups), SHARED_GROUP)
+    for i, g in enumerate(groups):
+        if g["prefix_len"]:
+            k = [g["k_cache"]]
+            d[i]["prefix_k_cache"] = _addresses("prefix k_cache", k, 1, (torch.float16,))[0]
+            d[i]["prefix_v_cache"] = _addresses("prefix v_cache", [g["v_cache"]], 1, (torch.float16,))[0]
+            d[i]["prefix_cap"] = g["k_cache"].shape[0]
+        if g["seqs"].dtype != DECODE_SEQ or not g["seqs"].flags.c_contiguous:
+            raise ValueError("seqs: a contiguous array of decode_seqs_desc() is needed")
+        d[i]["prefix_len"], d[i]["n_seqs"], d[i]["seqs"] = g["prefix_len"], len(g["seqs"]), g["seqs"].ctypes.data
+    return _Groups(d, [g["seqs"] for g in groups])
+
+
+class _Groups:
+    """Group descriptors, and the sequence arrays that they point to."""
+
+    def __init__(self, desc, seqs):
+        self.desc, self.seqs = desc, seqs
+
+
+def decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads) -> int:
+    """Bytes of a workspace for decode_shared(), n_seqs over all groups: allocate it zero-filled."""
+    return int(lib().sf37kv_decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads))
+
+
+def decode_shared(groups, q_heads, kv_heads, head_dim, cache_dtype, dtype, workspace, stream=None):
+    """One decode step of groups that share a prefix; cache_dtype: F16 or I8, of the sequences' own caches."""
+    d = groups.desc
+    check(lib().sf37kv_decode_shared(d.ctypes.data, len(d), q_heads, kv_heads, head_dim, cache_dtype, _IO[dtype],
+                                     workspace.data_ptr(), workspace.numel() * workspace.element_size(), _sp(stream)),
+          "sf37kv_decode_shared")
