@@ -5,8 +5,10 @@
 // For query head h of KV head h / G over rows r (log2 domain, base-2 exps):
 //   s_r = (q[h] . K[r]) log2(e) / sqrt(128),  out = sum_r 2^(s_r - m) V[r] / l,
 // one pass with a running reference m that is raised only when a score exceeds
-// it by more than 8.  I8 rows enter as their integer codes (exact in f16):
-// a key's scale multiplies its score, a value's scale its weight.
+// it by more than 8.  I8 rows enter as their integer codes: a key's scale
+// multiplies its score, a value's scale its weight.  q . codes is a product of
+// integers (q as two or three 8-bit digits, s8 x u8 tiles, exact in s32), so
+// keys need no conversion; value codes become f16, exactly.
 //
 // One CTA serves one KV head of one sequence over a run of rows (a split), so
 // each K/V byte is read once for all G query heads.  Four warps stream
@@ -20,11 +22,13 @@
 // not depend on which CTA is last.
 //
 // Sixteen M rows of a tile hold, by MODE:
-//   kPair  G <= 8:  eight heads twice, f16 "hi" and remainder "lo" of q and of
-//          the weights, 22 bits at no extra cost;
-//   kWide  G <= 16 and bf16 outputs: sixteen heads, weights rounded to f16 (half a step is 2^-11 of
-//          a weight; the output's own rounding has 2^-8);
-//   kTwo   G <= 16 and f32 outputs: two kPair tiles on the same K/V fragments.
+//   kPair  G <= 8: eight heads twice, f16 "hi" and remainder "lo" of the weights
+//          (and of an f16 path's q), 22 bits at no extra cost; I8: q in three digits;
+//   kHalf  the same for I8 and bf16: q in two digits, off by at most 2^-14 of the
+//          head's largest power of two (a bf16 q itself by 2^-8 of each element);
+//   kWide  G <= 16 and bf16: sixteen heads, weights rounded to f16 (half a step is
+//          2^-11 of a weight; the output's own rounding has 2^-8), I8: two digits;
+//   kTwo   G <= 16 and f32: two kPair tiles on the same K/V fragments.
 #include <algorithm>
 #include <climits>
 
@@ -34,11 +38,10 @@ namespace sf37kv {
 
 extern unsigned long long g_launches;
 
-enum { kPair = 0, kWide = 1, kTwo = 2 };
+enum { kPair = 0, kHalf = 1, kWide = 2, kTwo = 3 };
 
 constexpr float kSlack = 8.0f;
-constexpr int kWarps = 4;
-constexpr uint32_t kThreads = kWarps * 32;
+constexpr float kNone = -1e30f;  // reference of a state without rows
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
 constexpr uint32_t kMergePass = 32;    // partials joined per pass
@@ -78,6 +81,11 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(int (&d)[4], const uint4 &a, uint32_t b0, uint32_t b1) {  // s8 x u8
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
     uint4 r;
@@ -159,7 +167,6 @@ struct Stage {
     static constexpr uint32_t kV = 16 * kRow;
     static constexpr uint32_t kScales = 32 * kRow;
     static constexpr uint32_t kBytes = 32 * kRow + (I8 ? 128 : 0);
-    static constexpr int kStages = I8 ? 6 : 3;
     static __device__ __forceinline__ uint32_t k_swz(uint32_t r) {
         return I8 ? (r & 1u) << 2 : ((r & 1u) << 2) ^ (((r >> 1) & 3u) << 1);
     }
@@ -179,20 +186,40 @@ struct Stage {
     }
 };
 
-template <bool I8>
-constexpr size_t batch_smem(int tiles) {
-    return (size_t)kWarps * Stage<I8>::kStages * Stage<I8>::kBytes + (size_t)tiles * 8 * 32 * 16;
-}
+// Warps of a CTA, CTAs of an SM and stages of a warp.  An SM runs 8 warps (12
+// where the registers allow it, for I8: its blocks take more instructions for
+// their bytes), either as CTAs of four, which hide each other's starts and
+// ends, or as one wide CTA, which leaves fewer partials to join.
+template <int MODE, bool I8, bool WIDE>
+struct Shape {
+    static constexpr int kSmWarps = I8 && MODE != kTwo ? 12 : 8;
+    static constexpr int kWarps = WIDE ? kSmWarps : 4;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kCtas = kSmWarps / kWarps;
+    static constexpr int kStages = !I8 ? 3 : kSmWarps == 12 ? 4 : 6;
+    static constexpr uint32_t kUnit = kWarps * 16;  // rows that the warps take at once
+    static constexpr uint32_t kArea = kWarps * kStages * Stage<I8>::kBytes;
+    // q: an I8 q in kDigits digits of 8 bits, eight rows (a group) each, two groups a
+    // tile of 16 rows; an f16 q in tiles of the weights' layout
+    static constexpr int kDigits = MODE == kHalf || MODE == kWide ? 2 : 3;
+    static constexpr int kGroups = kDigits * (MODE == kWide || MODE == kTwo ? 2 : 1);
+    static constexpr int kQTiles = I8 ? (kGroups + 1) / 2 : MODE == kTwo ? 2 : 1;
+    static constexpr uint32_t kSmem = kArea + (8 * 32 * 16) * (!I8 && MODE == kTwo ? 2 : I8 && kQTiles > 2 ? 2 : 1);
+};
 
-template <int MODE, bool I8, int NJ>
-__global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_constant__ BatchParams<NJ> P) {
+template <int MODE, bool I8, bool WIDE, int NJ>
+__global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I8, WIDE>::kCtas)
+    batch_decode_kernel(const __grid_constant__ BatchParams<NJ> P) {
     using namespace bd;
     using St = Stage<I8>;
+    using Sh = Shape<MODE, I8, WIDE>;
     constexpr int NT = MODE == kTwo ? 2 : 1;   // M tiles
-    constexpr int NH = MODE == kPair ? 1 : 2;  // heads of a lane
-    constexpr int S = St::kStages;
+    constexpr int NH = MODE == kWide || MODE == kTwo ? 2 : 1;  // heads of a lane
+    constexpr int ND = Sh::kDigits, NQ = Sh::kQTiles;
+    constexpr int S = Sh::kStages, kWarps = Sh::kWarps, kThreads = Sh::kThreads;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float qfac[16], gate_s[16];
+    __shared__ int qoff[2 * NQ][8];  // I8: -128 times the sum of a group's row
     __shared__ float mw[kMergePass * 16], mM[16], mScale[16], mL[16];
     __shared__ uint32_t s_last;
 
@@ -213,113 +240,172 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
     const float *sbase = reinterpret_cast<const float *>((lane < 16 ? kbase : vbase) + row_bytes * J.cap) +
                          (uint64_t)kvh * J.cap;
     const uint32_t wbuf = (uint32_t)__cvta_generic_to_shared(smem) + warp * S * St::kBytes;
-    uint4 *Qs = reinterpret_cast<uint4 *>(smem + kWarps * S * St::kBytes);  // [tile][kk][lane]
-
-    // The CTA that covers the last row stores the appended one first: K by
-    // warp 0, V by warp 1.
-    if (J.k_new && row0 < row1 && row1 == J.end) {
-        if (warp < 2) {
-            uint8_t *cache = const_cast<uint8_t *>(warp ? vbase : kbase);
-            const float4 x = load_row4(warp ? J.v_new : J.k_new, kvh * 128u + lane * 4u, P.bf16);
-            const uint32_t slot = (J.end - 1u) % J.cap;
-            if (I8) {
-                store_i8_head(cache, J.cap, P.kv_heads, kvh, slot, lane, x);
-            } else {
-                uint2 w;
-                w.x = h2_bits(x.x, x.y);
-                w.y = h2_bits(x.z, x.w);
-                *reinterpret_cast<uint2 *>(cache + slot * row_bytes + kvh * 256u + lane * 8u) = w;
-            }
-        }
-        __syncthreads();
-    }
+    uint4 *Qs = reinterpret_cast<uint4 *>(smem + Sh::kArea);  // [tile][kk][lane]
 
     const uint32_t b_first = row0 + warp * 16u;
-    constexpr uint32_t kStep = kWarps * 16;
+    constexpr uint32_t kStep = Sh::kUnit;
     const uint32_t nblk = b_first < row1 ? (row1 - b_first + kStep - 1) / kStep : 0u;
     uint64_t pol;  // a step reads more than L2 holds: the stream is marked to leave first
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
+    // Lane's part of a block: 16-byte chunk c_ch of rows c_row + kRows * i.
+    constexpr uint32_t kCh = St::kRow / 16, kRows = 32 / kCh;
+    const uint32_t c_ch = lane % kCh, c_row = lane / kCh;
+    const uint64_t lane_off = c_row * row_bytes + kvh * St::kRow + c_ch * 16u;
+    uint32_t slot_next = b_first % J.cap;  // slot of the next block to issue
     auto issue = [&](uint32_t it) {
         if (it < nblk) {
-            const uint32_t bb = b_first + it * kStep, sb = bb % J.cap, st = wbuf + (it % S) * St::kBytes;
-            constexpr uint32_t kCh = St::kRow / 16;
+            const uint32_t bb = b_first + it * kStep, sb = slot_next, st = wbuf + (it % S) * St::kBytes;
+            slot_next += kStep;
+            if (slot_next >= J.cap) slot_next = slot_next - J.cap < J.cap ? slot_next - J.cap : slot_next % J.cap;
+            if (sb + 16u <= J.cap && bb + 16u <= row1) {  // 16 rows side by side
+                const uint8_t *kp = kbase + sb * row_bytes + lane_off, *vp = vbase + sb * row_bytes + lane_off;
 #pragma unroll
-            for (uint32_t i = 0; i < kCh / 2; i++) {
-                const uint32_t c = lane + 32u * i, r = c / kCh, ch = c % kCh;
-                uint32_t slot = sb + r;
-                if (slot >= J.cap) slot %= J.cap;
-                if (bb + r >= row1) slot = sb;  // past the end: a row that is read anyway, masked below
-                const uint64_t go = slot * row_bytes + kvh * St::kRow + ch * 16u;
-                cp16(st + r * St::kRow + ((ch ^ St::k_swz(r)) << 4), kbase + go, pol);
-                cp16(st + St::kV + r * St::kRow + ((ch ^ St::v_swz(r)) << 4), vbase + go, pol);
-            }
-            if (I8) {
-                const uint32_t r = lane & 15u;
-                uint32_t slot = sb + r;
-                if (slot >= J.cap) slot %= J.cap;
-                if (bb + r >= row1) slot = sb;
-                cp4(st + St::kScales + lane * 4u, sbase + slot);
+                for (uint32_t i = 0; i < kCh / 2; i++) {
+                    const uint32_t r = c_row + kRows * i;
+                    cp16(st + r * St::kRow + ((c_ch ^ St::k_swz(r)) << 4), kp, pol);
+                    cp16(st + St::kV + r * St::kRow + ((c_ch ^ St::v_swz(r)) << 4), vp, pol);
+                    kp += kRows * row_bytes;
+                    vp += kRows * row_bytes;
+                }
+                if (I8) cp4(st + St::kScales + lane * 4u, sbase + sb + (lane & 15u));
+            } else {
+                // the ring's end or the last rows: past row1 a row that is read anyway, masked below
+                auto slot_of = [&](uint32_t r) {
+                    uint32_t slot = sb + r;
+                    if (slot >= J.cap) slot %= J.cap;
+                    return bb + r < row1 ? slot : sb;
+                };
+#pragma unroll
+                for (uint32_t i = 0; i < kCh / 2; i++) {
+                    const uint32_t r = c_row + kRows * i;
+                    const uint64_t go = slot_of(r) * row_bytes + kvh * St::kRow + c_ch * 16u;
+                    cp16(st + r * St::kRow + ((c_ch ^ St::k_swz(r)) << 4), kbase + go, pol);
+                    cp16(st + St::kV + r * St::kRow + ((c_ch ^ St::v_swz(r)) << 4), vbase + go, pol);
+                }
+                if (I8) cp4(st + St::kScales + lane * 4u, sbase + slot_of(lane & 15u));
             }
         }
         cp_commit();
     };
+    // The CTA that covers the last row stores the appended one first, K and V by its
+    // last two warps.  A warp whose first stages hold that row starts to load after it.
+    const bool appends = J.k_new && row0 < row1 && row1 == J.end;
+    const bool late = appends && b_first < row1 && (J.end - 1u - b_first) % kStep < 16u &&
+                      (J.end - 1u - b_first) / kStep < S - 1;
+    if (!late) {
 #pragma unroll
-    for (int s = 0; s < S - 1; s++) issue(s);
+        for (int s = 0; s < S - 1; s++) issue(s);
+    }
+    if (appends && warp >= kWarps - 2) {
+        const bool value = warp == kWarps - 1;
+        uint8_t *cache = const_cast<uint8_t *>(value ? vbase : kbase);
+        const float4 x = load_row4(value ? J.v_new : J.k_new, kvh * 128u + lane * 4u, P.bf16);
+        const uint32_t slot = (J.end - 1u) % J.cap;
+        if (I8) {
+            store_i8_head(cache, J.cap, P.kv_heads, kvh, slot, lane, x);
+        } else {
+            uint2 w;
+            w.x = h2_bits(x.x, x.y);
+            w.y = h2_bits(x.z, x.w);
+            *reinterpret_cast<uint2 *>(cache + slot * row_bytes + kvh * 256u + lane * 8u) = w;
+        }
+    }
 
-    // q: scaled by a power of two for each head so that its largest element is
-    // in [1, 2) (f16 then holds a bf16 q exactly, and 22 bits of an f32 one).
-    if (warp < NT) {
-        const uint32_t h0 = warp * 8u + g;
-        float qv[MODE == kWide ? 2 : 1][8][4];
+    // q, scaled by a power of two for each head so that its largest element is in
+    // [1, 2): as f16 (a bf16 q exactly, an f32 one in two parts), or, for I8, as
+    // integers q * 2^21 or 2^13 in signed digits of 8 bits.
+    if (warp < NH) {
+        const uint32_t h = warp * 8u + g;
+        float qv[8][4];
+        float top = 0.f;
 #pragma unroll
-        for (int x = 0; x < (MODE == kWide ? 2 : 1); x++) {
-            const uint32_t h = h0 + 8u * x;
-            float top = 0.f;
+        for (uint32_t kk = 0; kk < 8; kk++) {
+            const float4 x = load_row4(J.q, (uint64_t)(kvh * G + min(h, G - 1u)) * 128u + St::k_dim(kk, t, 0), P.bf16);
+            qv[kk][0] = x.x;
+            qv[kk][1] = x.y;
+            qv[kk][2] = x.z;
+            qv[kk][3] = x.w;
 #pragma unroll
-            for (uint32_t kk = 0; kk < 8; kk++)
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(qv[kk][e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e2;
+        const float f = pow2_below(top, e2);
+        constexpr int kBits = ND == 3 ? 21 : 13;
+        if (t == 0) qfac[h] = pow2(e2) * (1.4426950408889634f * 0.08838834764831845f) * (I8 ? 1.f / (1 << kBits) : 1.f);
+        uint32_t *Q32 = reinterpret_cast<uint32_t *>(Qs);
+        if (I8) {
+            bool finite = true;
+            int sum[ND];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; e++) {
-                    const uint64_t i = (uint64_t)(kvh * G + min(h, G - 1u)) * 128u + St::k_dim(kk, t, e);
-                    const float q = P.bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(J.q)[i] << 16)
-                                           : reinterpret_cast<const float *>(J.q)[i];
-                    qv[x][kk][e] = h < G ? q : 0.f;
-                    top = fmaxf(top, fabsf(qv[x][kk][e]));
+            for (int d = 0; d < ND; d++) sum[d] = 0;
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++) {  // four dimensions: register kk & 1 of half a of step kk / 2
+                uint32_t w[ND];
+#pragma unroll
+                for (int d = 0; d < ND; d++) w[d] = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float x = qv[kk][e] * f;
+                    finite = finite && fabsf(x) < 2.f;
+                    // bytes of v + 0x80..80 are the digits of v plus 128
+                    const uint32_t v = (uint32_t)(__float2int_rn(x * (float)(1 << kBits)) + (ND == 3 ? 0x808080 : 0x8080));
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {  // digit 0 is the highest
+                        const uint32_t byte = (v >> (8 * (ND - 1 - d))) & 255u;
+                        sum[d] += (int)byte - 128;
+                        w[d] |= (byte ^ 128u) << (8 * e);
+                    }
                 }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            int e2;
-            const float f = pow2_below(top, e2);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    const int grp = (int)warp * ND + d;
+                    Q32[(((grp >> 1) * 4 + (kk >> 1)) * 32 + lane) * 4 + (grp & 1) + 2 * (kk & 1)] = w[d];
+                }
+                if (Sh::kGroups & 1) Q32[(((Sh::kGroups >> 1) * 4 + (kk >> 1)) * 32 + lane) * 4 + 1 + 2 * (kk & 1)] = 0;
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], 1);
+                sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], 2);
+                if (t == 0) qoff[warp * ND + d][g] = -128 * sum[d];
+            }
+            if ((Sh::kGroups & 1) && t == 0) qoff[Sh::kGroups][g] = 0;
+            __syncwarp();
+            // a q that is not finite has no digits: its scores are NaN
+            if (!finite) qfac[h] = __int_as_float(0x7fc00000);
+        } else {
 #pragma unroll
             for (int kk = 0; kk < 8; kk++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) qv[x][kk][e] *= f;
-            if (t == 0 && h < 16) qfac[h] = pow2(e2) * (1.4426950408889634f * 0.08838834764831845f);
-        }
-#pragma unroll
-        for (int kk = 0; kk < 8; kk++) {
-            uint32_t a[4];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const float x0 = qv[0][kk][2 * half], x1 = qv[0][kk][2 * half + 1];
-                const __half2 hv = __floats2half2_rn(x0, x1);
-                a[2 * half] = *reinterpret_cast<const uint32_t *>(&hv);
-                if (MODE == kWide) {
-                    constexpr int kB = MODE == kWide ? 1 : 0;
-                    a[2 * half + 1] = h2_bits(qv[kB][kk][2 * half], qv[kB][kk][2 * half + 1]);
-                } else {
-                    const float2 f = __half22float2(hv);
-                    a[2 * half + 1] = h2_bits(x0 - f.x, x1 - f.y);
+                for (int half = 0; half < 2; half++) {
+                    const float x0 = qv[kk][2 * half] * f, x1 = qv[kk][2 * half + 1] * f;
+                    const __half2 hv = __floats2half2_rn(x0, x1);
+                    const float2 hf = __half22float2(hv);
+                    const uint32_t hi = *reinterpret_cast<const uint32_t *>(&hv), lo = h2_bits(x0 - hf.x, x1 - hf.y);
+                    if (MODE == kWide) {
+                        Q32[(kk * 32 + lane) * 4 + 2 * half + warp] = hi;
+                    } else {
+                        Q32[((warp * 8 + kk) * 32 + lane) * 4 + 2 * half] = hi;
+                        Q32[((warp * 8 + kk) * 32 + lane) * 4 + 2 * half + 1] = lo;
+                    }
                 }
-            }
-            Qs[(warp * 8 + kk) * 32 + lane] = make_uint4(a[0], a[1], a[2], a[3]);
         }
     }
     if (tid < 16) gate_s[tid] = tid < G && J.gate ? sigmoid_dev(J.gate[kvh * G + tid]) : 1.f;
     __syncthreads();
+    if (late) {
+#pragma unroll
+        for (int s = 0; s < S - 1; s++) issue(s);
+    }
     float qf[NH];
 #pragma unroll
     for (int h = 0; h < NH; h++) qf[h] = qfac[g + 8u * h];
     const uint32_t qaddr = (uint32_t)__cvta_generic_to_shared(Qs + lane);
+    int q0[2 * NQ];
+#pragma unroll
+    for (int x = 0; x < 2 * NQ; x++) q0[x] = I8 ? qoff[x][g] : 0;
 
     float o[NT][16][4];
 #pragma unroll
@@ -333,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
     float m[NH], l[NH], f[NH];
 #pragma unroll
     for (int h = 0; h < NH; h++) {
-        m[h] = -INFINITY;
+        m[h] = kNone;
         l[h] = 0.f;
         f[h] = I8 ? pow2(kFMax) : 128.f;
     }
@@ -344,72 +430,118 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
         issue(it + S - 1);
         const uint32_t b = b_first + it * kStep, st = wbuf + (it % S) * St::kBytes;
 
-        float s[NT][2][4];
+        // scores of the lane's keys 8i + 2t + e, and the scales of the same values
+        float sc[NH][2][2], vs[2][2], ks[2][2];
+        if (I8) {
+            int s[NQ][2][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NQ; n++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.f;
+                for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int c = 0; c < (I8 ? 2 : 4); c++) {
-            uint4 u[2];
+                    for (int e = 0; e < 4; e++) s[n][i][e] = q0[2 * n + (e >> 1)];
 #pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                const uint32_t r = 8u * i + g;
-                u[i] = lds128(st + r * St::kRow + (((4u * c + t) ^ St::k_swz(r)) << 4));
-            }
+            for (int c = 0; c < 2; c++) {
+                uint4 u[2];
 #pragma unroll
-            for (int w = 0; w < (I8 ? 4 : 2); w++) {
-                const int kk = c * (I8 ? 4 : 2) + w;
+                for (uint32_t i = 0; i < 2; i++) {
+                    const uint32_t r = 8u * i + g;
+                    u[i] = lds128(st + r * St::kRow + (((4u * c + t) ^ St::k_swz(r)) << 4));
+                }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const uint4 q4 = lds128(qaddr + (n * 8 + kk) * 512);
-                    const uint32_t a[4] = {q4.x, q4.y, q4.z, q4.w};
+                for (int n = 0; n < NQ; n++) {
+                    const uint4 a0 = lds128(qaddr + (n * 4 + 2 * c) * 512), a1 = lds128(qaddr + (n * 4 + 2 * c + 1) * 512);
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        if (I8) mma(s[n][i], a, codes_lo(word(u[i], w)), codes_hi(word(u[i], w)));
-                        else mma(s[n][i], a, word(u[i], 2 * w), word(u[i], 2 * w + 1));
+                        mma(s[n][i], a0, u[i].x, u[i].y);
+                        mma(s[n][i], a1, u[i].z, u[i].w);
                     }
                 }
             }
-        }
-
-        // scores of the lane's keys 8i + 2t + e; the value scales of the same
-        float sc[NH][2][2], vs[2][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float2 ks = make_float2(1.f, 1.f), v2 = make_float2(1.f, 1.f);
-            if (I8) {
-                ks = lds64f(st + St::kScales + (8u * i + 2u * t) * 4u);
-                v2 = lds64f(st + St::kScales + 64u + (8u * i + 2u * t) * 4u);
+            for (int i = 0; i < 2; i++) {
+                const float2 k2 = lds64f(st + St::kScales + (8u * i + 2u * t) * 4u);
+                const float2 v2 = lds64f(st + St::kScales + 64u + (8u * i + 2u * t) * 4u);
+                ks[i][0] = k2.x;
+                ks[i][1] = k2.y;
+                vs[i][0] = v2.x;
+                vs[i][1] = v2.y;
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int h = 0; h < NH; h++) {
+                        auto digit = [&](int d) { return s[(h * ND + d) >> 1][i][e + 2 * ((h * ND + d) & 1)]; };
+                        // two digits: below 2^31; a third: two f32 roundings of the sum
+                        const int top2 = digit(0) * 256 + digit(1);
+                        sc[h][i][e] = ND == 3 ? fmaf((float)top2, 256.f, (float)digit(ND - 1)) : (float)top2;
+                    }
             }
+        } else {
+            float s[NT][2][4];
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const bool live = b + 8u * i + 2u * t + e < row1;
-                const float k = e ? ks.y : ks.x;
-                vs[i][e] = live ? (e ? v2.y : v2.x) : 0.f;
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int h = 0; h < NH; h++) {
-                    const float x = MODE == kWide ? s[0][i][e + 2 * h] : s[h % NT][i][e] + s[h % NT][i][e + 2];
-                    sc[h][i][e] = live ? x * (qf[h] * k) : -INFINITY;
+                for (int i = 0; i < 2; i++) s[n][i][0] = s[n][i][1] = s[n][i][2] = s[n][i][3] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint4 u[2];
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++) {
+                    const uint32_t r = 8u * i + g;
+                    u[i] = lds128(st + r * St::kRow + (((4u * c + t) ^ St::k_swz(r)) << 4));
                 }
+#pragma unroll
+                for (int w = 0; w < 2; w++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const uint4 q4 = lds128(qaddr + (n * 8 + 2 * c + w) * 512);
+                        const uint32_t a[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                        for (int i = 0; i < 2; i++) mma(s[n][i], a, word(u[i], 2 * w), word(u[i], 2 * w + 1));
+                    }
             }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    ks[i][e] = vs[i][e] = 1.f;
+#pragma unroll
+                    for (int h = 0; h < NH; h++)
+                        sc[h][i][e] = MODE == kWide ? s[0][i][e + 2 * h] : s[h % NT][i][e] + s[h % NT][i][e + 2];
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int h = 0; h < NH; h++) sc[h][i][e] *= I8 ? qf[h] * ks[i][e] : qf[h];
+        if (b + 16u > row1) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (b + 8u * i + 2u * t + e >= row1) {
+                        vs[i][e] = 0.f;
+#pragma unroll
+                        for (int h = 0; h < NH; h++) sc[h][i][e] = -INFINITY;
+                    }
         }
         float p[NH][2][2], w[NH][2][2];
         bool need[NH];
         auto weigh = [&](int h) {
-            const float mu = m[h] == -INFINITY ? 0.f : m[h];
             float xm = -INFINITY, wm = 0.f;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float x = sc[h][i][e] - mu;
+                    const float x = sc[h][i][e] - m[h];
                     xm = fmaxf(xm, x);
                     p[h][i][e] = fast_exp2(x);
                     w[h][i][e] = I8 ? p[h][i][e] * (vs[i][e] * f[h]) : p[h][i][e] * f[h];
                     wm = fmaxf(wm, w[h][i][e]);
                 }
-            need[h] = xm > kSlack || (m[h] == -INFINITY && xm > -INFINITY) || (I8 && wm > 32768.f);
+            need[h] = xm > kSlack || (I8 && wm > 32768.f);
         };
         bool any = false;
 #pragma unroll
@@ -427,30 +559,23 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
                 float mx = fmaxf(fmaxf(sc[h][0][0], sc[h][0][1]), fmaxf(sc[h][1][0], sc[h][1][1]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                fac[h] = 1.f;
                 const float mn = nd ? fmaxf(m[h], mx) : m[h];
-                if (nd) {
-                    const float alpha = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - mn);
-                    l[h] *= alpha;
-                    fac[h] = alpha;
-                    m[h] = mn;
-                }
+                fac[h] = fast_exp2(m[h] - mn);
+                l[h] *= fac[h];
+                m[h] = mn;
                 if (I8) {
-                    const float mu = mn == -INFINITY ? 0.f : mn;
                     float top = 0.f;
 #pragma unroll
                     for (int i = 0; i < 2; i++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) top = fmaxf(top, fast_exp2(sc[h][i][e] - mu) * vs[i][e]);
+                        for (int e = 0; e < 2; e++) top = fmaxf(top, fast_exp2(sc[h][i][e] - mn) * vs[i][e]);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (nd) {
-                        int e2;
-                        pow2_below(top, e2);
-                        const float fn = pow2(max(kFMin, min(kFMax, 7 - e2)));
-                        fac[h] *= fn / f[h];
-                        f[h] = fn;
-                    }
+                    int e2;
+                    pow2_below(top, e2);
+                    const float fn = nd ? pow2(max(kFMin, min(kFMax, 7 - e2))) : f[h];
+                    fac[h] *= fn / f[h];
+                    f[h] = fn;
                 }
                 weigh(h);
             }
@@ -526,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
     cp_wait<0>();
     __syncthreads();  // the stages become the merge buffer
 
-    // ---- the four warps' states to one ----
+    // ---- the warps' states to one ----
     float *Os = reinterpret_cast<float *>(smem);  // [warp*16 + head][128]
     float *Ms = Os + kWarps * 16 * 128, *Ls = Ms + kWarps * 16, *W = Ls + kWarps * 16, *PM = W + kWarps * 16,
           *PL = PM + 16;
@@ -550,16 +675,14 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
     }
     __syncthreads();
     if (tid < G) {
-        float M = -INFINITY, L = 0.f;
+        float M = kNone, L = 0.f;
 #pragma unroll
         for (int s = 0; s < kWarps; s++) M = fmaxf(M, Ms[s * 16 + tid]);
 #pragma unroll
         for (int s = 0; s < kWarps; s++) {
-            // a state whose only scores were NaN has m = -inf and l = NaN: its weight is 1, so that NaN stays
-            const float ms = Ms[s * 16 + tid], ls = Ls[s * 16 + tid];
-            const float w = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : fast_exp2(ms - M);
+            const float w = fast_exp2(Ms[s * 16 + tid] - M);
             W[s * 16 + tid] = w;
-            L += ls * w;
+            L += Ls[s * 16 + tid] * w;
         }
         PM[tid] = M;
         PL[tid] = L;
@@ -608,13 +731,12 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
     const uint32_t land = (uint32_t)__cvta_generic_to_shared(smem), ml_land = (uint32_t)__cvta_generic_to_shared(Qs);
     const float *ml_s = reinterpret_cast<const float *>(Qs);
     static_assert(kMergePass * 32 * 4 <= 8 * 32 * 16, "(m, l) pairs of a pass");
-    constexpr uint32_t kStageArea = kWarps * S * St::kBytes;
-    const uint32_t per = min(kMergePass, kStageArea / (G * 512u));
+    const uint32_t per = min(kMergePass, Sh::kArea / (G * 512u));
     if (tid < 16) {
-        mM[tid] = -INFINITY;
+        mM[tid] = kNone;
         mL[tid] = 0.f;
     }
-    constexpr int kPer = 4;  // float4 outputs of a thread, G <= 16
+    constexpr int kPer = (16 * 32 + kThreads - 1) / kThreads;  // float4 outputs of a thread, G <= 16
     float4 acc[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; k++) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -647,14 +769,14 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
             float M = fmaxf(ms, mo);
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-            const float w = ms == -INFINITY ? (ls == 0.f ? 0.f : 1.f) : fast_exp2(ms - M);
+            const float w = fast_exp2(ms - M);
             float L = ls * w;
 #pragma unroll
             for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
             mw[lane * 16u + h] = w;
             __syncwarp();
             if (lane == 0) {
-                const float sc = mo == -INFINITY ? (mL[h] == 0.f ? 0.f : 1.f) : fast_exp2(mo - M);
+                const float sc = fast_exp2(mo - M);
                 mScale[h] = sc;
                 mL[h] = mL[h] * sc + L;
                 mM[h] = M;
@@ -690,42 +812,60 @@ __global__ void __launch_bounds__(kThreads, 2) batch_decode_kernel(const __grid_
 }
 
 // ------------------------------------------------------------ planning
-// Rows of a split.  Two CTAs fit an SM, so 296 run at once.  A launch whose
-// CTAs can each take all of their share in one wave of at most kWaveRows rows does so
-// (fewest partials); more work is cut into about kWaves waves, whose ends even out.
-constexpr uint32_t kResident = 2 * kPlanSms, kWaves = 8;
-constexpr uint32_t kUnit = kWarps * 16;  // rows that the warps of a CTA take at once
+// Rows of a split.  Few pairs (sequence, KV head): one wave of wide CTAs, with
+// as many splits as fill it.  More pairs: the split whose CTAs, in whole waves of
+// `resident`, cost least, a CTA's start and end counting as kFixedRows rows; a
+// pair's splits are even, and a short pair is one.
+constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256;
 
-static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint32_t rows) {
+struct Plan {
+    bool wide;
+    uint32_t ctas;
+};
+static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint64_t rows) {
     uint64_t c = 0;
-    for (uint32_t i = 0; i < n; i++) c += std::max(1u, (seqs[i].end - seqs[i].start + rows - 1) / rows);
+    for (uint32_t i = 0; i < n; i++) c += std::max<uint64_t>(1, (seqs[i].end - seqs[i].start + rows - 1) / rows);
     return c;
 }
-
-static uint32_t plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads) {
+static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wide_unit, uint32_t unit,
+                        uint32_t resident) {
+    Plan plan;
     uint64_t total = 0;
     for (uint32_t i = 0; i < n; i++) total += seqs[i].end - seqs[i].start;
-    const uint64_t per_wave = (total * kv_heads + kResident - 1) / kResident;  // rows of a CTA in one wave
+    total *= kv_heads;
+    plan.wide = (uint64_t)n * kv_heads <= kPlanSms / 4;
+    const uint64_t u = plan.wide ? wide_unit : unit;
     uint64_t rows;
-    if (per_wave <= 2048) {
-        rows = std::max<uint64_t>(1, (per_wave + kUnit - 1) / kUnit) * kUnit;
-        if ((uint64_t)n * kv_heads <= kResident)
-            while (plan_ctas(seqs, n, (uint32_t)rows) * kv_heads > kResident) rows += std::max<uint64_t>(1, rows / (16 * kUnit)) * kUnit;
+    if (plan.wide) {
+        rows = std::max<uint64_t>(1, (total / kPlanSms + u - 1) / u) * u;
+        while (plan_ctas(seqs, n, rows) * kv_heads > kPlanSms) rows += std::max<uint64_t>(1, rows / (32 * u)) * u;
     } else {
-        rows = std::max<uint64_t>(1024, (total * kv_heads + kResident * kWaves - 1) / (kResident * kWaves));
-        rows = (rows + kUnit - 1) / kUnit * kUnit;
+        uint64_t best = UINT64_MAX;
+        rows = u;
+        for (uint64_t waves = 1; waves <= 8; waves++) {
+            // CTAs of about 1/waves of a slot's share, at most kMaxCtas beyond one for each pair
+            uint64_t r = std::max((total + waves * resident - 1) / (waves * resident), (total + kMaxCtas - 1) / kMaxCtas);
+            r = std::max<uint64_t>(1, (r + u - 1) / u) * u;
+            for (int k = 0; k < 2; k++, r += std::max<uint64_t>(1, r / (8 * u)) * u) {
+                const uint64_t c = plan_ctas(seqs, n, r) * kv_heads;
+                const uint64_t cost = (c + resident - 1) / resident * (total / c + kFixedRows);
+                if (cost < best) {
+                    best = cost;
+                    rows = r;
+                }
+            }
+        }
     }
-    uint32_t ctas = 0;
+    plan.ctas = 0;
     for (uint32_t i = 0; i < n; i++) {
         SeqDev &J = seqs[i];
-        const uint32_t len = J.end - J.start;
-        J.n_splits = std::max<uint32_t>(1u, (uint32_t)((len + rows - 1) / rows));
-        // even splits, whole units
-        J.split_rows = std::max<uint32_t>(kUnit, ((len + J.n_splits - 1) / J.n_splits + kUnit - 1) / kUnit * kUnit);
-        J.cta_begin = ctas;
-        ctas += J.n_splits * kv_heads;
+        const uint64_t len = J.end - J.start;
+        J.n_splits = (uint32_t)std::max<uint64_t>(1, (len + rows - 1) / rows);
+        J.split_rows = (uint32_t)std::max<uint64_t>(u, ((len + J.n_splits - 1) / J.n_splits + u - 1) / u * u);
+        J.cta_begin = plan.ctas;
+        plan.ctas += J.n_splits * kv_heads;
     }
-    return ctas;
+    return plan;
 }
 
 // Sequences of a launch: the counters bound them with many KV heads.
@@ -739,8 +879,7 @@ struct Layout {
 };
 static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads, bool shared) {
     const uint64_t n = std::min<uint64_t>(n_seqs, seqs_per_launch(kv_heads)), g = std::min<uint64_t>(n_groups, kPrefixGroups);
-    // plan_splits() cuts at most kResident * kWaves CTAs beyond one for each (sequence, KV head)
-    const uint64_t ctas = n * kv_heads + kResident * kWaves;
+    const uint64_t ctas = n * kv_heads + kMaxCtas;
     const uint64_t tiles = shared ? prefix_tiles_bound(g, n, q_heads, kv_heads) : 0;
     Layout w;
     w.part = kCounters * 4u;
@@ -751,16 +890,16 @@ static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint3
 }
 
 // ------------------------------------------------------------ launches
-template <int MODE, bool I8, int NJ>
+template <int MODE, bool I8, bool WIDE, int NJ>
 static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
                   cudaStream_t stream) {
-    constexpr size_t smem = batch_smem<I8>(MODE == kTwo ? 2 : 1);
+    using Sh = Shape<MODE, I8, WIDE>;
     static bool ready[64];
     int dev = 0;
     if (int rc = check_cuda(cudaGetDevice(&dev), "decode get device")) return rc;
     if (dev < 0 || dev >= 64 || !ready[dev]) {
-        if (int rc = check_cuda(cudaFuncSetAttribute(batch_decode_kernel<MODE, I8, NJ>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+        if (int rc = check_cuda(cudaFuncSetAttribute(batch_decode_kernel<MODE, I8, WIDE, NJ>,
+                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Sh::kSmem),
                                 "decode shared memory"))
             return rc;
         if (dev >= 0 && dev < 64) ready[dev] = true;
@@ -777,8 +916,8 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchPara
     P.pre_ml = head.pre_ml;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(Sh::kThreads);
+    cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = stream;
     // After a prefix launch the CTAs start as its CTAs leave, and stream their own
     // rows meanwhile; every CTA waits for that launch before it reads its
@@ -788,26 +927,30 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchPara
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = after_prefix ? 1 : 0;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, NJ>, P);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, WIDE, NJ>, P);
     if (e == cudaSuccess) e = cudaGetLastError();
     g_launches++;
     return check_cuda(e, "decode launch");
 }
 
 template <int MODE, bool I8>
-static int launch_n(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
-                    cudaStream_t stream) {
+static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool after_prefix, cudaStream_t stream) {
+    const Plan plan = plan_splits(seqs, n, head.kv_heads, Shape<MODE, I8, true>::kUnit, Shape<MODE, I8, false>::kUnit,
+                                  Shape<MODE, I8, false>::kCtas * kPlanSms);
     // The descriptors travel as kernel parameters; a small launch carries few.
-    return n <= kSmallSeqs ? launch<MODE, I8, kSmallSeqs>(seqs, n, ctas, head, after_prefix, stream)
-                           : launch<MODE, I8, kMaxSeqs>(seqs, n, ctas, head, after_prefix, stream);
+    const bool few = n <= kSmallSeqs;
+    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
+    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
+    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
+    return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
 }
 
 template <bool I8>
-static int launch_mode(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
-                       cudaStream_t stream) {
-    if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, ctas, head, after_prefix, stream);
-    if (head.bf16) return launch_n<kWide, I8>(seqs, n, ctas, head, after_prefix, stream);
-    return launch_n<kTwo, I8>(seqs, n, ctas, head, after_prefix, stream);
+static int launch_mode(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool after_prefix, cudaStream_t stream) {
+    if (head.group <= 8 && head.bf16 && I8) return launch_n<I8 ? kHalf : kPair, I8>(seqs, n, head, after_prefix, stream);
+    if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, head, after_prefix, stream);
+    if (head.bf16) return launch_n<kWide, I8>(seqs, n, head, after_prefix, stream);
+    return launch_n<kTwo, I8>(seqs, n, head, after_prefix, stream);
 }
 
 static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, uint32_t prefix_len, bool ring_clamp) {
@@ -954,13 +1097,12 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
                 J.pre_splits = X.splits;
                 J.pre_row = i % T * head.group;
             }
-            const uint32_t ctas = plan_splits(sd, n, kv_heads);
             if (n_pg)
                 if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
                                               (float *)(ws + W.ml), stream))
                     return rc;
-            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, ctas, head, n_pg > 0, stream)
-                                              : launch_mode<false>(sd, n, ctas, head, n_pg > 0, stream);
+            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, n_pg > 0, stream)
+                                              : launch_mode<false>(sd, n, head, n_pg > 0, stream);
             if (rc) return rc;
         }
     }

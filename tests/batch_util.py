@@ -73,12 +73,22 @@ def attend(q, k, v, gate):
     return o.reshape(-1, D), mag.reshape(-1, D), reach.reshape(-1, 1)
 
 
-def bound(want, mag, reach, n_rows, dtype, p_f16):
-    """Largest error of an output.  A score (log2 units) sums 8 tile products in f32 (each step may drop 2^-23 of at
+def coarse_q(q, k):
+    """Largest error (log2 units) of a score over int8 caches from a bf16 query: held to half a unit of 2^-13 of the
+    power of two below its largest element, against sum |k|.  q [q_heads, 128], k [rows, kv_heads, 128]."""
+    if k.shape[0] == 0:
+        return 0.0
+    step = 2.0 ** torch.floor(torch.log2(q.double().abs().amax(-1))) * 2.0 ** -14
+    reach = k.abs().sum(-1).amax(0).repeat_interleave(q.shape[0] // k.shape[1])
+    return (step * reach * (math.log2(math.e) / math.sqrt(D))).view(-1, 1)
+
+
+def bound(want, mag, reach, n_rows, dtype, p_f16, score=0.0):
+    """Largest error of an output, `score` being an error of the scores beyond the following.  A score (log2 units) sums 8 tile products in f32 (each step may drop 2^-23 of at
     most `reach`) of operands held to 22 bits: 2^-19 * reach, a relative error ln 2 of that in its weight; the
     exponential 2^-21; the weight 2^-22 in two f16 parts, or 2^-11 in one; the output sums n_rows / 16 tile products at
     2^-23 each, and the merge and the division a few 2^-23.  Numerator and denominator each carry it."""
-    w = 0.6932 * reach * 2.0 ** -19 + 2.0 ** -21 + (2.0 ** -11 if p_f16 else 2.0 ** -22) + (n_rows / 16 + 16) * 2.0 ** -23
+    w = 0.6932 * (reach * 2.0 ** -19 + score) + 2.0 ** -21 + (2.0 ** -11 if p_f16 else 2.0 ** -22) + (n_rows / 16 + 16) * 2.0 ** -23
     return 2 * w * mag + 1e-30 + (2.0 ** -8 * want.abs() * (1 + 2 * 2.0 ** -8) if dtype == torch.bfloat16 else 0)
 
 

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from sf37_b200 import kv
-from tests.batch_util import (D, attend, attended, bound, check, fill_i8, i8_views, quantise, rows, values, workspace)
+from tests.batch_util import (D, attend, attended, bound, check, coarse_q, fill_i8, i8_views, quantise, rows, values, workspace)
 
 pytestmark = pytest.mark.gpu
 
@@ -41,7 +41,8 @@ def _case(caps, poss, heads, group, dtype, window=0, append=False, gate=True, sc
                 assert torch.equal(raw, before[i][j]), f"cache of sequence {i}"
                 kvals.append(attended(values(raw, caps[i], heads)[0], caps[i], poss[i], _start(poss[i], caps[i], window)))
             want, mag, reach = attend(q[i], kvals[0], kvals[1], None if gt is None else gt[i])
-            tol = bound(want, mag, reach, kvals[0].shape[0], dtype, p_f16=group > 8 and dtype == torch.bfloat16)
+            tol = bound(want, mag, reach, kvals[0].shape[0], dtype, p_f16=group > 8 and dtype == torch.bfloat16,
+                        score=coarse_q(q[i], kvals[0]) if dtype == torch.bfloat16 else 0.0)
             check(out[i], want, tol, f"sequence {i}")
 
 

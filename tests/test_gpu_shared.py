@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from sf37_b200 import kv
-from tests.batch_util import D, attend, attended, bound, check, fill_i8, rows, values, workspace
+from tests.batch_util import D, attend, attended, bound, check, coarse_q, fill_i8, rows, values, workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -50,7 +50,8 @@ def _case(groups, heads, group, dtype, cache="f16", append=False, scale=1.0, see
                 kx = torch.cat([pk[first:plen].double(), attended(kx, cap, pos[i], max(first, plen))])
                 vx = torch.cat([pv[first:plen].double(), attended(vx, cap, pos[i], max(first, plen))])
                 want, mag, reach = attend(q[i], kx, vx, None if gt is None else gt[i])
-                tol = bound(want, mag, reach, kx.shape[0], dtype, p_f16=dtype == torch.bfloat16)
+                tol = bound(want, mag, reach, kx.shape[0], dtype, p_f16=dtype == torch.bfloat16,
+                            score=coarse_q(q[i], kx) if i8 and dtype == torch.bfloat16 else 0.0)
                 check(out[i], want, tol, f"prefix {plen} sequence {i}")
     assert kv.device_error() == 0
 
