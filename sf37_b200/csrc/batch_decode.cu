@@ -44,6 +44,7 @@ constexpr float kSlack = 8.0f;
 constexpr float kNone = -1e30f;  // reference of a state without rows
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
+constexpr uint32_t kMapped = 1024;     // slots with a direct map to their sequence
 constexpr uint32_t kMergePass = 32;    // partials joined per pass
 // Range of the weights' power of two (kernel below): the ratio of two is finite.
 constexpr int kFMin = -86, kFMax = 40;
@@ -54,7 +55,7 @@ struct SeqDev {
     void *out;
     const void *k_new, *v_new;
     uint32_t start, end, cap;            // own rows [start, end)
-    uint32_t split_rows, n_splits, cta_begin;
+    uint32_t split_rows, n_splits, slot;  // its splits are slots slot, slot + 1, ...
     // partials of the shared prefix: tile pre_tile + kvh * pre_kvh + split, row pre_row on
     uint32_t pre_tile, pre_kvh, pre_splits, pre_row;
 };
@@ -62,8 +63,9 @@ __host__ __device__ constexpr uint32_t part_stride(uint32_t g) { return g * 128u
 
 template <int NJ>
 struct BatchParams {
+    uint8_t seq_of[kMapped];  // sequence of a slot; CTA = slot * kv_heads + KV head
     SeqDev seq[NJ];
-    uint32_t n, group, kv_heads, bf16;
+    uint32_t n, slots, group, kv_heads, bf16;
     float *part;          // [cta][part_stride(G)]: O [G][128], then (m, l) [G]
     uint32_t *counters;   // [sequence][kv head]
     const float *pre_part, *pre_ml;
@@ -149,6 +151,14 @@ __device__ __forceinline__ void store_out4(void *out, uint64_t i, float4 x, bool
     w.y = *reinterpret_cast<const uint32_t *>(&b);
     *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(out) + i) = w;
 }
+// (a, l) += (x, lx) * w
+__device__ __forceinline__ void fold(float4 &a, float &l, const float4 &x, float lx, float w) {
+    a.x = fmaf(x.x, w, a.x);
+    a.y = fmaf(x.y, w, a.y);
+    a.z = fmaf(x.z, w, a.z);
+    a.w = fmaf(x.w, w, a.w);
+    l = fmaf(lx, w, l);
+}
 __device__ __forceinline__ float4 normalise(float4 a, float l, float g) {
     if (l == 0.f) return make_float4(0.f, 0.f, 0.f, 0.f);  // no row attended to
     return make_float4(a.x / l * g, a.y / l * g, a.z / l * g, a.w / l * g);
@@ -186,17 +196,19 @@ struct Stage {
     }
 };
 
-// Warps of a CTA, CTAs of an SM and stages of a warp.  An SM runs 8 warps (12
-// where the registers allow it, for I8: its blocks take more instructions for
-// their bytes), either as CTAs of four, which hide each other's starts and
-// ends, or as one wide CTA, which leaves fewer partials to join.
+// Warps of a CTA, CTAs of an SM and stages of a warp.  An SM runs 12 warps (8 in
+// kTwo, for their registers), either as CTAs of four, which hide each other's
+// starts and ends, or as one wide CTA, which leaves fewer partials to join.
+// More stages only lengthen the queue to HBM, and with it every other access:
+// 8 layers x 32769 rows of I8 took 95 us with three stages, 100 with four, 102
+// with two; f16 rows 76 us with two stages of 12 warps, 80 with three of 8.
 template <int MODE, bool I8, bool WIDE>
 struct Shape {
-    static constexpr int kSmWarps = I8 && MODE != kTwo ? 12 : 8;
+    static constexpr int kSmWarps = MODE != kTwo ? 12 : 8;
     static constexpr int kWarps = WIDE ? kSmWarps : 4;
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kCtas = kSmWarps / kWarps;
-    static constexpr int kStages = !I8 ? 3 : kSmWarps == 12 ? 4 : 6;
+    static constexpr int kStages = (I8 ? 3 : 2) + (MODE == kTwo ? 1 : 0);
     static constexpr uint32_t kUnit = kWarps * 16;  // rows that the warps take at once
     static constexpr uint32_t kArea = kWarps * kStages * Stage<I8>::kBytes;
     // q: an I8 q in kDigits digits of 8 bits, eight rows (a group) each, two groups a
@@ -220,19 +232,22 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float qfac[16], gate_s[16];
     __shared__ int qoff[2 * NQ][8];  // I8: -128 times the sum of a group's row
-    __shared__ float mw[kMergePass * 16], mM[16], mScale[16], mL[16];
     __shared__ uint32_t s_last;
 
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
-    uint32_t lo = 0, hi = P.n;  // the sequence whose CTAs hold blockIdx.x
-    while (hi - lo > 1) {
-        const uint32_t mid = (lo + hi) >> 1;
-        if (P.seq[mid].cta_begin <= blockIdx.x) lo = mid;
-        else hi = mid;
+    const uint32_t slot_id = blockIdx.x / P.kv_heads, kvh = blockIdx.x - slot_id * P.kv_heads;
+    uint32_t lo = 0;
+    if (P.slots <= kMapped) {
+        lo = P.seq_of[slot_id];
+    } else {
+        for (uint32_t hi = P.n; hi - lo > 1;) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (P.seq[mid].slot <= slot_id) lo = mid;
+            else hi = mid;
+        }
     }
     const SeqDev &J = P.seq[lo];
-    const uint32_t G = P.group, local = blockIdx.x - J.cta_begin;
-    const uint32_t kvh = local / J.n_splits, split = local - kvh * J.n_splits;
+    const uint32_t G = P.group, split = slot_id - J.slot;
     const uint32_t row0 = J.start + split * J.split_rows;
     const uint32_t row1 = min(row0 + J.split_rows, J.end);
     const uint64_t row_bytes = (uint64_t)P.kv_heads * St::kRow;
@@ -287,6 +302,14 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         }
         cp_commit();
     };
+    // q is asked for before the stream, so that it does not queue behind it.
+    float4 qx[8];
+    if (warp < NH) {
+        const uint64_t at = (uint64_t)(kvh * G + min(warp * 8u + g, G - 1u)) * 128u;
+#pragma unroll
+        for (uint32_t kk = 0; kk < 8; kk++) qx[kk] = load_row4(J.q, at + St::k_dim(kk, t, 0), P.bf16);
+    }
+    const float gate = tid < G && J.gate ? J.gate[kvh * G + tid] : 0.f;
     // The CTA that covers the last row stores the appended one first, K and V by its
     // last two warps.  A warp whose first stages hold that row starts to load after it.
     const bool appends = J.k_new && row0 < row1 && row1 == J.end;
@@ -316,17 +339,12 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     // integers q * 2^21 or 2^13 in signed digits of 8 bits.
     if (warp < NH) {
         const uint32_t h = warp * 8u + g;
-        float qv[8][4];
         float top = 0.f;
 #pragma unroll
-        for (uint32_t kk = 0; kk < 8; kk++) {
-            const float4 x = load_row4(J.q, (uint64_t)(kvh * G + min(h, G - 1u)) * 128u + St::k_dim(kk, t, 0), P.bf16);
-            qv[kk][0] = x.x;
-            qv[kk][1] = x.y;
-            qv[kk][2] = x.z;
-            qv[kk][3] = x.w;
+        for (int kk = 0; kk < 8; kk++) {
+            const float x[4] = {qx[kk].x, qx[kk].y, qx[kk].z, qx[kk].w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(qv[kk][e]));
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[e]));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -347,7 +365,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                 for (int d = 0; d < ND; d++) w[d] = 0;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float x = qv[kk][e] * f;
+                    const float x = (e == 0 ? qx[kk].x : e == 1 ? qx[kk].y : e == 2 ? qx[kk].z : qx[kk].w) * f;
                     finite = finite && fabsf(x) < 2.f;
                     // bytes of v + 0x80..80 are the digits of v plus 128
                     const uint32_t v = (uint32_t)(__float2int_rn(x * (float)(1 << kBits)) + (ND == 3 ? 0x808080 : 0x8080));
@@ -380,7 +398,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
             for (int kk = 0; kk < 8; kk++)
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
-                    const float x0 = qv[kk][2 * half] * f, x1 = qv[kk][2 * half + 1] * f;
+                    const float x0 = (half ? qx[kk].z : qx[kk].x) * f, x1 = (half ? qx[kk].w : qx[kk].y) * f;
                     const __half2 hv = __floats2half2_rn(x0, x1);
                     const float2 hf = __half22float2(hv);
                     const uint32_t hi = *reinterpret_cast<const uint32_t *>(&hv), lo = h2_bits(x0 - hf.x, x1 - hf.y);
@@ -393,7 +411,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                 }
         }
     }
-    if (tid < 16) gate_s[tid] = tid < G && J.gate ? sigmoid_dev(J.gate[kvh * G + tid]) : 1.f;
+    if (tid < 16) gate_s[tid] = J.gate ? sigmoid_dev(gate) : 1.f;
     __syncthreads();
     if (late) {
 #pragma unroll
@@ -653,8 +671,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 
     // ---- the warps' states to one ----
     float *Os = reinterpret_cast<float *>(smem);  // [warp*16 + head][128]
-    float *Ms = Os + kWarps * 16 * 128, *Ls = Ms + kWarps * 16, *W = Ls + kWarps * 16, *PM = W + kWarps * 16,
-          *PL = PM + 16;
+    float2 *MLs = reinterpret_cast<float2 *>(Os + kWarps * 16 * 128);  // [warp*16 + head] (m, l)
 #pragma unroll
     for (int h = 0; h < NH; h++) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -668,24 +685,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                 const float x = MODE == kWide ? o[0][jt][e + 2 * h] : o[h % NT][jt][e] + o[h % NT][jt][e + 2];
                 Os[os_at(row, St::v_dim(jt, 2u * t + e))] = x * inv;
             }
-        if (t == 0) {
-            Ms[row] = m[h];
-            Ls[row] = l[h];
-        }
-    }
-    __syncthreads();
-    if (tid < G) {
-        float M = kNone, L = 0.f;
-#pragma unroll
-        for (int s = 0; s < kWarps; s++) M = fmaxf(M, Ms[s * 16 + tid]);
-#pragma unroll
-        for (int s = 0; s < kWarps; s++) {
-            const float w = fast_exp2(Ms[s * 16 + tid] - M);
-            W[s * 16 + tid] = w;
-            L += Ls[s * 16 + tid] * w;
-        }
-        PM[tid] = M;
-        PL[tid] = L;
+        if (t == 0) MLs[row] = make_float2(m[h], l[h]);
     }
     __syncthreads();
     const bool single = J.n_splits == 1 && J.pre_splits == 0;
@@ -694,24 +694,23 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     const uint64_t out0 = (uint64_t)kvh * G * 128u;
     for (uint32_t idx = tid; idx < G * 32u; idx += kThreads) {
         const uint32_t h = idx >> 5, d4 = (idx & 31u) * 4u;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float M = kNone, L = 0.f;
 #pragma unroll
+        for (int s = 0; s < kWarps; s++) M = fmaxf(M, MLs[s * 16 + h].x);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int s = 0; s < kWarps; s++) {
-            const float w = W[s * 16 + h];
-            const float4 x = *reinterpret_cast<const float4 *>(Os + os_at(s * 16u + h, d4));
-            a.x = fmaf(x.x, w, a.x);
-            a.y = fmaf(x.y, w, a.y);
-            a.z = fmaf(x.z, w, a.z);
-            a.w = fmaf(x.w, w, a.w);
+            const float2 ml = MLs[s * 16 + h];
+            fold(a, L, *reinterpret_cast<const float4 *>(Os + os_at(s * 16u + h, d4)), ml.y, fast_exp2(ml.x - M));
         }
-        if (single) store_out4(J.out, out0 + idx * 4u, normalise(a, PL[h], gate_s[h]), P.bf16);
+        if (single) store_out4(J.out, out0 + idx * 4u, normalise(a, L, gate_s[h]), P.bf16);
         else __stcg(reinterpret_cast<float4 *>(part + idx * 4u), a);
+        if (!single && (idx & 31u) == 0) __stcg(reinterpret_cast<float2 *>(part + G * 128u + 2u * h), make_float2(M, L));
     }
     // A shared prefix's partials come from the launch before this one, which
     // this kernel may overlap until here (programmatic dependent launch).
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (single) return;
-    if (tid < G) __stcg(reinterpret_cast<float2 *>(part + G * 128u + 2u * tid), make_float2(PM[tid], PL[tid]));
     __syncthreads();
     uint32_t *ctr = P.counters + (uint64_t)lo * P.kv_heads + kvh;
     if (tid == 0) {
@@ -725,28 +724,29 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 
     // ---- the last CTA joins all partials of (sequence, KV head) ----
     const uint32_t n_src = J.n_splits + J.pre_splits;
-    const float *own = P.part + (uint64_t)(J.cta_begin + kvh * J.n_splits) * stride;
+    const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;
     const uint64_t tile0 = (uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh;
     // the partials land in the stages, their (m, l) pairs where q was
     const uint32_t land = (uint32_t)__cvta_generic_to_shared(smem), ml_land = (uint32_t)__cvta_generic_to_shared(Qs);
     const float *ml_s = reinterpret_cast<const float *>(Qs);
     static_assert(kMergePass * 32 * 4 <= 8 * 32 * 16, "(m, l) pairs of a pass");
     const uint32_t per = min(kMergePass, Sh::kArea / (G * 512u));
-    if (tid < 16) {
-        mM[tid] = kNone;
-        mL[tid] = 0.f;
-    }
     constexpr int kPer = (16 * 32 + kThreads - 1) / kThreads;  // float4 outputs of a thread, G <= 16
     float4 acc[kPer];
+    float M[kPer], L[kPer];
 #pragma unroll
-    for (int k = 0; k < kPer; k++) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < kPer; k++) {
+        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        M[k] = kNone;
+        L[k] = 0.f;
+    }
     for (uint32_t s0 = 0; s0 < n_src; s0 += per) {
         const uint32_t cnt = min(per, n_src - s0);
         for (uint32_t s = 0; s < cnt; s++) {
             const uint32_t x = s0 + s;
             const float *po, *pm;
             if (x < J.n_splits) {
-                po = own + (uint64_t)x * stride;
+                po = own + (uint64_t)x * P.kv_heads * stride;
                 pm = po + G * 128u;
             } else {
                 const uint64_t row = (tile0 + (x - J.n_splits)) * 128u + J.pre_row;
@@ -759,47 +759,24 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         cp_commit();
         cp_wait<0>();
         __syncthreads();
-        for (uint32_t h = warp; h < G; h += kWarps) {
-            float ms = -INFINITY, ls = 0.f;
-            if (lane < cnt) {
-                ms = ml_s[lane * 32u + 2u * h];
-                ls = ml_s[lane * 32u + 2u * h + 1u];
-            }
-            const float mo = mM[h];
-            float M = fmaxf(ms, mo);
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-            const float w = fast_exp2(ms - M);
-            float L = ls * w;
-#pragma unroll
-            for (int k = 16; k > 0; k >>= 1) L += __shfl_xor_sync(0xffffffffu, L, k);
-            mw[lane * 16u + h] = w;
-            __syncwarp();
-            if (lane == 0) {
-                const float sc = fast_exp2(mo - M);
-                mScale[h] = sc;
-                mL[h] = mL[h] * sc + L;
-                mM[h] = M;
-            }
-        }
-        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kPer; k++) {
             const uint32_t idx = tid + (uint32_t)k * kThreads;
             if (idx < G * 32u) {
-                const uint32_t h = idx >> 5;
-                const float sc = mScale[h];
-                float4 a = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
+                const float2 *ml = reinterpret_cast<const float2 *>(ml_s) + (idx >> 5);
+                float mn = M[k];
+#pragma unroll 4
+                for (uint32_t s = 0; s < cnt; s++) mn = fmaxf(mn, ml[s * 16u].x);
+                const float sc = fast_exp2(M[k] - mn);
+                M[k] = mn;
+                L[k] *= sc;
+                acc[k] = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
 #pragma unroll 4
                 for (uint32_t s = 0; s < cnt; s++) {
-                    const float w = mw[s * 16u + h];
-                    const float4 x = *reinterpret_cast<const float4 *>(smem + (s * G * 32u + idx) * 16u);
-                    a.x = fmaf(x.x, w, a.x);
-                    a.y = fmaf(x.y, w, a.y);
-                    a.z = fmaf(x.z, w, a.z);
-                    a.w = fmaf(x.w, w, a.w);
+                    const float2 x = ml[s * 16u];
+                    fold(acc[k], L[k], *reinterpret_cast<const float4 *>(smem + (s * G * 32u + idx) * 16u), x.y,
+                         fast_exp2(x.x - mn));
                 }
-                acc[k] = a;
             }
         }
         __syncthreads();
@@ -807,7 +784,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 #pragma unroll
     for (int k = 0; k < kPer; k++) {
         const uint32_t idx = tid + (uint32_t)k * kThreads;
-        if (idx < G * 32u) store_out4(J.out, out0 + idx * 4u, normalise(acc[k], mL[idx >> 5], gate_s[idx >> 5]), P.bf16);
+        if (idx < G * 32u) store_out4(J.out, out0 + idx * 4u, normalise(acc[k], L[k], gate_s[idx >> 5]), P.bf16);
     }
 }
 
@@ -820,7 +797,7 @@ constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256;
 
 struct Plan {
     bool wide;
-    uint32_t ctas;
+    uint32_t slots;
 };
 static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint64_t rows) {
     uint64_t c = 0;
@@ -856,14 +833,18 @@ static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wi
             }
         }
     }
-    plan.ctas = 0;
     for (uint32_t i = 0; i < n; i++) {
         SeqDev &J = seqs[i];
         const uint64_t len = J.end - J.start;
         J.n_splits = (uint32_t)std::max<uint64_t>(1, (len + rows - 1) / rows);
         J.split_rows = (uint32_t)std::max<uint64_t>(u, ((len + J.n_splits - 1) / J.n_splits + u - 1) / u * u);
-        J.cta_begin = plan.ctas;
-        plan.ctas += J.n_splits * kv_heads;
+    }
+    // The longest first: the short ones even out the end.
+    if (!plan.wide) std::sort(seqs, seqs + n, [](const SeqDev &a, const SeqDev &b) { return a.split_rows > b.split_rows; });
+    plan.slots = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        seqs[i].slot = plan.slots;
+        plan.slots += seqs[i].n_splits;
     }
     return plan;
 }
@@ -891,7 +872,7 @@ static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint3
 
 // ------------------------------------------------------------ launches
 template <int MODE, bool I8, bool WIDE, int NJ>
-static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchParams<1> &head, bool after_prefix,
+static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchParams<1> &head, bool after_prefix,
                   cudaStream_t stream) {
     using Sh = Shape<MODE, I8, WIDE>;
     static bool ready[64];
@@ -906,6 +887,9 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchPara
     }
     BatchParams<NJ> P;
     std::copy(seqs, seqs + n, P.seq);
+    for (uint32_t i = 0; i < n && slots <= kMapped; i++)
+        std::fill(P.seq_of + seqs[i].slot, P.seq_of + seqs[i].slot + seqs[i].n_splits, (uint8_t)i);
+    P.slots = slots;
     P.n = n;
     P.group = head.group;
     P.kv_heads = head.kv_heads;
@@ -915,7 +899,7 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t ctas, const BatchPara
     P.pre_part = head.pre_part;
     P.pre_ml = head.pre_ml;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
+    cfg.gridDim = dim3(slots * head.kv_heads);
     cfg.blockDim = dim3(Sh::kThreads);
     cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = stream;
@@ -939,10 +923,10 @@ static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool a
                                   Shape<MODE, I8, false>::kCtas * kPlanSms);
     // The descriptors travel as kernel parameters; a small launch carries few.
     const bool few = n <= kSmallSeqs;
-    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
-    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
-    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
-    return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan.ctas, head, after_prefix, stream);
+    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
+    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
+    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
+    return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
 }
 
 template <bool I8>
