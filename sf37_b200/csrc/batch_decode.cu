@@ -793,22 +793,29 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 // as many splits as fill it.  More pairs: the split whose CTAs, in whole waves of
 // `resident`, cost least, a CTA's start and end counting as kFixedRows rows; a
 // pair's splits are even, and a short pair is one.
-constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256;
+constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256, kWaves = 4;
 
 struct Plan {
     bool wide;
     uint32_t slots;
 };
 static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint64_t rows) {
+    const uint32_t r = (uint32_t)std::min<uint64_t>(rows, kMaxPos);
     uint64_t c = 0;
-    for (uint32_t i = 0; i < n; i++) c += std::max<uint64_t>(1, (seqs[i].end - seqs[i].start + rows - 1) / rows);
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t len = seqs[i].end - seqs[i].start;
+        c += len <= r ? 1u : (len - 1u) / r + 1u;
+    }
     return c;
 }
 static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wide_unit, uint32_t unit,
                         uint32_t resident) {
     Plan plan;
-    uint64_t total = 0;
-    for (uint32_t i = 0; i < n; i++) total += seqs[i].end - seqs[i].start;
+    uint64_t total = 0, longest = 1;
+    for (uint32_t i = 0; i < n; i++) {
+        total += seqs[i].end - seqs[i].start;
+        longest = std::max<uint64_t>(longest, seqs[i].end - seqs[i].start);
+    }
     total *= kv_heads;
     plan.wide = (uint64_t)n * kv_heads <= kPlanSms / 4;
     const uint64_t u = plan.wide ? wide_unit : unit;
@@ -817,21 +824,27 @@ static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wi
         rows = std::max<uint64_t>(1, (total / kPlanSms + u - 1) / u) * u;
         while (plan_ctas(seqs, n, rows) * kv_heads > kPlanSms) rows += std::max<uint64_t>(1, rows / (32 * u)) * u;
     } else {
+        // The smallest split whose CTAs fit w waves, for the w that costs least.  A
+        // guess of half a split lost for each pair keeps the search short.
+        const uint64_t half = (uint64_t)n * kv_heads / 2, least = (total + kMaxCtas - 1) / kMaxCtas;
         uint64_t best = UINT64_MAX;
-        rows = u;
-        for (uint64_t waves = 1; waves <= 8; waves++) {
-            // CTAs of about 1/waves of a slot's share, at most kMaxCtas beyond one for each pair
-            uint64_t r = std::max((total + waves * resident - 1) / (waves * resident), (total + kMaxCtas - 1) / kMaxCtas);
+        rows = longest;
+        const uint64_t w0 = std::max<uint64_t>(1, ((uint64_t)n * kv_heads + resident - 1) / resident);
+        for (uint64_t w = w0; w < w0 + kWaves; w++) {
+            const uint64_t room = w * resident;
+            uint64_t r = std::max<uint64_t>(least, total / (room - half));
             r = std::max<uint64_t>(1, (r + u - 1) / u) * u;
-            for (int k = 0; k < 2; k++, r += std::max<uint64_t>(1, r / (8 * u)) * u) {
-                const uint64_t c = plan_ctas(seqs, n, r) * kv_heads;
-                const uint64_t cost = (c + resident - 1) / resident * (total / c + kFixedRows);
-                if (cost < best) {
-                    best = cost;
-                    rows = r;
-                }
+            uint64_t c = plan_ctas(seqs, n, r) * kv_heads;
+            for (int k = 0; c > room && r < longest; k++, c = plan_ctas(seqs, n, r) * kv_heads)
+                r += std::max<uint64_t>(1, r / ((k < 8 ? 16 : 2) * u)) * u;
+            const uint64_t cost = (c + resident - 1) / resident * (total / c + kFixedRows);
+            if (cost < best) {
+                best = cost;
+                rows = r;
             }
         }
+        rows = std::max(rows, least);
+        rows = std::max<uint64_t>(1, (rows + u - 1) / u) * u;
     }
     for (uint32_t i = 0; i < n; i++) {
         SeqDev &J = seqs[i];
