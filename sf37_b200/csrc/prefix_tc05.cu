@@ -24,6 +24,7 @@
 // raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
 // the largest.  S and O accumulate in f32 (TMEM), m and l in f32 registers.
 #include <algorithm>
+#include <type_traits>
 
 #include "batch_internal.cuh"
 #include "tc05.cuh"
@@ -109,7 +110,11 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
     const uint32_t si = mt * T + sl;             // sequence within the group
     const bool valid = sl < T && si < Gr.n_seqs;
-    const PrefixSeq &Q = P.seq[Gr.seq0 + min(si, Gr.n_seqs - 1u)];
+    // The rows of a warp belong to several sequences: their entries are read by
+    // generic loads, which coalesce (lane-divergent constant loads took 6 us here).
+    const PrefixSeq *tab = P.seq;
+    asm volatile("" : "+l"(tab));
+    const PrefixSeq Q = tab[Gr.seq0 + min(si, Gr.n_seqs - 1u)];
     // Q tiles: scaled by a power of two for each row so that its largest element
     // is in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.
     const bool loads_q = warp < 16 && (!solo || st == 0);
@@ -247,7 +252,8 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
         bool ok = true;
         // One pass over this thread's 64 scores with reference mu: weights (f16 pairs,
         // and their remainders) into w and wl, their sum, the largest x - mu.
-        auto pass = [&](uint32_t k0, bool full, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la, float &xm) {
+        auto pass_of = [&](auto masked, uint32_t k0, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la,
+                           float &xm) {
             float lb = 0.f, xa = -INFINITY, xb = -INFINITY;
             la = 0.f;
 #pragma unroll
@@ -259,7 +265,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     float x0 = fmaf(v[2 * i], qs, -mu), x1 = fmaf(v[2 * i + 1], qs, -mu);
-                    if (!full) {
+                    if (decltype(masked)::value) {
                         const uint32_t kp = kb + 2u * i;
                         if (kp < s_row || kp >= kend) x0 = -INFINITY;
                         if (kp + 1u < s_row || kp + 1u >= kend) x1 = -INFINITY;
@@ -278,6 +284,10 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             }
             la += lb;
             xm = fmaxf(xa, xb);
+        };
+        auto pass = [&](uint32_t k0, bool full, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la, float &xm) {
+            if (full) pass_of(std::false_type(), k0, mu, w, wl, la, xm);
+            else pass_of(std::true_type(), k0, mu, w, wl, la, xm);
         };
         for (uint32_t s = 0; s < n_steps; s++) {
             const uint32_t k0 = kbeg + (solo ? 2u * s + st : s) * 128u;
@@ -340,16 +350,15 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
         if (ok) l = xch[0][st][0][r] + xch[0][st][1][r];
         // Partial tile of (kv head, m tile, split).
         const uint64_t row = ((uint64_t)Gr.part0 + ((uint64_t)kvh * Gr.m_tiles + mt) * Gr.splits + split) * 128u + r;
-        float4 *op = reinterpret_cast<float4 *>(P.part + row * 128u + cb);
         float wA = 1.f;
         const float *ob = reinterpret_cast<const float *>(gsm + T_K * kTile);  // stream 1's O, [128 columns][128 rows]
+        if (hh == 0) {
+            xch[1][st][0][r] = m;
+            xch[1][st][1][r] = l;
+        }
+        asm volatile("bar.sync 9, 512;" ::: "memory");  // both streams' MMAs are done: the K and V tiles are free
         if (solo) {
-            // Join the streams: stream 1 leaves (m, l) and its O, scaled, in the K tiles (all MMAs on them are done).
-            if (hh == 0) {
-                xch[1][st][0][r] = m;
-                xch[1][st][1][r] = l;
-            }
-            asm volatile("bar.sync 9, 512;" ::: "memory");
+            // Join the streams: stream 1 leaves (m, l) and its O, scaled, in the K tiles.
             const float m0 = xch[1][0][0][r], m1 = xch[1][1][0][r], l0 = xch[1][0][1][r], l1 = xch[1][1][1][r];
             const float mj = fmaxf(m0, m1);
             wA = m0 == -INFINITY ? (l0 == 0.f ? 0.f : 1.f) : fast_exp2(m0 - mj);
@@ -370,7 +379,11 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             l = l0 * wA + l1 * wB;
         }
         if (!abort_sh && (!solo || st == 0)) {
+            // O goes through shared memory (16-byte chunk c of row r at c ^ (r & 31)), so that
+            // the global stores are whole rows: stream 0 by the V tiles, stream 1 by the K tiles
+            // (solo: stream 1's O is there until it is added).
             fence_after();
+            uint8_t *stage = gsm + (st == 0 ? T_V : T_K) * kTile + r * 512u;
 #pragma unroll
             for (int q2 = 0; q2 < 2; q2++) {
                 float v[32];
@@ -383,11 +396,20 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
                         if (nt > 1) v[i] += ob[(cb + q2 * 32u + i) * 128u + r];
                     }
                 }
-                if (valid)
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        op[q2 * 8 + i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                for (uint32_t i = 0; i < 8; i++)
+                    *reinterpret_cast<float4 *>(stage + (((cb / 4u + q2 * 8u + i) ^ (r & 31u)) << 4)) =
+                        make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
+            pair_any(false);  // the two warps' halves of 32 rows are in place; each stores 16 of them
+            const uint32_t rows = min(T, Gr.n_seqs - mt * T) * G;  // of the tile's, those that hold a head
+            const uint32_t r0 = (warp & 3u) * 32u + hh * 16u;
+            const uint8_t *tile_sm = gsm + (st == 0 ? T_V : T_K) * kTile;
+            float *tile_out = P.part + (row - r) * 128u;
+#pragma unroll 4
+            for (uint32_t x = r0; x < min(r0 + 16u, rows); x++)
+                *reinterpret_cast<float4 *>(tile_out + x * 128u + lane * 4u) =
+                    *reinterpret_cast<const float4 *>(tile_sm + x * 512u + ((lane ^ (x & 31u)) << 4));
             if (valid && hh == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
         }
     }
