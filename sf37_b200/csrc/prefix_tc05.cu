@@ -103,61 +103,82 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     // next waits before it reads them: it may start as SMs become free.
     asm volatile("griddepcontrol.launch_dependents;");
 
-    const uint32_t st = warp >> 3;               // stream of a softmax warp
-    const uint32_t hh = (warp >> 2) & 1u;        // column half
-    const uint32_t r = ((warp & 3u) << 5) | lane;
-    const uint32_t sl = r / G, hl = r - sl * G;
-    const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
-    const uint32_t si = mt * T + sl;             // sequence within the group
-    const bool valid = sl < T && si < Gr.n_seqs;
-    // The rows of a warp belong to several sequences: their entries are read by
-    // generic loads, which coalesce (lane-divergent constant loads took 6 us here).
+    // Q tiles: scaled by a power of two for each row so that its largest element
+    // is in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.  A warp
+    // reads whole rows, 16 lanes (bf16) or 32 (f32) each: with a row a thread,
+    // 32 lines a load, this start took 8 us.  Rows belong to several sequences;
+    // their table is read by generic loads (lane-divergent constant loads replay).
     const PrefixSeq *tab = P.seq;
     asm volatile("" : "+l"(tab));
-    const PrefixSeq Q = tab[Gr.seq0 + min(si, Gr.n_seqs - 1u)];
-    // Q tiles: scaled by a power of two for each row so that its largest element
-    // is in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.
-    const bool loads_q = warp < 16 && (!solo || st == 0);
-    float qv[64];
-    if (loads_q) {
-        const uint64_t at = (uint64_t)(kvh * G + min(hl, G - 1u)) * 128u + 64u * hh;
-        float top = 0.f;
+    if (warp < 16) {
+        constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
+        const uint32_t per_warp = (solo ? 128u : 256u) / 16u, c = lane % kLanes;
+        uint4 raw[8];
+        float scale[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const float4 x = load_row4(Q.q, at + 4u * i, !F32);
-            qv[4 * i] = x.x;
-            qv[4 * i + 1] = x.y;
-            qv[4 * i + 2] = x.z;
-            qv[4 * i + 3] = x.w;
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t x = warp * per_warp + i * kAtOnce + lane / kLanes;  // row of both tiles
+            if (i * kAtOnce < per_warp) {
+                const uint32_t sl = (x & 127u) / G, hl = (x & 127u) - sl * G;
+                const PrefixSeq q = tab[Gr.seq0 + min((mt0 + (x >> 7)) * T + sl, Gr.n_seqs - 1u)];
+                raw[i] = __ldg(reinterpret_cast<const uint4 *>(q.q) + (uint64_t)(kvh * G + hl) * kLanes + c);
+            }
         }
-        xch[0][st][hh][r] = top;
-    }
-    __syncthreads();
-    if (loads_q) {
-        const float top = fmaxf(xch[0][st][0][r], xch[0][st][1][r]);
-        const int e = max(-126, min(126, (int)((__float_as_uint(top) >> 23) & 255u) - 127));
-        const float f = __int_as_float((127 - e) << 23);
-        if (hh == 0) qscale_sh[st][r] = __int_as_float((127 + e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
-        uint8_t *qt = gsm + (T_Q + (F32 ? 0u : st)) * kTile;
 #pragma unroll
-        for (uint32_t c = 0; c < 8; c++) {
-            uint4 hv, lv;
-            uint32_t *ho = &hv.x, *lo = &lv.x;
+        for (uint32_t i = 0; i < 8; i++) {
+            if (i * kAtOnce < per_warp) {
+                const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float a = qv[8 * c + 2 * i] * f, b = qv[8 * c + 2 * i + 1] * f;
-                ho[i] = pack_h2(a, b);
+                for (int k = 0; k < 4; k++)
+                    top = F32 ? fmaxf(top, fabsf(__uint_as_float(u[k])))
+                              : fmaxf(top, fmaxf(fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xffff0000u))));
+#pragma unroll
+                for (uint32_t k = kLanes / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                scale[i] = top;
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            if (i * kAtOnce < per_warp) {
+                const uint32_t x = warp * per_warp + i * kAtOnce + lane / kLanes, r = x & 127u;
+                const int e = max(-126, min(126, (int)((__float_as_uint(scale[i]) >> 23) & 255u) - 127));
+                const float f = __int_as_float((127 - e) << 23);
+                if (c == 0)
+                    qscale_sh[x >> 7][r] = __int_as_float((127 + e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
+                const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                uint8_t *qt = gsm + (T_Q + (x >> 7)) * kTile;
                 if (F32) {
-                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&ho[i]));
-                    lo[i] = pack_h2(a - h.x, b - h.y);
+                    uint32_t hv[2], lv[2];
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const float a = __uint_as_float(u[2 * k]) * f, b = __uint_as_float(u[2 * k + 1]) * f;
+                        hv[k] = pack_h2(a, b);
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hv[k]));
+                        lv[k] = pack_h2(a - h.x, b - h.y);
+                    }
+                    *reinterpret_cast<uint2 *>(qt + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(hv[0], hv[1]);
+                    *reinterpret_cast<uint2 *>(qt + kTile + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(lv[0], lv[1]);
+                } else {
+                    uint4 hv;
+                    uint32_t *ho = &hv.x;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        ho[k] = pack_h2(__uint_as_float(u[k] << 16) * f, __uint_as_float(u[k] & 0xffff0000u) * f);
+                    *reinterpret_cast<uint4 *>(qt + tile_off(r, c)) = hv;
                 }
             }
-            *reinterpret_cast<uint4 *>(qt + tile_off(r, 8u * hh + c)) = hv;
-            if (F32) *reinterpret_cast<uint4 *>(qt + kTile + tile_off(r, 8u * hh + c)) = lv;
         }
         fence_async_smem();
     }
+    const uint32_t st = warp >> 3;               // stream of a softmax warp
+    const uint32_t hh = (warp >> 2) & 1u;        // column half
+    const uint32_t r = ((warp & 3u) << 5) | lane;
+    const uint32_t sl = r / G;
+    const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
+    const uint32_t si = mt * T + sl;             // sequence within the group
+    const bool valid = sl < T && si < Gr.n_seqs;
+    const uint32_t first = tab[Gr.seq0 + min(si, Gr.n_seqs - 1u)].start;
     fence_before();
     __syncthreads();
     fence_after();
@@ -194,11 +215,13 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
         // S of step i + 2 overwrites the columns from which PV of step i reads P:
         // MMAs issued by one thread execute in order.
         if (lane == 0) {
-            auto issue_s = [&](uint32_t i) -> bool {
+            auto wait_k = [&](uint32_t i) {
+                const uint32_t j = solo ? i : i >> 1;
+                return (!solo && (i & 1u)) || wait_bar(bar(B_KFULL + (j & 1u)), (j >> 1) & 1u);
+            };
+            auto issue_s = [&](uint32_t i) {
                 const uint32_t t = i & 1u, j = solo ? i : i >> 1;
-                if ((solo || t == 0) && !wait_bar(bar(B_KFULL + (j & 1u)), (j >> 1) & 1u)) return false;
                 const uint32_t kt = tile(T_K + (j & 1u)), qt = tile(T_Q + (solo ? 0u : t));
-                fence_after();
 #pragma unroll
                 for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++) {
                     const uint32_t off = ((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u;
@@ -207,25 +230,33 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
                 }
                 commit(bar(B_SFULL + t));
                 if (solo || t == 1) commit(bar(B_KEMPTY + (j & 1u)));
-                return true;
             };
-            auto issue_pv = [&](uint32_t i) -> bool {
+            auto issue_pv = [&](uint32_t i) {
                 const uint32_t t = i & 1u, j = solo ? i : i >> 1;
-                if (!wait_bar(bar(B_PFULL + t), (i >> 1) & 1u)) return false;
-                if ((solo || t == 0) && !wait_bar(bar(B_VFULL + (j & 1u)), (j >> 1) & 1u)) return false;
                 const uint32_t vt = tile(T_V + (j & 1u));
-                fence_after();
 #pragma unroll
                 for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++)
                     mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, sdesc(vt + (kk & 7u) * 2048u, kHalf, 1024),
                            idesc(1), (i > 1 || kk > 0) ? 1u : 0u);
                 commit(bar(B_ODONE + t));
                 if (solo || t == 1) commit(bar(B_VEMPTY + (j & 1u)));
-                return true;
             };
-            bool ok = issue_s(0) && (steps < 2 || issue_s(1));
-            for (uint32_t i = 0; i < steps && ok && !abort_sh; i++)
-                ok = issue_pv(i) && (i + 2 >= steps || issue_s(i + 2));
+            bool ok = true;
+            for (uint32_t i = 0; i < 2 && i < steps && ok; i++) {
+                ok = wait_k(i);
+                fence_after();
+                if (ok) issue_s(i);
+            }
+            // The tiles are waited for before P, so that nothing stands between P and its MMAs.
+            for (uint32_t i = 0; i < steps && ok && !abort_sh; i++) {
+                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
+                ok = (!solo && t) || wait_bar(bar(B_VFULL + (j & 1u)), (j >> 1) & 1u);
+                ok = ok && (i + 2 >= steps || wait_k(i + 2)) && wait_bar(bar(B_PFULL + t), (i >> 1) & 1u);
+                if (!ok) break;
+                fence_after();
+                issue_pv(i);
+                if (i + 2 < steps) issue_s(i + 2);
+            }
             if (!ok) abort_sh = 1;
         }
     } else {
@@ -245,7 +276,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
                 : "memory");
             return rr != 0;
         };
-        const uint32_t s_row = max(Q.start, kbeg);
+        const uint32_t s_row = max(first, kbeg);
         const float qs = qscale_sh[solo ? 0 : st][r];
         const uint32_t n_steps = solo ? (nt + 1u - st) >> 1 : nt;
         float m = -INFINITY, l = 0.f;

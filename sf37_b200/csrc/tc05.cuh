@@ -64,19 +64,23 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;"); }
 
+__device__ __forceinline__ bool try_bar(uint32_t bar, uint32_t phase) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(phase), "r"(kSuspendNs)
+        : "memory");
+    return ok != 0;
+}
 // Bounded parity wait; returns false on timeout.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t phase) {
+    if (try_bar(bar, phase)) return true;
     const long long t0 = clock64();
-    for (;;) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(ok)
-            : "r"(bar), "r"(phase), "r"(kSuspendNs));
-        if (ok) return true;
+    while (!try_bar(bar, phase))
         if (clock64() - t0 > kWaitCycles) return false;
-    }
+    return true;
 }
 
 // Warp-uniform wait: lane 0 polls, the result is broadcast, and the warp is
