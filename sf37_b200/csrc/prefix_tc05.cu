@@ -53,8 +53,8 @@ template <bool F32, int NS>
 __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
     using namespace tc05;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_SFULL = 8, B_PFULL = 10, B_ODONE = 12, N_BARS = 14 };
-    enum { T_Q = 0, T_K = 2, T_V = 4 };  // 32 KB tiles; Q: two tiles (pair) or hi and lo (F32)
+    enum { B_KFULL = 0, B_KEMPTY = 3, B_VFULL = 6, B_VEMPTY = 8, B_SFULL = 10, B_PFULL = 12, B_ODONE = 14, N_BARS = 16 };
+    enum { T_Q = 0, T_K = 2, T_V = 4 };  // 32 KB tiles; Q: two tiles (pair) or hi and lo (F32), else a third K tile
     __shared__ __align__(8) uint64_t bars[N_BARS];
     __shared__ uint32_t tmem_base_sh;
     __shared__ volatile int abort_sh;
@@ -82,9 +82,11 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     const uint32_t steps = solo ? nt : 2u * nt;
 
     if (tid == 0) {
-        for (uint32_t t = 0; t < 2; t++) {
+        for (uint32_t t = 0; t < 3; t++) {
             bar_init(bar(B_KFULL + t), 1);
             bar_init(bar(B_KEMPTY + t), 1);
+        }
+        for (uint32_t t = 0; t < 2; t++) {
             bar_init(bar(B_VFULL + t), 1);
             bar_init(bar(B_VEMPTY + t), 1);
             bar_init(bar(B_SFULL + t), 1);
@@ -185,80 +187,97 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     const uint32_t tmem = tmem_base_sh;
 
     if (warp == 17) {
-        // ---------------- TMA loader: K and V double-buffered ----------------
-        if (lane == 0) {
+        // ---------------- TMA loader: a ring of K tiles and one of V tiles ----------------
+        auto loader = [&](auto kind) {
+            constexpr uint32_t kRing = decltype(kind)::value && !F32 ? 3 : 2, kTile0 = kRing == 3 ? 1 : T_K;
             const int32_t x0 = (int32_t)(kvh * 128u);
-            auto load = [&](uint32_t which, uint32_t j) {  // which: 0 = K, 1 = V
-                const uint32_t b = j & 1u;
+            auto load = [&](uint32_t full, uint32_t dst, const CUtensorMap *map, uint32_t j) {
                 const int32_t y = (int32_t)(kbeg + j * 128u);
-                const uint32_t full = bar((which ? B_VFULL : B_KFULL) + b);
-                const uint32_t dst = tile((which ? T_V : T_K) + b);
-                const CUtensorMap *map = which ? &Gr.vmap : &Gr.kmap;
                 bar_expect_tx(full, kTile);
                 tma_load_2d(dst, map, x0, y, full);
                 tma_load_2d(dst + kHalf, map, x0 + 64, y, full);
             };
-            for (uint32_t j = 0; j < 2 && j < nt; j++) {
-                load(0, j);
-                load(1, j);
+            auto load_k = [&](uint32_t j) { load(bar(B_KFULL + j % kRing), tile(kTile0 + j % kRing), &Gr.kmap, j); };
+            auto load_v = [&](uint32_t j) { load(bar(B_VFULL + (j & 1u)), tile(T_V + (j & 1u)), &Gr.vmap, j); };
+            for (uint32_t j = 0; j < kRing && j < nt; j++) {
+                load_k(j);
+                if (j < 2) load_v(j);
             }
             for (uint32_t j = 0; j + 2 < nt && !abort_sh; j++) {
-                if (!wait_bar(bar(B_KEMPTY + (j & 1u)), (j >> 1) & 1u)) { abort_sh = 1; break; }
-                load(0, j + 2);
+                if (j + kRing < nt) {
+                    if (!wait_bar(bar(B_KEMPTY + j % kRing), (j / kRing) & 1u)) { abort_sh = 1; break; }
+                    load_k(j + kRing);
+                }
                 if (!wait_bar(bar(B_VEMPTY + (j & 1u)), (j >> 1) & 1u)) { abort_sh = 1; break; }
-                load(1, j + 2);
+                load_v(j + 2);
             }
+        };
+        if (lane == 0) {
+            if (solo) loader(std::true_type());
+            else loader(std::false_type());
         }
     } else if (warp == 16) {
         // ---------------- MMA issuer ----------------
-        // Step i belongs to stream i & 1 and key tile i (solo) or i / 2 (pair).
-        // S of step i + 2 overwrites the columns from which PV of step i reads P:
-        // MMAs issued by one thread execute in order.
-        if (lane == 0) {
-            auto wait_k = [&](uint32_t i) {
-                const uint32_t j = solo ? i : i >> 1;
-                return (!solo && (i & 1u)) || wait_bar(bar(B_KFULL + (j & 1u)), (j >> 1) & 1u);
-            };
-            auto issue_s = [&](uint32_t i) {
-                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
-                const uint32_t kt = tile(T_K + (j & 1u)), qt = tile(T_Q + (solo ? 0u : t));
+        // Step i belongs to stream i & 1 and takes key tile i (solo) or i / 2 (pair).  S
+        // of step i + 2 overwrites the columns from which PV of step i reads P: MMAs
+        // issued by one thread execute in order.  The streams wait for this thread,
+        // so it computes little: each kind has its own loop, descriptors are a base
+        // and an offset, and tiles are waited for before P (100 cycles more a step took
+        // 64 x 32768 from 123 to 129 us).
+        auto issuer = [&](auto kind) -> bool {
+            constexpr bool kSolo = decltype(kind)::value;
+            constexpr uint32_t kRing = kSolo && !F32 ? 3 : 2, kTile0 = kRing == 3 ? 1 : T_K, kSteps = F32 ? 16 : 8;
+            const uint64_t qd = sdesc(tile(T_Q), 16, 1024), kd = sdesc(tile(kTile0), 16, 1024),
+                           vd = sdesc(tile(T_V), kHalf, 1024);
+            uint32_t ks = 0, kp = 0, vs = 0, vp = 0;  // next K tile's and V tile's slot and phase
+            auto issue_s = [&](uint32_t t) {
+                const uint64_t a = qd + (kSolo ? 0u : t * (kTile >> 4)), b = kd + ks * (kTile >> 4);
 #pragma unroll
-                for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++) {
-                    const uint32_t off = ((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u;
-                    mma(tmem + t * 128u, sdesc(qt + (kk >> 3) * kTile + off, 16, 1024), sdesc(kt + off, 16, 1024),
-                        idesc(0), kk > 0);
+                for (uint32_t kk = 0; kk < kSteps; kk++) {
+                    const uint32_t off = (((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u) >> 4;
+                    mma(tmem + t * 128u, a + (kk >> 3) * (kTile >> 4) + off, b + off, idesc(0), kk > 0);
                 }
                 commit(bar(B_SFULL + t));
-                if (solo || t == 1) commit(bar(B_KEMPTY + (j & 1u)));
+                if (kSolo || t == 1) {
+                    commit(bar(B_KEMPTY + ks));
+                    if (++ks == kRing) {
+                        ks = 0;
+                        kp ^= 1u;
+                    }
+                }
             };
-            auto issue_pv = [&](uint32_t i) {
-                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
-                const uint32_t vt = tile(T_V + (j & 1u));
+            auto issue_pv = [&](uint32_t t, uint32_t acc, bool last) {
+                const uint64_t b = vd + vs * (kTile >> 4);
 #pragma unroll
-                for (uint32_t kk = 0; kk < (F32 ? 16u : 8u); kk++)
-                    mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, sdesc(vt + (kk & 7u) * 2048u, kHalf, 1024),
-                           idesc(1), (i > 1 || kk > 0) ? 1u : 0u);
-                commit(bar(B_ODONE + t));
-                if (solo || t == 1) commit(bar(B_VEMPTY + (j & 1u)));
+                for (uint32_t kk = 0; kk < kSteps; kk++)
+                    mma_ts(tmem + 256u + t * 128u, tmem + t * 128u + kk * 8u, b + (kk & 7u) * 128u, idesc(1), kk > 0 ? 1u : acc);
+                if (last) commit(bar(B_ODONE + t));
+                if (kSolo || t == 1) {
+                    commit(bar(B_VEMPTY + vs));
+                    vs ^= 1u;
+                    vp ^= vs == 0;
+                }
             };
-            bool ok = true;
-            for (uint32_t i = 0; i < 2 && i < steps && ok; i++) {
-                ok = wait_k(i);
+            for (uint32_t i = 0; i < 2 && i < steps; i++) {
+                if ((kSolo || i == 0) && !wait_bar(bar(B_KFULL + ks), kp)) return false;
                 fence_after();
-                if (ok) issue_s(i);
+                issue_s(i);
             }
-            // The tiles are waited for before P, so that nothing stands between P and its MMAs.
-            for (uint32_t i = 0; i < steps && ok && !abort_sh; i++) {
-                const uint32_t t = i & 1u, j = solo ? i : i >> 1;
-                ok = (!solo && t) || wait_bar(bar(B_VFULL + (j & 1u)), (j >> 1) & 1u);
-                ok = ok && (i + 2 >= steps || wait_k(i + 2)) && wait_bar(bar(B_PFULL + t), (i >> 1) & 1u);
-                if (!ok) break;
+            for (uint32_t i = 0; i < steps && !abort_sh; i++) {
+                const uint32_t t = i & 1u;
+                const bool more = i + 2 < steps;
+                if (kSolo || t == 0) {
+                    if (!wait_bar(bar(B_VFULL + vs), vp)) return false;
+                    if (more && !wait_bar(bar(B_KFULL + ks), kp)) return false;
+                }
+                if (!wait_bar(bar(B_PFULL + t), (i >> 1) & 1u)) return false;
                 fence_after();
-                issue_pv(i);
-                if (i + 2 < steps) issue_s(i + 2);
+                issue_pv(t, i > 1, !more);
+                if (more) issue_s(t);
             }
-            if (!ok) abort_sh = 1;
-        }
+            return true;
+        };
+        if (lane == 0 && !(solo ? issuer(std::true_type()) : issuer(std::false_type()))) abort_sh = 1;
     } else {
         // ---------------- softmax of stream st, column half hh ----------------
         const uint32_t lane_off = ((warp & 3u) * 32u) << 16;
@@ -372,7 +391,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             fence_before();
             bar_arrive(bar(B_PFULL + st));
         }
-        const bool got_e = n_steps == 0 || (ok && !abort_sh && wait_bar_warp(bar(B_ODONE + st), (n_steps - 1) & 1u));
+        const bool got_e = n_steps == 0 || (ok && !abort_sh && wait_bar_warp(bar(B_ODONE + st), 0));
         if (ok) {
             xch[0][st][hh][r] = l;
             if (pair_any(!got_e)) ok = false;
