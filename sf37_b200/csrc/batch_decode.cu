@@ -66,6 +66,7 @@ struct BatchParams {
     uint8_t seq_of[kMapped];  // sequence of a slot; CTA = slot * kv_heads + KV head
     SeqDev seq[NJ];
     uint32_t n, slots, group, kv_heads, bf16;
+    uint32_t join;        // sequences with a prefix are joined by join_kernel
     float *part;          // [cta][part_stride(G)]: O [G][128], then (m, l) [G]
     uint32_t *counters;   // [sequence][kv head]
     const float *pre_part, *pre_ml;
@@ -234,6 +235,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     __shared__ int qoff[2 * NQ][8];  // I8: -128 times the sum of a group's row
     __shared__ uint32_t s_last;
 
+    if (P.join) asm volatile("griddepcontrol.launch_dependents;");  // (join_kernel, which waits)
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     const uint32_t slot_id = blockIdx.x / P.kv_heads, kvh = blockIdx.x - slot_id * P.kv_heads;
     uint32_t lo = 0;
@@ -708,9 +710,11 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         if (!single && (idx & 31u) == 0) __stcg(reinterpret_cast<float2 *>(part + G * 128u + 2u * h), make_float2(M, L));
     }
     // A shared prefix's partials come from the launch before this one, which
-    // this kernel may overlap until here (programmatic dependent launch).
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (single) return;
+    // this kernel may overlap until here (programmatic dependent launch).  With
+    // join_kernel to follow, CTAs do not wait for it but make room for others; the last one
+    // waits, so that this launch does not end before that one.
+    if (!P.join || blockIdx.x + 1u == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (single || (P.join && J.pre_splits)) return;
     __syncthreads();
     uint32_t *ctr = P.counters + (uint64_t)lo * P.kv_heads + kvh;
     if (tid == 0) {
@@ -788,6 +792,79 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     }
 }
 
+// ------------------------------------------------------------ join
+// One CTA per (sequence, KV head) with a shared prefix: its own partials and the
+// prefix's, in that order.  Bound by L2: (splits of both) * G * 520 bytes a CTA.
+template <int NJ>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ BatchParams<NJ> P) {
+    using namespace bd;
+    __shared__ float2 ml_s[32][16];
+    const uint32_t tid = threadIdx.x, G = P.group;
+    const uint32_t lo = blockIdx.x / P.kv_heads, kvh = blockIdx.x - lo * P.kv_heads;
+    const SeqDev &J = P.seq[lo];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (J.pre_splits == 0) return;
+    const uint32_t stride = part_stride(G), n_src = J.n_splits + J.pre_splits;
+    const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;
+    const uint64_t row0 = ((uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh) * 128u + J.pre_row;
+    auto source = [&](uint32_t x) {
+        return x < J.n_splits ? own + (uint64_t)x * P.kv_heads * stride
+                              : P.pre_part + (row0 + (uint64_t)(x - J.n_splits) * 128u) * 128u;
+    };
+    float4 acc[2];
+    float M[2], L[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        M[k] = kNone;
+        L[k] = 0.f;
+    }
+    for (uint32_t s0 = 0; s0 < n_src; s0 += 32u) {
+        const uint32_t cnt = min(32u, n_src - s0);
+        __syncthreads();
+        for (uint32_t i = tid; i < cnt * 16u; i += 256u) {
+            const uint32_t x = s0 + (i >> 4), h = i & 15u;
+            if (h < G)
+                ml_s[i >> 4][h] = __ldcg(x < J.n_splits
+                                             ? reinterpret_cast<const float2 *>(source(x) + G * 128u) + h
+                                             : reinterpret_cast<const float2 *>(P.pre_ml) + row0 +
+                                                   (uint64_t)(x - J.n_splits) * 128u + h);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const uint32_t idx = tid + (uint32_t)k * 256u, h = idx >> 5;
+            if (idx < G * 32u) {
+                float mn = M[k];
+                for (uint32_t s = 0; s < cnt; s++) mn = fmaxf(mn, ml_s[s][h].x);
+                const float sc = fast_exp2(M[k] - mn);
+                M[k] = mn;
+                L[k] *= sc;
+                acc[k] = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
+                for (uint32_t s = 0; s < cnt; s += 8u) {
+                    float4 x[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++)
+                        if (s + i < cnt) x[i] = __ldcg(reinterpret_cast<const float4 *>(source(s0 + s + i)) + idx);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++)
+                        if (s + i < cnt) {
+                            const float2 ml = ml_s[s + i][h];
+                            fold(acc[k], L[k], x[i], ml.y, fast_exp2(ml.x - mn));
+                        }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t idx = tid + (uint32_t)k * 256u, h = idx >> 5;
+        if (idx < G * 32u)
+            store_out4(J.out, (uint64_t)kvh * G * 128u + idx * 4u,
+                       normalise(acc[k], L[k], J.gate ? sigmoid_dev(J.gate[kvh * G + h]) : 1.f), P.bf16);
+    }
+}
+
 // ------------------------------------------------------------ planning
 // Rows of a split.  Few pairs (sequence, KV head): one wave of wide CTAs, with
 // as many splits as fill it.  More pairs: the split whose CTAs, in whole waves of
@@ -809,8 +886,9 @@ static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint64_t rows) {
     return c;
 }
 static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wide_unit, uint32_t unit,
-                        uint32_t resident) {
+                        uint32_t ctas_per_sm, uint32_t sms) {
     Plan plan;
+    const uint32_t resident = ctas_per_sm * sms;
     uint64_t total = 0, longest = 1;
     for (uint32_t i = 0; i < n; i++) {
         total += seqs[i].end - seqs[i].start;
@@ -821,8 +899,9 @@ static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wi
     const uint64_t u = plan.wide ? wide_unit : unit;
     uint64_t rows;
     if (plan.wide) {
-        rows = std::max<uint64_t>(1, (total / kPlanSms + u - 1) / u) * u;
-        while (plan_ctas(seqs, n, rows) * kv_heads > kPlanSms) rows += std::max<uint64_t>(1, rows / (32 * u)) * u;
+        const uint64_t room = std::max<uint64_t>(sms, (uint64_t)n * kv_heads);
+        rows = std::max<uint64_t>(1, (total / room + u - 1) / u) * u;
+        while (plan_ctas(seqs, n, rows) * kv_heads > room) rows += std::max<uint64_t>(1, rows / (32 * u)) * u;
     } else {
         // The smallest split whose CTAs fit w waves, for the w that costs least.  A
         // guess of half a split lost for each pair keeps the search short.
@@ -916,24 +995,36 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchPar
     cfg.blockDim = dim3(Sh::kThreads);
     cfg.dynamicSmemBytes = Sh::kSmem;
     cfg.stream = stream;
-    // After a prefix launch the CTAs start as its CTAs leave, and stream their own
+    // After a prefix launch the CTAs start on the SMs that it leaves, and stream their own
     // rows meanwhile; every CTA waits for that launch before it reads its
-    // partials.  This kernel lets nothing start before its own end.
+    // partials.  This kernel lets nothing but join_kernel start before its own end.
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = after_prefix ? 1 : 0;
+    P.join = after_prefix && !WIDE;
     cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, WIDE, NJ>, P);
     if (e == cudaSuccess) e = cudaGetLastError();
     g_launches++;
+    if (e == cudaSuccess && P.join) {
+        cfg.gridDim = dim3(n * head.kv_heads);
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        e = cudaLaunchKernelEx(&cfg, join_kernel<NJ>, P);
+        if (e == cudaSuccess) e = cudaGetLastError();
+        g_launches++;
+    }
     return check_cuda(e, "decode launch");
 }
 
 template <int MODE, bool I8>
-static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool after_prefix, cudaStream_t stream) {
+static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32_t prefix_ctas,
+                    cudaStream_t stream) {
     const Plan plan = plan_splits(seqs, n, head.kv_heads, Shape<MODE, I8, true>::kUnit, Shape<MODE, I8, false>::kUnit,
-                                  Shape<MODE, I8, false>::kCtas * kPlanSms);
+                                  Shape<MODE, I8, false>::kCtas,
+                                  prefix_ctas < kPlanSms ? kPlanSms - prefix_ctas : kPlanSms);
+    const bool after_prefix = prefix_ctas > 0;
     // The descriptors travel as kernel parameters; a small launch carries few.
     const bool few = n <= kSmallSeqs;
     if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
@@ -943,11 +1034,12 @@ static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool a
 }
 
 template <bool I8>
-static int launch_mode(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, bool after_prefix, cudaStream_t stream) {
-    if (head.group <= 8 && head.bf16 && I8) return launch_n<I8 ? kHalf : kPair, I8>(seqs, n, head, after_prefix, stream);
-    if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, head, after_prefix, stream);
-    if (head.bf16) return launch_n<kWide, I8>(seqs, n, head, after_prefix, stream);
-    return launch_n<kTwo, I8>(seqs, n, head, after_prefix, stream);
+static int launch_mode(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32_t prefix_ctas,
+                    cudaStream_t stream) {
+    if (head.group <= 8 && head.bf16 && I8) return launch_n<I8 ? kHalf : kPair, I8>(seqs, n, head, prefix_ctas, stream);
+    if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, head, prefix_ctas, stream);
+    if (head.bf16) return launch_n<kWide, I8>(seqs, n, head, prefix_ctas, stream);
+    return launch_n<kTwo, I8>(seqs, n, head, prefix_ctas, stream);
 }
 
 static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, uint32_t prefix_len, bool ring_clamp) {
@@ -1082,7 +1174,10 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
                     return set_error(SF37KV_EINVAL, "%s: a cache that one sequence appends to is given twice", what);
                 continue;
             }
-            if (n_pg) prefix_plan(pg, n_pg, q_heads, kv_heads, !head.bf16);
+            uint64_t own = 0;  // rows
+            for (uint32_t k = 0; k < n; k++) own += sd[k].end - sd[k].start;
+            const uint32_t prefix_ctas =
+                n_pg ? prefix_plan(pg, n_pg, q_heads, kv_heads, !head.bf16, own, dtype == SF37KV_I8) : 0;
             for (uint32_t k = 0; k < n; k++) {
                 SeqDev &J = sd[k];
                 J.pre_tile = J.pre_kvh = J.pre_splits = J.pre_row = 0;
@@ -1098,8 +1193,8 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
                 if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
                                               (float *)(ws + W.ml), stream))
                     return rc;
-            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, n_pg > 0, stream)
-                                              : launch_mode<false>(sd, n, head, n_pg > 0, stream);
+            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, prefix_ctas, stream)
+                                              : launch_mode<false>(sd, n, head, prefix_ctas, stream);
             if (rc) return rc;
         }
     }

@@ -104,10 +104,12 @@ struct PrefixGroup {
 // Sequences of one 128-row tile: row sl * G + hl holds head hl of sequence sl.
 static inline uint32_t prefix_seqs_per_tile(uint32_t group) { return 128u / group; }
 
-// Splits each group's rows over CTAs; returns the number of 128-row partial
-// tiles, each 128 x 128 f32 (unnormalised outputs) and 128 (max, sum) pairs.
-// Partial of (kv head h, m tile t, split s): part0 + (h * m_tiles + t) * splits + s.
-uint64_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32);
+// Splits each group's rows over CTAs, considering that the launch that follows
+// reads own_rows own rows (f16 or I8) on the SMs left; returns the number of CTAs.  A partial tile is
+// 128 x 128 f32 (unnormalised outputs) and 128 (reference, sum) pairs; that of
+// (kv head h, m tile t, split s) is part0 + (h * m_tiles + t) * splits + s.
+uint32_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32, uint64_t own_rows,
+                     bool own_i8);
 // Partial tiles that prefix_plan() stays within.
 uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads);
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,

@@ -348,16 +348,30 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             uint32_t w[2][16], wl[2][16];
             float la = 0.f, xm = -INFINITY;
             const float mu0 = m == -INFINITY ? 0.f : m;
-            if (got) pass(k0, full, mu0, w, wl, la, xm);
+            if (got && (F32 || s > 0)) pass(k0, full, mu0, w, wl, la, xm);
+            if (!F32 && got && s == 0) {  // no reference yet: the largest score alone (F32: no registers for it)
+#pragma unroll
+                for (int q2 = 0; q2 < 2; q2++) {
+                    float v[32];
+                    tmem_ld32(t_s + cb + q2 * 32u, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const uint32_t kp = k0 + cb + (uint32_t)(q2 * 32 + i);
+                        if (full || (kp >= s_row && kp < kend)) xm = fmaxf(xm, v[i]);
+                    }
+                }
+                xm *= qs;
+            }
             if (pair_any(!got)) { abort_sh = 1; ok = false; break; }
             const bool need = (m == -INFINITY && xm > -INFINITY) || xm > kRaise;
-            if (pair_any(need)) {
+            if (pair_any(need || (!F32 && s == 0))) {
                 // raise the rows' references: exchange the maximum with the other half, rescale O, redo P
                 xch[s & 1u][st][hh][r] = xm + mu0;
                 pair_any(false);
                 const float mx = fmaxf(xch[s & 1u][st][0][r], xch[s & 1u][st][1][r]) - kHead;
                 const bool raise = mx > -INFINITY && (m == -INFINITY || mx > m + (kRaise - kHead));
-                if (__any_sync(0xffffffffu, raise)) {
+                if (__any_sync(0xffffffffu, raise || (!F32 && s == 0))) {
                     const float alpha = !raise ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - mx);
                     if (s > 0) {
 #pragma unroll
@@ -471,19 +485,28 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------ planning
-// Every CTA takes the same number of key tiles (splits of a group differ by its
-// last): the fewest that fit w waves of one CTA an SM, w the smallest possible or one
-// more, whichever costs less with kFixed tiles' time for a CTA's start and end.
-constexpr uint64_t kFixed = 4;
+// Every CTA takes the same number of key tiles (splits of a group differ by
+// its last).  More CTAs shorten this launch; fewer leave SMs to the launch that
+// reads the sequences' own rows, which runs beside it.  The plan minimises the
+// time of both by measured rates (us): a CTA's start and end, a key tile of two
+// Q tiles or of one (bf16, f32), and the own rows at the rate of HBM or of the SMs left.
+constexpr double kCtaUs = 15.0, kPairUs = 2.35, kSoloUs = 1.5, kSoloF32Us = 2.5;
+constexpr double kHbmBytesUs = 5.8e6, kSmI8BytesUs = 4.6e4, kSmF16BytesUs = 7e4, kOwnUs = 12.0;
 
-uint64_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32) {
+uint32_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t kv_heads, bool f32, uint64_t own_rows,
+                     bool own_i8) {
     const uint32_t T = prefix_seqs_per_tile(q_heads / kv_heads);
-    uint64_t units = 0, work = 0, most = 1;
+    const double own_bytes = (double)own_rows * kv_heads * (own_i8 ? 264.0 : 512.0);
+    const double sm_bytes_us = own_i8 ? kSmI8BytesUs : kSmF16BytesUs;
+    uint64_t units = 0, work = 0, most = 1, pairs = 0;
+    bool pair = false;
     for (uint32_t i = 0; i < n; i++) {
         PrefixGroup &X = groups[i];
         X.m_tiles = (X.n_seqs + T - 1) / T;
+        pair = pair || (!f32 && X.m_tiles > 1);
         const uint64_t ctas = (uint64_t)kv_heads * (f32 ? X.m_tiles : (X.m_tiles + 1) / 2);
         const uint64_t nt = (X.len - X.lo + 127) / 128;
+        pairs += (uint64_t)X.n_seqs * kv_heads;
         units += ctas;
         work += ctas * nt;
         most = std::max(most, nt);
@@ -496,27 +519,47 @@ uint64_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t
         }
         return c;
     };
-    uint64_t best_tps = most, best_cost = UINT64_MAX;
+    const double tile_us = f32 ? kSoloF32Us : pair ? kPairUs : kSoloUs;
+    uint64_t best_tps = most;
+    double best = 1e300;
     const uint64_t w0 = (units + kPlanSms - 1) / kPlanSms;
-    for (uint64_t w = w0; w <= w0 + 1; w++) {
-        uint64_t tps = std::max<uint64_t>(1, (work + w * kPlanSms - 1) / (w * kPlanSms));
-        while (tps < most && ctas_at(tps) > w * kPlanSms) tps += std::max<uint64_t>(1, tps / 32);
+    for (uint64_t room = (w0 + 1) * kPlanSms; room >= units && room > 0;) {
+        uint64_t tps = std::max<uint64_t>(1, (work + room - 1) / room);
+        while (tps < most && ctas_at(tps) > room) tps += std::max<uint64_t>(1, tps / 32);
         tps = std::min(tps, most);
-        const uint64_t cost = (ctas_at(tps) + kPlanSms - 1) / kPlanSms * (tps + kFixed);
-        if (cost < best_cost) {
-            best_cost = cost;
+        const uint64_t c = ctas_at(tps), waves = (c + kPlanSms - 1) / kPlanSms;
+        const double prefix_us = (double)waves * (kCtaUs + (double)tps * tile_us);
+        // few pairs: wide CTAs, one an SM, which wait for this launch themselves
+        const bool wide = pairs <= kPlanSms / 4;
+        const uint64_t free_sms = waves == 1 ? kPlanSms - c : 0, slots = wide ? free_sms : 3 * free_sms;
+        const double alone = kOwnUs + own_bytes / kHbmBytesUs;
+        double beside = 1e300;
+        if (free_sms && !(wide && pairs > slots)) {
+            // more (sequence, KV head) pairs than CTAs run in whole waves of them
+            const double uneven = pairs > slots ? (double)((pairs + slots - 1) / slots * slots) / (double)pairs : 1.0;
+            beside = kOwnUs + std::max(own_bytes / kHbmBytesUs, uneven * own_bytes / ((double)free_sms * sm_bytes_us));
+        }
+        const double cost = std::min(prefix_us + alone, std::max(prefix_us, beside));
+        if (cost < best) {
+            best = cost;
             best_tps = tps;
         }
+        // Next: a second wave's room, a full one, then eight SMs less each time.
+        const uint64_t next = room > w0 * kPlanSms ? w0 * kPlanSms : room - 8;
+        if (room <= 8 || c < room - 8) room = std::min(next, std::max<uint64_t>(c, 1) - 1);
+        else room = next;
+        if (w0 > 1 && room < w0 * kPlanSms) break;
     }
-    uint64_t tiles = 0;
+    uint64_t tiles = 0, ctas = 0;
     for (uint32_t i = 0; i < n; i++) {
         PrefixGroup &X = groups[i];
         X.tiles_per_split = (uint32_t)best_tps;
         X.splits = (uint32_t)(((X.len - X.lo + 127) / 128 + best_tps - 1) / best_tps);
         X.part0 = (uint32_t)tiles;
         tiles += (uint64_t)kv_heads * X.m_tiles * X.splits;
+        ctas += (uint64_t)kv_heads * (f32 ? X.m_tiles : (X.m_tiles + 1) / 2) * X.splits;
     }
-    return tiles;
+    return (uint32_t)ctas;
 }
 
 // CTAs stay within units + 2 * kPlanSms, a CTA has at most two tiles, and
