@@ -46,37 +46,53 @@ __device__ __forceinline__ float4 load_row4(const void *p, uint64_t i, bool bf16
                        __uint_as_float(w.y & 0xffff0000u));
 }
 
-// The integer nearest to x / s, ties to even, decided exactly: x * (1/s) is at
-// most one off, and the remainder x - c*s is an exact f32 (a multiple of the
-// smaller of ulp(x), ulp(s) and at most 1.5 s), so comparing 2r with s is too.
-__device__ __forceinline__ int i8_code(float x, float s, float inv) {
-    int c = __float2int_rn(x * inv);
-    const float r = fmaf(-(float)c, s, x), r2 = r + r;
-    if (r2 > s || (r2 == s && (c & 1))) c++;
-    else if (-r2 > s || (-r2 == s && (c & 1))) c--;
-    return c;
+// max(a, |x|), NaN where either is.
+__device__ __forceinline__ float max_abs_nan(float a, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(x)));
+    return r;
 }
+// The scale of a head whose largest |element| (NaN if one is) is a.
+__device__ __forceinline__ float i8_scale(float a) {
+    if (!(a <= 3.402823466e38f)) return __int_as_float(0x7fc00000);
+    const float s = __fdiv_rn(a, 127.0f);
+    return s < 1.17549435e-38f ? 0.f : s;
+}
+// Byte c + 128 in the low bits: c the integer nearest to x / s, ties to even,
+// decided exactly.  inv = 1 / s.  x * inv + 1.5 * 2^23 rounds to an integer that
+// is at most one off; the remainder x - c*s is an exact f32 (a multiple of the
+// smaller of ulp(x), ulp(s) and at most 1.5 s), so comparing 2r with s is exact too.
+__device__ __forceinline__ uint32_t i8_byte(float x, float s, float inv) {
+    constexpr float kMagic = 12582912.0f + 128.0f;  // the integer's low byte is c + 128
+    const float t = fmaf(x, inv, kMagic), c = t - kMagic;
+    const float r = fmaf(-c, s, x), r2 = r + r;
+    uint32_t b = __float_as_uint(t);
+    if (fabsf(r2) >= s) {  // a tie, or one off (rare)
+        const bool odd = (b & 1u) != 0;
+        if (r2 > s || (r2 == s && odd)) b++;
+        else if (-r2 > s || (-r2 == s && odd)) b--;
+    }
+    return b;
+}
+// Four codes to a word.
+__device__ __forceinline__ uint32_t i8_pack(float x, float y, float z, float w, float s, float inv) {
+    const uint32_t a = __byte_perm(i8_byte(x, s, inv), i8_byte(y, s, inv), 0x0040);
+    const uint32_t b = __byte_perm(i8_byte(z, s, inv), i8_byte(w, s, inv), 0x0040);
+    return __byte_perm(a, b, 0x5410);
+}
+constexpr uint32_t kI8Zero = 0x80808080u;  // four zeros: also the codes of a NaN scale
 
 // Quantises one head (four elements a lane, all 32 lanes) and stores its codes
 // and scale in slot `slot` of an I8 cache.
 __device__ __forceinline__ void store_i8_head(uint8_t *cache, uint32_t cap, uint32_t heads, uint32_t head, uint32_t slot,
                                               uint32_t lane, float4 x) {
-    const bool finite = fabsf(x.x) <= 3.402823466e38f && fabsf(x.y) <= 3.402823466e38f &&
-                        fabsf(x.z) <= 3.402823466e38f && fabsf(x.w) <= 3.402823466e38f;
-    float a = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    float a = max_abs_nan(max_abs_nan(max_abs_nan(fabsf(x.x), x.y), x.z), x.w);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    float s = __fdiv_rn(a, 127.0f);
-    if (s < 1.17549435e-38f) s = 0.f;
-    if (!__all_sync(0xffffffffu, finite)) s = __int_as_float(0x7fc00000);
-    uint32_t w = 0x80808080u;  // zeros: also the codes of a NaN scale
-    if (s > 0.f) {
-        const float inv = __frcp_rn(s);
-        w = (uint32_t)(i8_code(x.x, s, inv) + 128) | ((uint32_t)(i8_code(x.y, s, inv) + 128) << 8) |
-            ((uint32_t)(i8_code(x.z, s, inv) + 128) << 16) | ((uint32_t)(i8_code(x.w, s, inv) + 128) << 24);
-    }
+    for (int o = 16; o > 0; o >>= 1) a = max_abs_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+    const float s = i8_scale(a);
     const uint64_t kv_dim = (uint64_t)heads * 128u;
-    *reinterpret_cast<uint32_t *>(cache + slot * kv_dim + head * 128u + lane * 4u) = w;
+    *reinterpret_cast<uint32_t *>(cache + slot * kv_dim + head * 128u + lane * 4u) =
+        s > 0.f ? i8_pack(x.x, x.y, x.z, x.w, s, __frcp_rn(s)) : kI8Zero;
     if (lane == 0) reinterpret_cast<float *>(cache + cap * kv_dim)[(uint64_t)head * cap + slot] = s;
 }
 

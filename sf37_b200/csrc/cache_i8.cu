@@ -30,25 +30,85 @@ struct AppendI8Job {
 struct AppendI8Params {
     AppendI8Job job[kMaxJobs];
     uint32_t row_begin[kMaxJobs + 1];
-    uint32_t n_jobs, heads, bf16;
+    uint32_t n_jobs, heads, rows_each;  // rows_each: of every job, or 0 where they differ
 };
 
-// One warp per head of one row, K and V together: four elements a lane, so
-// a head's maximum is five shuffles and its codes one 128-byte store.
+// Job of row `row` (or block, by its begin array).
+template <typename Begin>
+__device__ __forceinline__ uint32_t job_of(const Begin &begin, uint32_t n, uint32_t each, uint32_t row) {
+    if (each) return row / each;
+    uint32_t lo = 0;
+    for (uint32_t hi = n; hi - lo > 1;) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (begin[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Eight lanes per head of one row, K and V together: 16 elements a lane in
+// 128-byte runs, all loads first; a head's maximum is three shuffles.  8192 rows of
+// 8 heads, bf16: @APPEND@.
+template <bool BF16>
 __global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
-    const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t unit = (uint64_t)blockIdx.x * 8u + (threadIdx.x >> 5);
-    const uint32_t row = (uint32_t)(unit / P.heads), head = (uint32_t)(unit - (uint64_t)row * P.heads);
-    if (row >= P.row_begin[P.n_jobs]) return;
-    uint32_t j = 0;
-    while (j + 1 < P.n_jobs && P.row_begin[j + 1] <= row) j++;
+    const uint32_t lane8 = threadIdx.x & 7u, unit = blockIdx.x * 32u + (threadIdx.x >> 3);
+    const uint32_t row = unit / P.heads, head = unit - row * P.heads;
+    const bool live = row < P.row_begin[P.n_jobs];
+    const uint32_t j = live ? job_of(P.row_begin, P.n_jobs, P.rows_each, row) : 0u;
     const AppendI8Job &J = P.job[j];
-    const uint32_t t = row - P.row_begin[j];
-    const uint32_t slot = (uint32_t)(((uint64_t)J.pos0 + t) % J.cap);
-    const uint64_t src = ((uint64_t)t * P.heads + head) * 128u + lane * 4u;
-    const float4 k = load_row4(J.k, src, P.bf16), v = load_row4(J.v, src, P.bf16);
-    store_i8_head(J.k_cache, J.cap, P.heads, head, slot, lane, k);
-    store_i8_head(J.v_cache, J.cap, P.heads, head, slot, lane, v);
+    const uint32_t t = live ? row - P.row_begin[j] : 0u;
+    const uint64_t src = ((uint64_t)t * P.heads + head) * 128u;
+    const uint64_t kv_dim = (uint64_t)P.heads * 128u;
+    constexpr uint32_t kRun = BF16 ? 8 : 4, kRuns = 16 / kRun;  // elements of a load, loads
+    uint4 raw[2][kRuns];
+    if (live) {
+#pragma unroll
+        for (uint32_t i = 0; i < kRuns; i++) {
+            const uint64_t at = src + (i * 8u + lane8) * kRun;
+            const uint32_t size = BF16 ? 2u : 4u;
+            raw[0][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.k) + at * size));
+            raw[1][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.v) + at * size));
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kRuns; i++) raw[0][i] = raw[1][i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    const uint32_t slot = (J.pos0 + t) % J.cap;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        float x[16];
+#pragma unroll
+        for (uint32_t i = 0; i < kRuns; i++) {
+            const uint32_t w[4] = {raw[which][i].x, raw[which][i].y, raw[which][i].z, raw[which][i].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (BF16) {
+                    x[(8 * i + 2 * e) & 15] = __uint_as_float(w[e] << 16);
+                    x[(8 * i + 2 * e + 1) & 15] = __uint_as_float(w[e] & 0xffff0000u);
+                } else {
+                    x[(4 * i + e) & 15] = __uint_as_float(w[e]);
+                }
+            }
+        }
+        float a = fabsf(x[0]);
+#pragma unroll
+        for (int e = 1; e < 16; e++) a = max_abs_nan(a, x[e]);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) a = max_abs_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+        const float s = i8_scale(a), inv = s > 0.f ? __frcp_rn(s) : 0.f;
+        uint32_t codes[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            codes[q] = s > 0.f ? i8_pack(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3], s, inv) : kI8Zero;
+        if (!live) continue;
+        uint8_t *cache = which ? J.v_cache : J.k_cache, *dst = cache + slot * kv_dim + head * 128u;
+#pragma unroll
+        for (uint32_t i = 0; i < kRuns; i++) {
+            if (BF16) *reinterpret_cast<uint2 *>(dst + (i * 8u + lane8) * 8u) = make_uint2(codes[(2 * i) & 3], codes[(2 * i + 1) & 3]);
+            else *reinterpret_cast<uint32_t *>(dst + (i * 8u + lane8) * 4u) = codes[i & 3];
+        }
+        if (lane8 == 0) reinterpret_cast<float *>(cache + J.cap * kv_dim)[(uint64_t)head * J.cap + slot] = s;
+    }
 }
 
 // ------------------------------------------------------------ read back
@@ -60,19 +120,20 @@ struct ReadI8Job {
 struct ReadI8Params {
     ReadI8Job job[kMaxJobs];
     uint32_t blk_begin[kMaxJobs + 1];
-    uint32_t n_jobs, heads;
+    uint32_t n_jobs, heads, blks_each;
 };
 
 // One CTA per kReadRows rows of one job's K (blockIdx.y 0) or V (1).  A thread
 // writes 16 bytes at a time, so stores are coalesced and loads are 4 (f32) or
-// 8 (f16) contiguous codes; 32 or 16 neighbouring threads share a scale.
+// 8 (f16) contiguous codes; 32 or 16 neighbouring threads share a scale.  A
+// code becomes f32 as the low bits of 2^23 + c + 128, less 2^23 + 128.  32768 rows of 8
+// heads to f16: @READ@.
 constexpr uint32_t kReadRows = 16;
 
 template <bool F16>
 __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ ReadI8Params P) {
-    constexpr uint32_t E = F16 ? 8u : 4u;  // elements a thread and step
-    uint32_t j = 0;
-    while (j + 1 < P.n_jobs && P.blk_begin[j + 1] <= blockIdx.x) j++;
+    constexpr uint32_t E = F16 ? 8u : 4u, kAtOnce = 4;  // elements a thread and step, steps at once
+    const uint32_t j = job_of(P.blk_begin, P.n_jobs, P.blks_each, blockIdx.x);
     const ReadI8Job &J = P.job[j];
     const uint32_t r0 = (blockIdx.x - P.blk_begin[j]) * kReadRows;
     const uint32_t nr = min(kReadRows, J.rows - r0);
@@ -80,34 +141,40 @@ __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ Re
     void *dst = blockIdx.y ? J.v_dst : J.k_dst;
     const uint64_t kv_dim = (uint64_t)P.heads * 128u;
     const float *scales = reinterpret_cast<const float *>(src + kv_dim * J.src_cap);
-    const uint32_t per_row = P.heads * (128u / E);
-    const uint64_t first = (uint64_t)J.first + r0;
-    const uint32_t s_src = (uint32_t)(first % J.src_cap), s_dst = (uint32_t)(first % J.dst_cap);
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < nr * per_row; i += 256u) {
-        const uint32_t r = i / per_row, c = i - r * per_row;
-        uint32_t a = s_src + r, b = s_dst + r;
-        if (a >= J.src_cap) a %= J.src_cap;
-        if (b >= J.dst_cap) b %= J.dst_cap;
-        const float s = __ldg(scales + (uint64_t)(c / (128u / E)) * J.src_cap + a);
-        const uint8_t *p = src + a * kv_dim + c * E;
-        float x[E];
-        if (F16) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p);
+    const uint32_t per_row = P.heads * (128u / E), n = nr * per_row;
+    const uint32_t s_src = (J.first + r0) % J.src_cap, s_dst = (J.first + r0) % J.dst_cap;
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 256u * kAtOnce) {
+        uint2 w[kAtOnce];
+        float s[kAtOnce];
+        uint64_t to[kAtOnce];
 #pragma unroll
-            for (uint32_t e = 0; e < E; e++) x[e] = (float)((int)(((e < 4 ? w.x : w.y) >> (8u * (e & 3u))) & 255u) - 128) * s;
-            uint4 h;
-            h.x = h2_bits(x[0], x[1]);
-            h.y = h2_bits(x[2], x[3]);
-            h.z = h2_bits(x[4 % E], x[5 % E]);
-            h.w = h2_bits(x[6 % E], x[7 % E]);
-            *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(dst) + b * kv_dim + c * E) = h;
-        } else {
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(p);
+        for (uint32_t k = 0; k < kAtOnce; k++) {
+            const uint32_t i = i0 + k * 256u;
+            if (i < n) {
+                const uint32_t r = i / per_row, c = i - r * per_row;
+                uint32_t a = s_src + r, b = s_dst + r;
+                if (a >= J.src_cap) a = a - J.src_cap < J.src_cap ? a - J.src_cap : a % J.src_cap;
+                if (b >= J.dst_cap) b = b - J.dst_cap < J.dst_cap ? b - J.dst_cap : b % J.dst_cap;
+                s[k] = __ldg(scales + (uint64_t)(c / (128u / E)) * J.src_cap + a);
+                const uint8_t *p = src + a * kv_dim + c * E;
+                if (F16) w[k] = __ldg(reinterpret_cast<const uint2 *>(p));
+                else w[k].x = __ldg(reinterpret_cast<const uint32_t *>(p));
+                to[k] = b * kv_dim + c * E;
+            }
+        }
 #pragma unroll
-            for (uint32_t e = 0; e < E; e++) x[e] = (float)((int)((w >> (8u * e)) & 255u) - 128) * s;
-            *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + b * kv_dim + c * E) =
-                make_float4(x[0], x[1], x[2], x[3]);
+        for (uint32_t k = 0; k < kAtOnce; k++) {
+            if (i0 + k * 256u >= n) continue;
+            float x[8];
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++)
+                x[e] = (__uint_as_float(__byte_perm(e < 4 ? w[k].x : w[k].y, 0x4B000000u, 0x7650u | (e & 3u))) - 8388736.0f) * s[k];
+            if (F16) {
+                *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(dst) + to[k]) =
+                    make_uint4(h2_bits(x[0], x[1]), h2_bits(x[2], x[3]), h2_bits(x[4 % E], x[5 % E]), h2_bits(x[6 % E], x[7 % E]));
+            } else {
+                *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + to[k]) = make_float4(x[0], x[1], x[2], x[3]);
+            }
         }
     }
 }
@@ -152,7 +219,8 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
             AppendI8Params P;
             P.n_jobs = 0;
             P.heads = kv_heads;
-            P.bf16 = row_type == SF37KV_Q_BF16;
+            const bool bf16 = row_type == SF37KV_Q_BF16;
+            P.rows_each = 0;
             uint64_t rows = 0;
             uint32_t i = base;
             const void *seen[2 * kMaxJobs];
@@ -162,12 +230,13 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
                 // With n_tok > cap only the last cap rows stay, as in a sequential append.
                 const uint32_t keep = L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap, skip = L.n_tok - keep;
                 if ((rows + keep) * kv_heads > kMaxUnits) break;
-                const uint64_t off = (uint64_t)skip * kv_heads * 128u * (P.bf16 ? 2u : 4u);
+                const uint64_t off = (uint64_t)skip * kv_heads * 128u * (bf16 ? 2u : 4u);
                 P.job[P.n_jobs] = AppendI8Job{(uint8_t *)L.cache.k_cache, (uint8_t *)L.cache.v_cache,
                                               (const char *)L.k + off, (const char *)L.v + off, L.pos0 + skip,
                                               L.cache.cap};
                 seen[2 * P.n_jobs] = L.cache.k_cache;
                 seen[2 * P.n_jobs + 1] = L.cache.v_cache;
+                P.rows_each = P.n_jobs == 0 || P.rows_each == keep ? keep : 0u;
                 P.row_begin[P.n_jobs++] = (uint32_t)rows;
                 rows += keep;
             }
@@ -179,7 +248,9 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
                 continue;
             }
             P.row_begin[P.n_jobs] = (uint32_t)rows;
-            append_i8_kernel<<<(unsigned)((rows * kv_heads + 7u) / 8u), 256, 0, s>>>(P);
+            const unsigned grid = (unsigned)((rows * kv_heads + 31u) / 32u);
+            if (bf16) append_i8_kernel<true><<<grid, 256, 0, s>>>(P);
+            else append_i8_kernel<false><<<grid, 256, 0, s>>>(P);
             g_launches++;
             if (int rc = check_cuda(cudaGetLastError(), "append_i8 launch")) return rc;
         }
@@ -211,6 +282,7 @@ extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_lay
         ReadI8Params P;
         P.n_jobs = 0;
         P.heads = kv_heads;
+        P.blks_each = 0;
         uint64_t blks = 0;
         uint32_t i = base;
         for (; i < n_layers && P.n_jobs < (uint32_t)kMaxJobs; i++) {
@@ -220,6 +292,7 @@ extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_lay
             if (blks + nb > kMaxUnits) break;
             P.job[P.n_jobs] = ReadI8Job{(const uint8_t *)L.src.k_cache, (const uint8_t *)L.src.v_cache, L.dst.k_cache,
                                         L.dst.v_cache, L.first_pos, L.rows, L.src.cap, L.dst.cap};
+            P.blks_each = P.n_jobs == 0 || P.blks_each == nb ? nb : 0u;
             P.blk_begin[P.n_jobs++] = (uint32_t)blks;
             blks += nb;
         }
