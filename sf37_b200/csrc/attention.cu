@@ -1248,6 +1248,14 @@ static void mark_pre(cudaStream_t s, JobDev *jobs, uint32_t n) {
     }
 }
 
+// Forgets the stream's record: a kernel of another kind that lets its successor
+// start early (batch_decode.cu) was launched on it.
+void stream_record_drop(cudaStream_t s) {
+    std::lock_guard<std::mutex> lk(g_stream_rec_mu);
+    for (StreamRecord &x : g_stream_rec)
+        if (x.used && x.stream == s) x.used = false;
+}
+
 void note_stream_appends(cudaStream_t s, const JobDev *jobs, uint32_t n) {
     std::lock_guard<std::mutex> lk(g_stream_rec_mu);
     StreamRecord *r = nullptr;

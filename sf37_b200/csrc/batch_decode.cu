@@ -66,7 +66,7 @@ struct BatchParams {
     uint8_t seq_of[kMapped];  // sequence of a slot; CTA = slot * kv_heads + KV head
     SeqDev seq[NJ];
     uint32_t n, slots, group, kv_heads, bf16;
-    uint32_t join;        // sequences with a prefix are joined by join_kernel
+    uint32_t after_prefix, join;  // sequences with a prefix are joined by join_kernel
     float *part;          // [cta][part_stride(G)]: O [G][128], then (m, l) [G]
     uint32_t *counters;   // [sequence][kv head]
     const float *pre_part, *pre_ml;
@@ -235,7 +235,11 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     __shared__ int qoff[2 * NQ][8];  // I8: -128 times the sum of a group's row
     __shared__ uint32_t s_last;
 
-    if (P.join) asm volatile("griddepcontrol.launch_dependents;");  // (join_kernel, which waits)
+    // Launched early (programmatic dependent launch), the CTAs wait here for the
+    // kernel before, whatever it was; after a prefix launch, which has itself waited
+    // and writes partials only, they may read caches and q at once.
+    if (!P.after_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     const uint32_t slot_id = blockIdx.x / P.kv_heads, kvh = blockIdx.x - slot_id * P.kv_heads;
     uint32_t lo = 0;
@@ -997,12 +1001,15 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchPar
     cfg.stream = stream;
     // After a prefix launch the CTAs start on the SMs that it leaves, and stream their own
     // rows meanwhile; every CTA waits for that launch before it reads its
-    // partials.  This kernel lets nothing but join_kernel start before its own end.
+    // partials.  Otherwise they start as the kernel before drains, and wait for it.  What follows
+    // may start early too: sf37kv_decode, whose kernels read some caches before they wait, is told.
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = after_prefix ? 1 : 0;
+    cfg.numAttrs = 1;
+    stream_record_drop(stream);
+    P.after_prefix = after_prefix;
     P.join = after_prefix && !WIDE;
     cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, WIDE, NJ>, P);
     if (e == cudaSuccess) e = cudaGetLastError();

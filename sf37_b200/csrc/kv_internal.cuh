@@ -71,6 +71,9 @@ struct AttnJob {
     const sf37kv_qk_prep *prep = nullptr;
 };
 
+// The next decode launch on the stream streams no cache before it waits.
+void stream_record_drop(cudaStream_t stream);
+
 // Launches attention for n jobs (any n; chunked internally).
 // dtype: SF37KV_F32 or SF37KV_F16.  Writes out = softmax(qK^T/sqrt(d))V *
 // sigmoid(gate) per head; an empty row range writes zeros.
