@@ -807,6 +807,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Batch
     const uint32_t lo = blockIdx.x / P.kv_heads, kvh = blockIdx.x - lo * P.kv_heads;
     const SeqDev &J = P.seq[lo];
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     if (J.pre_splits == 0) return;
     const uint32_t stride = part_stride(G), n_src = J.n_splits + J.pre_splits;
     const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;

@@ -101,8 +101,10 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // Nothing but workspace partials is written here, and the kernel launched
-    // next waits before it reads them: it may start as SMs become free.
+    // The kernel before (which may still drain: programmatic dependent launch) is
+    // waited for; then the next one, which reads this kernel's partials after a
+    // wait of its own, may start as SMs become free.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
     // Q tiles: scaled by a power of two for each row so that its largest element
@@ -609,9 +611,20 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
     P.heads_per_kv = q_heads / kv_heads;
     P.kv_heads = kv_heads;
     P.tpt = prefix_seqs_per_tile(P.heads_per_kv);
-    prefix_tc05_kernel<F32, NS><<<ctas, 576, smem, stream>>>(P);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(576);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_tc05_kernel<F32, NS>, P);
+    if (e == cudaSuccess) e = cudaGetLastError();
     g_launches++;
-    return check_cuda(cudaGetLastError(), "prefix launch");
+    return check_cuda(e, "prefix launch");
 }
 
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
