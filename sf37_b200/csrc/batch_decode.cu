@@ -1059,6 +1059,8 @@ static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, u
     if (!aligned16(L.k_new) || !aligned16(L.v_new) || ((uintptr_t)L.gate & 3u))
         return set_error(SF37KV_EINVAL, "%s: sequence %u k_new/v_new must be 16-byte and gate 4-byte aligned", what, i);
     if (L.pos >= kMaxPos) return set_error(SF37KV_EINVAL, "%s: sequence %u position %u exceeds %u", what, i, L.pos, kMaxPos);
+    if (L.k_new && L.cache.sliding && L.cache.window == 0)
+        return set_error(SF37KV_EINVAL, "%s: sequence %u appends to a window of no rows", what, i);
     if (ring_clamp) return SF37KV_OK;
     const uint32_t have = L.pos + 1u;
     if (have < prefix_len)

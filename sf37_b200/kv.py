@@ -251,6 +251,13 @@ def _item(x):
     return x[0]
 
 
+def _records(layers, dtype, name):
+    """Address and length of a descriptor array."""
+    if layers.dtype != dtype or layers.ndim != 1 or not layers.flags.c_contiguous:
+        raise ValueError(f"a contiguous array of {name}() is needed")
+    return layers.ctypes.data, len(layers)
+
+
 def i8_cache_bytes(cap, kv_heads, head_dim=128) -> int:
     """Bytes of one int8 cache of K (or V); allocate it as uint8 (zero-filled or not)."""
     return int(lib().sf37kv_i8_cache_bytes(cap, kv_heads, head_dim))
@@ -270,7 +277,7 @@ def append_i8_desc(k_cache, v_cache, cap, pos0, k, v):
 
 def append_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Quantises the rows of append_i8_desc() into their caches; dtype: the rows' torch dtype."""
-    check(lib().sf37kv_append_i8(layers.ctypes.data, len(layers), kv_heads, head_dim, _IO[dtype], _sp(stream)),
+    check(lib().sf37kv_append_i8(*_records(layers, APPEND_I8_LAYER, "append_i8_desc"), kv_heads, head_dim, _IO[dtype], _sp(stream)),
           "sf37kv_append_i8")
 
 
@@ -288,7 +295,7 @@ def read_i8_desc(k_cache, v_cache, cap, dst_k, dst_v, dst_cap, first_pos, rows):
 
 def read_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Reads the rows of read_i8_desc() back; dtype: the destinations' torch dtype."""
-    check(lib().sf37kv_read_i8(layers.ctypes.data, len(layers), kv_heads, head_dim, _DT[dtype], _sp(stream)),
+    check(lib().sf37kv_read_i8(*_records(layers, READ_I8_LAYER, "read_i8_desc"), kv_heads, head_dim, _DT[dtype], _sp(stream)),
           "sf37kv_read_i8")
 
 
@@ -301,6 +308,11 @@ def decode_seqs_desc(k_cache, v_cache, cap, pos, q, out, gate=None, k_new=None, 
     cache = (torch.uint8, torch.float16)
     d["k_cache"], d["v_cache"] = _addresses("k_cache", k_cache, n, cache), _addresses("v_cache", v_cache, n, cache)
     d["cap"], d["sliding"], d["window"], d["pos"] = cap, np.asarray(sliding, dtype=bool), window, pos
+    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
+        per_row = 132 if _item(c).dtype == torch.uint8 else 128
+        sizes = [_item(c).numel()] * n if isinstance(c, torch.Tensor) else [t.numel() for t in c]
+        if any(s < int(r) * per_row for s, r in zip(sizes, d["cap"])):
+            raise ValueError(f"{name}: smaller than cap rows of one head")
     heads, dtype = _item(q).shape[0], (_item(q).dtype,)
     d["q"], d["out"] = _addresses("q", q, n, tuple(_IO), (heads, 128)), _addresses("out", out, n, dtype, (heads, 128))
     if gate is not None:
@@ -320,7 +332,7 @@ def decode_i8_workspace(n_seqs, q_heads, kv_heads) -> int:
 
 def decode_i8(seqs, q_heads, kv_heads, head_dim, dtype, workspace, stream=None):
     """One decode step over int8 caches; dtype: torch dtype of q and out."""
-    check(lib().sf37kv_decode_i8(seqs.ctypes.data, len(seqs), q_heads, kv_heads, head_dim, _IO[dtype],
+    check(lib().sf37kv_decode_i8(*_records(seqs, DECODE_SEQ, "decode_seqs_desc"), q_heads, kv_heads, head_dim, _IO[dtype],
                                  workspace.data_ptr(), workspace.numel() * workspace.element_size(), _sp(stream)),
           "sf37kv_decode_i8")
 
@@ -335,9 +347,8 @@ def shared_groups_desc(groups):
             d[i]["prefix_k_cache"] = _addresses("prefix k_cache", k, 1, (torch.float16,))[0]
             d[i]["prefix_v_cache"] = _addresses("prefix v_cache", [g["v_cache"]], 1, (torch.float16,))[0]
             d[i]["prefix_cap"] = g["k_cache"].shape[0]
-        if g["seqs"].dtype != DECODE_SEQ or not g["seqs"].flags.c_contiguous:
-            raise ValueError("seqs: a contiguous array of decode_seqs_desc() is needed")
-        d[i]["prefix_len"], d[i]["n_seqs"], d[i]["seqs"] = g["prefix_len"], len(g["seqs"]), g["seqs"].ctypes.data
+        d[i]["prefix_len"] = g["prefix_len"]
+        d[i]["seqs"], d[i]["n_seqs"] = _records(g["seqs"], DECODE_SEQ, "decode_seqs_desc")
     return _Groups(d, [g["seqs"] for g in groups])
 
 

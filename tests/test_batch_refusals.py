@@ -122,6 +122,9 @@ def test_decode_refuses_calls():
     _refused(L.sf37kv_decode_i8(d.ctypes.data, 3, 64, 8, 128, 0, P + 16, need, None), EINVAL, "workspace")
     _refused(L.sf37kv_decode_i8(d.ctypes.data, 3, 64, 8, 128, 0, P, need - 1, None), EINVAL, "workspace")
     d["k_new"][1] = d["v_new"][1] = P
+    d["sliding"][1] = 1
+    _refused(L.sf37kv_decode_i8(d.ctypes.data, 3, 64, 8, 128, 0, P, need, None), EINVAL, "window of no rows")
+    d["sliding"][1] = 0
     d["k_cache"][2] = d["k_cache"][1]
     _refused(L.sf37kv_decode_i8(d.ctypes.data, 3, 64, 8, 128, 0, P, need, None), EINVAL, "twice")
     assert L.sf37kv_decode_i8(None, 0, 64, 8, 128, 0, None, 0, None) == 0
