@@ -128,11 +128,12 @@ def test_descriptor_checks():
         kv.append_i8_desc(raw, raw.clone(), 4, 0, k.half(), k.half())
     with pytest.raises(ValueError, match="CUDA"):
         kv.append_i8_desc(raw, raw.clone(), 4, 0, k.cpu(), k.cpu())
-    d = kv.append_i8_desc(raw, raw.clone(), 4, 0, k, k)
+    other = raw.clone()
+    d = kv.append_i8_desc(raw, other, 4, 0, k, k)
     with pytest.raises(ValueError, match="contiguous array"):
-        kv.append_i8(d[::2], 1, D, k.dtype)
+        kv.append_i8(d[::-1], 1, D, k.dtype)
     with pytest.raises(ValueError, match="contiguous array"):
         kv.read_i8(d, 1, D, torch.float32)
     q = rows(1, 2, 4)
     with pytest.raises(ValueError, match="smaller than cap"):
-        kv.decode_seqs_desc(raw, raw.clone(), 4000, 0, q, q.clone())
+        kv.decode_seqs_desc(raw, other, 4000, 0, q, q.clone())
