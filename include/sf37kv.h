@@ -259,8 +259,9 @@ int sf37kv_decode_i8(const sf37kv_decode_seq *seqs, uint32_t n_seqs, uint32_t q_
  * cache must still hold every own row of the window (else EINVAL), and prefix rows that
  * any sequence of the group attends to must be finite.  prefix_len may be 0.  An I8 prefix is
  * read back once with sf37kv_read_i8.
- * io_type F32 computes to f32 accuracy (queries and weights in two f16 parts);
- * BF16 rounds the weights to f16, which its output's rounding covers.
+ * io_type F32 keeps queries and weights in two f16 parts (outputs are a few
+ * 1e-6 off, by the tensor cores' truncating sums); BF16 rounds the weights to
+ * f16, which its output's rounding covers.
  * Workspace and limits as sf37kv_decode_i8; n_seqs in the workspace query is
  * the total over the groups. */
 typedef struct {

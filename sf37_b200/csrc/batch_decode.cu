@@ -22,9 +22,9 @@
 // not depend on which CTA is last.
 //
 // Sixteen M rows of a tile hold, by MODE:
-//   kPair  G <= 8: eight heads twice, f16 "hi" and remainder "lo" of the weights
+//   kPair  G <= 8, f32: eight heads twice, f16 "hi" and remainder "lo" of the weights
 //          (and of an f16 path's q), 22 bits at no extra cost; I8: q in three digits;
-//   kHalf  the same for I8 and bf16: q in two digits, off by at most 2^-14 of the
+//   kHalf  G <= 8, bf16: the same; I8: q in two digits, off by at most 2^-14 of the
 //          head's largest power of two (a bf16 q itself by 2^-8 of each element);
 //   kWide  G <= 16 and bf16: sixteen heads, weights rounded to f16 (half a step is
 //          2^-11 of a weight; the output's own rounding has 2^-8), I8: two digits;
@@ -42,6 +42,9 @@ enum { kPair = 0, kHalf = 1, kWide = 2, kTwo = 3 };
 
 constexpr float kSlack = 8.0f;
 constexpr float kNone = -1e30f;  // reference of a state without rows
+// The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each block (measured),
+// 9e-6 over 512 of them.  f32 outputs take O into sums of their own after this many.
+constexpr uint32_t kTake = 32;
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
 constexpr uint32_t kMapped = 1024;     // slots with a direct map to their sequence
@@ -198,18 +201,18 @@ struct Stage {
 };
 
 // Warps of a CTA, CTAs of an SM and stages of a warp.  An SM runs 12 warps (8 in
-// kTwo, for their registers), either as CTAs of four, which hide each other's
+// kTwo, for their registers, and with f32 outputs over f16 caches, for the sums' memory), either as CTAs of four, which hide each other's
 // starts and ends, or as one wide CTA, which leaves fewer partials to join.
 // More stages only lengthen the queue to HBM, and with it every other access:
 // 8 layers x 32769 rows of I8 took 95 us with three stages, 100 with four, 102
 // with two; f16 rows 76 us with two stages of 12 warps, 80 with three of 8.
 template <int MODE, bool I8, bool WIDE>
 struct Shape {
-    static constexpr int kSmWarps = MODE != kTwo ? 12 : 8;
+    static constexpr int kSmWarps = MODE == kTwo || (MODE == kPair && !I8) ? 8 : 12;
     static constexpr int kWarps = WIDE ? kSmWarps : 4;
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kCtas = kSmWarps / kWarps;
-    static constexpr int kStages = (I8 ? 3 : 2) + (MODE == kTwo ? 1 : 0);
+    static constexpr int kStages = !I8 ? 2 : MODE == kTwo ? 4 : 3;
     static constexpr uint32_t kUnit = kWarps * 16;  // rows that the warps take at once
     static constexpr uint32_t kArea = kWarps * kStages * Stage<I8>::kBytes;
     // q: an I8 q in kDigits digits of 8 bits, eight rows (a group) each, two groups a
@@ -217,7 +220,11 @@ struct Shape {
     static constexpr int kDigits = MODE == kHalf || MODE == kWide ? 2 : 3;
     static constexpr int kGroups = kDigits * (MODE == kWide || MODE == kTwo ? 2 : 1);
     static constexpr int kQTiles = I8 ? (kGroups + 1) / 2 : MODE == kTwo ? 2 : 1;
-    static constexpr uint32_t kSmem = kArea + (8 * 32 * 16) * (!I8 && MODE == kTwo ? 2 : I8 && kQTiles > 2 ? 2 : 1);
+    static constexpr uint32_t kQArea = (8 * 32 * 16) * (!I8 && MODE == kTwo ? 2 : I8 && kQTiles > 2 ? 2 : 1);
+    // f32 outputs: sums of O out of the tensor core's accumulators, one float a lane each
+    static constexpr int kSums = MODE == kPair ? 32 : MODE == kTwo ? 64 : 0;
+    static constexpr uint32_t kSmem = kArea + kQArea + kWarps * kSums * 32 * 4;
+    static_assert(kCtas * (kSmem + 2048) <= 228 * 1024, "CTAs of an SM");
 };
 
 template <int MODE, bool I8, bool WIDE, int NJ>
@@ -448,7 +455,25 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         f[h] = I8 ? pow2(kFMax) : 128.f;
     }
 
+    // f32 outputs: this lane's sums of O (the two parts of a weight joined)
+    float *sums = reinterpret_cast<float *>(smem + Sh::kArea + Sh::kQArea) + warp * (Sh::kSums * 32) + lane;
+    bool taken = false;
+    auto take = [&]() {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float *x = sums + ((n * 16 + i) * 2 + e) * 32;
+                    *x = (taken ? *x : 0.f) + (o[n][i][e] + o[n][i][e + 2]);
+                    o[n][i][e] = o[n][i][e + 2] = 0.f;
+                }
+        taken = true;
+    };
+
     for (uint32_t it = 0; it < nblk; it++) {
+        if (Sh::kSums && it > 0 && it % kTake == 0) take();
         cp_wait<S - 2>();
         __syncwarp();
         issue(it + S - 1);
@@ -609,6 +634,9 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                 for (int i = 0; i < 16; i++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) o[n][i][e] *= MODE == kWide ? fac[(e >> 1) % NH] : fac[n % NH];
+            if (Sh::kSums && taken)
+#pragma unroll 4
+                for (int x = 0; x < Sh::kSums; x++) sums[x * 32] *= fac[(x >> 5) % NH];
         }
         uint32_t pa[NT][4];
 #pragma unroll
@@ -688,7 +716,8 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         for (uint32_t jt = 0; jt < 16; jt++)
 #pragma unroll
             for (uint32_t e = 0; e < 2; e++) {
-                const float x = MODE == kWide ? o[0][jt][e + 2 * h] : o[h % NT][jt][e] + o[h % NT][jt][e + 2];
+                float x = MODE == kWide ? o[0][jt][e + 2 * h] : o[h % NT][jt][e] + o[h % NT][jt][e + 2];
+                if (Sh::kSums && taken) x += sums[((h % NT) * 32 + jt * 2 + e) * 32];
                 Os[os_at(row, St::v_dim(jt, 2u * t + e))] = x * inv;
             }
         if (t == 0) MLs[row] = make_float2(m[h], l[h]);
@@ -1044,7 +1073,7 @@ static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32
 template <bool I8>
 static int launch_mode(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32_t prefix_ctas,
                     cudaStream_t stream) {
-    if (head.group <= 8 && head.bf16 && I8) return launch_n<I8 ? kHalf : kPair, I8>(seqs, n, head, prefix_ctas, stream);
+    if (head.group <= 8 && head.bf16) return launch_n<kHalf, I8>(seqs, n, head, prefix_ctas, stream);
     if (head.group <= 8) return launch_n<kPair, I8>(seqs, n, head, prefix_ctas, stream);
     if (head.bf16) return launch_n<kWide, I8>(seqs, n, head, prefix_ctas, stream);
     return launch_n<kTwo, I8>(seqs, n, head, prefix_ctas, stream);

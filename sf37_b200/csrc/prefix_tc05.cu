@@ -13,9 +13,9 @@
 // K/V tile; with one (solo) the streams take alternate K/V tiles of the same
 // Q tile and are joined through shared memory at the end.
 //
-// Warps 0-7 and 8-15 are the softmax of stream 0 and 1, two threads for each
-// row (64 score columns each); warp 16 issues the MMAs, warp 17 the TMA loads,
-// as in prefill_tc05.cu.  TMEM: S_0, S_1, O_0, O_1 (128 columns each); P
+// Warps 0-3 and 4-7 are the softmax of stream 0 and 1, one row a thread (two
+// threads a row, as in prefill_tc05.cu, were as fast in bf16, but left F32 no registers); warp 8
+// issues the MMAs, warp 9 the TMA loads.  TMEM: S_0, S_1, O_0, O_1 (128 columns each); P
 // (f16) overwrites its S.  F32 (f32 queries and outputs): q and P are two
 // f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits: twice the MMAs; P_lo
 // takes the second half of S's columns.
@@ -44,13 +44,84 @@ struct PrefixParams {
     PrefixDev group[kPrefixGroups];
     PrefixSeq seq[NS];
     float *part, *ml;
+    uint32_t take0;  // first of one partial tile for each CTA, for stream 1's sums (F32)
     uint32_t n_groups, heads_per_kv, kv_heads, tpt;
 };
 
 constexpr float kHead = 7.0f, kRaise = 15.0f;
+constexpr float kNone = -1e30f;  // reference of a row without keys
+// The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each MMA (measured).
+// F32 takes O into sums in memory after this many key tiles of a stream (256 MMAs, 4e-6; 16000
+// keys, 40 sequences: 99 us with half as many, 85 with none).
+constexpr uint32_t kTake = 16;
+
+// Q tiles: scaled by a power of two for each row so that its largest element is
+// in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.  Of the
+// 8 warps each reads whole rows, 16 lanes (bf16) or 32 (f32) each: with a row a
+// thread, 32 lines a load, this took 8 us.  `rows` is 128 or 256 (two tiles).
+template <bool F32>
+__device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, uint32_t mt0, uint32_t rows, uint32_t kvh,
+                                    uint32_t G, uint32_t T, uint8_t *tiles, float *qscale) {
+    using namespace tc05;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+            constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
+    const uint32_t c = lane % kLanes;
+    for (uint32_t x0 = warp * (rows / 8u); x0 < (warp + 1u) * (rows / 8u); x0 += 8u * kAtOnce) {
+        uint4 raw[8];
+        float scale[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t x = x0 + i * kAtOnce + lane / kLanes;  // row of both tiles
+            const uint32_t sl = (x & 127u) / G, hl = (x & 127u) - sl * G;
+            const PrefixSeq q = tab[min((mt0 + (x >> 7)) * T + sl, n_seqs - 1u)];
+            raw[i] = __ldg(reinterpret_cast<const uint4 *>(q.q) + (uint64_t)(kvh * G + hl) * kLanes + c);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                top = F32 ? fmaxf(top, fabsf(__uint_as_float(u[k])))
+                          : fmaxf(top, fmaxf(fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xffff0000u))));
+#pragma unroll
+            for (uint32_t k = kLanes / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+            scale[i] = top;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t x = x0 + i * kAtOnce + lane / kLanes, r = x & 127u;
+            const int e = max(-126, min(126, (int)((__float_as_uint(scale[i]) >> 23) & 255u) - 127));
+            const float f = __int_as_float((127 - e) << 23);
+            if (c == 0) qscale[x] = __int_as_float((127 + e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
+            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            uint8_t *qt = tiles + (x >> 7) * kTile;
+            if (F32) {
+                uint32_t hv[2], lv[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const float a = __uint_as_float(u[2 * k]) * f, b = __uint_as_float(u[2 * k + 1]) * f;
+                    hv[k] = pack_h2(a, b);
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hv[k]));
+                    lv[k] = pack_h2(a - h.x, b - h.y);
+                }
+                *reinterpret_cast<uint2 *>(qt + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(hv[0], hv[1]);
+                *reinterpret_cast<uint2 *>(qt + kTile + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(lv[0], lv[1]);
+            } else {
+                uint4 hv;
+                uint32_t *ho = &hv.x;
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    ho[k] = pack_h2(__uint_as_float(u[k] << 16) * f, __uint_as_float(u[k] & 0xffff0000u) * f);
+                *reinterpret_cast<uint4 *>(qt + tile_off(r, c)) = hv;
+            }
+        }
+    }
+    fence_async_smem();
+}
 
 template <bool F32, int NS>
-__global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
+__global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
     using namespace tc05;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     enum { B_KFULL = 0, B_KEMPTY = 3, B_VFULL = 6, B_VEMPTY = 8, B_SFULL = 10, B_PFULL = 12, B_ODONE = 14, N_BARS = 16 };
@@ -58,7 +129,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     __shared__ __align__(8) uint64_t bars[N_BARS];
     __shared__ uint32_t tmem_base_sh;
     __shared__ volatile int abort_sh;
-    __shared__ float xch[2][2][2][128];  // [parity][stream][half][row]
+    __shared__ float2 ml_sh[2][128];  // [stream][row] (m, l)
     __shared__ float qscale_sh[2][128];
 
     const uint32_t sraw = (uint32_t)__cvta_generic_to_shared(smem_raw);
@@ -90,7 +161,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             bar_init(bar(B_VFULL + t), 1);
             bar_init(bar(B_VEMPTY + t), 1);
             bar_init(bar(B_SFULL + t), 1);
-            bar_init(bar(B_PFULL + t), 256);
+            bar_init(bar(B_PFULL + t), 128);
             bar_init(bar(B_ODONE + t), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;");
@@ -107,80 +178,16 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // Q tiles: scaled by a power of two for each row so that its largest element
-    // is in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.  A warp
-    // reads whole rows, 16 lanes (bf16) or 32 (f32) each: with a row a thread,
-    // 32 lines a load, this start took 8 us.  Rows belong to several sequences;
-    // their table is read by generic loads (lane-divergent constant loads replay).
+    // The sequences' table is read by generic loads: lane-divergent constant loads replay.
     const PrefixSeq *tab = P.seq;
     asm volatile("" : "+l"(tab));
-    if (warp < 16) {
-        constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
-        const uint32_t per_warp = (solo ? 128u : 256u) / 16u, c = lane % kLanes;
-        uint4 raw[8];
-        float scale[8];
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t x = warp * per_warp + i * kAtOnce + lane / kLanes;  // row of both tiles
-            if (i * kAtOnce < per_warp) {
-                const uint32_t sl = (x & 127u) / G, hl = (x & 127u) - sl * G;
-                const PrefixSeq q = tab[Gr.seq0 + min((mt0 + (x >> 7)) * T + sl, Gr.n_seqs - 1u)];
-                raw[i] = __ldg(reinterpret_cast<const uint4 *>(q.q) + (uint64_t)(kvh * G + hl) * kLanes + c);
-            }
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            if (i * kAtOnce < per_warp) {
-                const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                float top = 0.f;
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    top = F32 ? fmaxf(top, fabsf(__uint_as_float(u[k])))
-                              : fmaxf(top, fmaxf(fabsf(__uint_as_float(u[k] << 16)), fabsf(__uint_as_float(u[k] & 0xffff0000u))));
-#pragma unroll
-                for (uint32_t k = kLanes / 2; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-                scale[i] = top;
-            }
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            if (i * kAtOnce < per_warp) {
-                const uint32_t x = warp * per_warp + i * kAtOnce + lane / kLanes, r = x & 127u;
-                const int e = max(-126, min(126, (int)((__float_as_uint(scale[i]) >> 23) & 255u) - 127));
-                const float f = __int_as_float((127 - e) << 23);
-                if (c == 0)
-                    qscale_sh[x >> 7][r] = __int_as_float((127 + e) << 23) * (1.4426950408889634f * 0.08838834764831845f);
-                const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                uint8_t *qt = gsm + (T_Q + (x >> 7)) * kTile;
-                if (F32) {
-                    uint32_t hv[2], lv[2];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const float a = __uint_as_float(u[2 * k]) * f, b = __uint_as_float(u[2 * k + 1]) * f;
-                        hv[k] = pack_h2(a, b);
-                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hv[k]));
-                        lv[k] = pack_h2(a - h.x, b - h.y);
-                    }
-                    *reinterpret_cast<uint2 *>(qt + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(hv[0], hv[1]);
-                    *reinterpret_cast<uint2 *>(qt + kTile + tile_off(r, c >> 1) + 8u * (c & 1u)) = make_uint2(lv[0], lv[1]);
-                } else {
-                    uint4 hv;
-                    uint32_t *ho = &hv.x;
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        ho[k] = pack_h2(__uint_as_float(u[k] << 16) * f, __uint_as_float(u[k] & 0xffff0000u) * f);
-                    *reinterpret_cast<uint4 *>(qt + tile_off(r, c)) = hv;
-                }
-            }
-        }
-        fence_async_smem();
-    }
-    const uint32_t st = warp >> 3;               // stream of a softmax warp
-    const uint32_t hh = (warp >> 2) & 1u;        // column half
+    if (warp < 8)
+        load_q<F32>(tab + Gr.seq0, Gr.n_seqs, mt0, solo ? 128u : 256u, kvh, G, T, gsm + T_Q * kTile, &qscale_sh[0][0]);
+    const uint32_t st = warp >> 2;  // stream of a softmax warp
     const uint32_t r = ((warp & 3u) << 5) | lane;
     const uint32_t sl = r / G;
     const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
-    const uint32_t si = mt * T + sl;             // sequence within the group
+    const uint32_t si = mt * T + sl;  // sequence within the group
     const bool valid = sl < T && si < Gr.n_seqs;
     const uint32_t first = tab[Gr.seq0 + min(si, Gr.n_seqs - 1u)].start;
     fence_before();
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
     fence_after();
     const uint32_t tmem = tmem_base_sh;
 
-    if (warp == 17) {
+    if (warp == 9) {
         // ---------------- TMA loader: a ring of K tiles and one of V tiles ----------------
         auto loader = [&](auto kind) {
             constexpr uint32_t kRing = decltype(kind)::value && !F32 ? 3 : 2, kTile0 = kRing == 3 ? 1 : T_K;
@@ -218,7 +225,7 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
             if (solo) loader(std::true_type());
             else loader(std::false_type());
         }
-    } else if (warp == 16) {
+    } else if (warp == 8) {
         // ---------------- MMA issuer ----------------
         // Step i belongs to stream i & 1 and takes key tile i (solo) or i / 2 (pair).  S
         // of step i + 2 overwrites the columns from which PV of step i reads P: MMAs
@@ -236,8 +243,9 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
                 const uint64_t a = qd + (kSolo ? 0u : t * (kTile >> 4)), b = kd + ks * (kTile >> 4);
 #pragma unroll
                 for (uint32_t kk = 0; kk < kSteps; kk++) {
-                    const uint32_t off = (((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u) >> 4;
-                    mma(tmem + t * 128u, a + (kk >> 3) * (kTile >> 4) + off, b + off, idesc(0), kk > 0);
+                    // F32: the remainders' products first, so that they are not cut off a large sum
+                    const uint32_t off = (((kk >> 2) & 1u) * kHalf + (kk & 3u) * 32u) >> 4, lo = F32 ? 1u - (kk >> 3) : 0u;
+                    mma(tmem + t * 128u, a + lo * (kTile >> 4) + off, b + off, idesc(0), kk > 0);
                 }
                 commit(bar(B_SFULL + t));
                 if (kSolo || t == 1) {
@@ -274,209 +282,191 @@ __global__ void __launch_bounds__(576, 1) prefix_tc05_kernel(const __grid_consta
                 }
                 if (!wait_bar(bar(B_PFULL + t), (i >> 1) & 1u)) return false;
                 fence_after();
-                issue_pv(t, i > 1, !more);
+                issue_pv(t, F32 ? (i >> 1) % kTake != 0 : i > 1, !more);
                 if (more) issue_s(t);
             }
             return true;
         };
         if (lane == 0 && !(solo ? issuer(std::true_type()) : issuer(std::false_type()))) abort_sh = 1;
     } else {
-        // ---------------- softmax of stream st, column half hh ----------------
+        // ---------------- softmax of stream st, one row a thread ----------------
         const uint32_t lane_off = ((warp & 3u) * 32u) << 16;
-        const uint32_t cb = 64u * hh;
         const uint32_t t_s = tmem + st * 128u + lane_off, t_o = tmem + 256u + st * 128u + lane_off;
-        const uint32_t pair_bar = 1u + st * 4u + (warp & 3u);  // the two warps that share these rows
-        // Pair barrier that also ORs a flag, so both warps take the same exit.
-        auto pair_any = [&](bool v) -> bool {
-            uint32_t rr;
-            asm volatile(
-                "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-                "bar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
-                : "=r"(rr)
-                : "r"((uint32_t)v), "r"(pair_bar)
-                : "memory");
-            return rr != 0;
-        };
         const uint32_t s_row = max(first, kbeg);
         const float qs = qscale_sh[solo ? 0 : st][r];
         const uint32_t n_steps = solo ? (nt + 1u - st) >> 1 : nt;
-        float m = -INFINITY, l = 0.f;
+        float m = kNone, l = 0.f;
         bool ok = true;
-        // One pass over this thread's 64 scores with reference mu: weights (f16 pairs,
-        // and their remainders) into w and wl, their sum, the largest x - mu.
-        auto pass_of = [&](auto masked, uint32_t k0, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la,
-                           float &xm) {
-            float lb = 0.f, xa = -INFINITY, xb = -INFINITY;
-            la = 0.f;
+        // Partial tile of (kv head, m tile, split); F32: this thread's sums of O, relative to
+        // 2^m_taken (stream 0's in the partial tile that it writes at the end).
+        const uint64_t row = ((uint64_t)Gr.part0 + ((uint64_t)kvh * Gr.m_tiles + mt) * Gr.splits + split) * 128u + r;
+        float *sums = P.part + (st == 0 ? row - r : ((uint64_t)P.take0 + blockIdx.x) * 128u) * 128u + r;  // [column][row]
+        float m_taken = kNone;
+        // 32 columns of O and of the sums
+        auto read_o = [&](int c, bool add, float scale, float (&v)[32]) {
+            tmem_ld32(t_o + c * 32u, v);
+            tmem_wait_ld();
+            if (add) {
 #pragma unroll
-            for (int q2 = 0; q2 < 2; q2++) {
-                float v[32];
-                tmem_ld32(t_s + cb + q2 * 32u, v);
-                tmem_wait_ld();
-                const uint32_t kb = k0 + cb + (uint32_t)(q2 * 32);
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float x0 = fmaf(v[2 * i], qs, -mu), x1 = fmaf(v[2 * i + 1], qs, -mu);
-                    if (decltype(masked)::value) {
-                        const uint32_t kp = kb + 2u * i;
-                        if (kp < s_row || kp >= kend) x0 = -INFINITY;
-                        if (kp + 1u < s_row || kp + 1u >= kend) x1 = -INFINITY;
-                    }
-                    xa = fmaxf(xa, x0);
-                    xb = fmaxf(xb, x1);
-                    const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                    la += p0;
-                    lb += p1;
-                    w[q2][i] = pack_h2(p0, p1);
-                    if (F32) {
-                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[q2][i]));
-                        wl[q2][i] = pack_h2(p0 - h.x, p1 - h.y);
-                    }
-                }
+                for (int i = 0; i < 32; i++) v[i] = fmaf(sums[(c * 32 + i) * 128], scale, v[i]);
             }
-            la += lb;
-            xm = fmaxf(xa, xb);
-        };
-        auto pass = [&](uint32_t k0, bool full, float mu, uint32_t (&w)[2][16], uint32_t (&wl)[2][16], float &la, float &xm) {
-            if (full) pass_of(std::false_type(), k0, mu, w, wl, la, xm);
-            else pass_of(std::true_type(), k0, mu, w, wl, la, xm);
         };
         for (uint32_t s = 0; s < n_steps; s++) {
             const uint32_t k0 = kbeg + (solo ? 2u * s + st : s) * 128u;
             __syncwarp();
-            const bool got = !abort_sh && wait_bar_warp(bar(B_SFULL + st), s & 1u);
+            ok = !abort_sh && wait_bar_warp(bar(B_SFULL + st), s & 1u);
+            if (!ok) break;
             fence_after();
-            const bool full = __all_sync(0xffffffffu, k0 >= s_row && k0 + 128u <= kend);
-            uint32_t w[2][16], wl[2][16];
-            float la = 0.f, xm = -INFINITY;
-            const float mu0 = m == -INFINITY ? 0.f : m;
-            if (got && (F32 || s > 0)) pass(k0, full, mu0, w, wl, la, xm);
-            if (!F32 && got && s == 0) {  // no reference yet: the largest score alone (F32: no registers for it)
+            if (F32 && s > 0 && s % kTake == 0) {  // PV of this step starts O anew
+                const float scale = fast_exp2(m_taken - m);
 #pragma unroll
-                for (int q2 = 0; q2 < 2; q2++) {
+                for (int c = 0; c < 4; c++) {
                     float v[32];
-                    tmem_ld32(t_s + cb + q2 * 32u, v);
-                    tmem_wait_ld();
+                    read_o(c, s > kTake, scale, v);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const uint32_t kp = k0 + cb + (uint32_t)(q2 * 32 + i);
-                        if (full || (kp >= s_row && kp < kend)) xm = fmaxf(xm, v[i]);
+                    for (int i = 0; i < 32; i++) sums[(c * 32 + i) * 128] = v[i];
+                }
+                m_taken = m;
+            }
+            const bool edge = __any_sync(0xffffffffu, k0 < s_row || k0 + 128u > kend);
+            // scores 32c .. 32c+31, -inf outside the row's keys
+            auto mask = [&](int c, float (&x)[32]) {
+                if (edge)
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (k0 + 32u * c + i < s_row || k0 + 32u * c + i >= kend) x[i] = -INFINITY;
+            };
+            auto top_of = [&](const float (&x)[32]) {
+                float a = x[0], b = x[1];
+#pragma unroll
+                for (int i = 2; i < 32; i += 2) {
+                    a = fmaxf(a, x[i]);
+                    b = fmaxf(b, x[i + 1]);
+                }
+                return fmaxf(a, b);
+            };
+            // The first half is read twice, the second half stays in registers.
+            float v[2][32], u[2][32];
+            tmem_ld32(t_s, u[0]);
+            tmem_ld32(t_s + 32u, u[1]);
+            tmem_wait_ld();
+            tmem_ld32(t_s + 64u, v[0]);
+            tmem_ld32(t_s + 96u, v[1]);
+            mask(0, u[0]);
+            mask(1, u[1]);
+            float mx = fmaxf(top_of(u[0]), top_of(u[1]));
+            tmem_wait_ld();
+            tmem_ld32(t_s, u[0]);
+            mask(2, v[0]);
+            mask(3, v[1]);
+            const float top = fmaxf(mx, fmaxf(top_of(v[0]), top_of(v[1]))) * qs;
+            const bool raise = top - m > kRaise;
+            if (__any_sync(0xffffffffu, raise)) {
+                const float mn = raise ? top - kHead : m, alpha = fast_exp2(m - mn);
+                if (s > 0) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        float o[32];
+                        tmem_ld32(t_o + c * 32u, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] *= alpha;
+                        tmem_st32(t_o + c * 32u, o);
                     }
                 }
-                xm *= qs;
+                l *= alpha;
+                m = mn;
             }
-            if (pair_any(!got)) { abort_sh = 1; ok = false; break; }
-            const bool need = (m == -INFINITY && xm > -INFINITY) || xm > kRaise;
-            if (pair_any(need || (!F32 && s == 0))) {
-                // raise the rows' references: exchange the maximum with the other half, rescale O, redo P
-                xch[s & 1u][st][hh][r] = xm + mu0;
-                pair_any(false);
-                const float mx = fmaxf(xch[s & 1u][st][0][r], xch[s & 1u][st][1][r]) - kHead;
-                const bool raise = mx > -INFINITY && (m == -INFINITY || mx > m + (kRaise - kHead));
-                if (__any_sync(0xffffffffu, raise || (!F32 && s == 0))) {
-                    const float alpha = !raise ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - mx);
-                    if (s > 0) {
+            // P over S: keys 32c .. 32c+31 in columns 16c .. 16c+15 (remainders 64 columns on)
+            float la = 0.f, lb = 0.f;
+            auto weigh = [&](int c, const float (&x)[32]) {
+                uint32_t w[16], wl[16];
 #pragma unroll
-                        for (int q2 = 0; q2 < 2; q2++) {
-                            float v[32];
-                            tmem_ld32(t_o + cb + q2 * 32u, v);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] *= alpha;
-                            tmem_st32(t_o + cb + q2 * 32u, v);
-                        }
-                        tmem_wait_st();
+                for (int i = 0; i < 16; i++) {
+                    const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
+                    la += p0;
+                    lb += p1;
+                    w[i] = pack_h2(p0, p1);
+                    if (F32) {
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                        wl[i] = pack_h2(p0 - h.x, p1 - h.y);
                     }
-                    if (raise) {
-                        l *= alpha;
-                        m = mx;
-                    }
-                    pass(k0, full, m == -INFINITY ? 0.f : m, w, wl, la, xm);
                 }
-                pair_any(false);  // both halves have re-read S
-            }
-            // (both halves have read S: P overwrites columns of either)
-            l += la;
-            tmem_st16u(t_s + cb / 2u, w[0]);
-            tmem_st16u(t_s + cb / 2u + 16u, w[1]);
-            if (F32) {
-                tmem_st16u(t_s + 64u + cb / 2u, wl[0]);
-                tmem_st16u(t_s + 64u + cb / 2u + 16u, wl[1]);
-            }
+                tmem_st16u(t_s + c * 16u, w);
+                if (F32) tmem_st16u(t_s + 64u + c * 16u, wl);
+            };
+            tmem_wait_ld();
+            mask(0, u[0]);
+            weigh(0, u[0]);
+            tmem_ld32(t_s + 32u, u[1]);
+            tmem_wait_ld();
+            mask(1, u[1]);
+            weigh(1, u[1]);
+            weigh(2, v[0]);
+            weigh(3, v[1]);
+            l += la + lb;
             tmem_wait_st();
             fence_before();
             bar_arrive(bar(B_PFULL + st));
         }
-        const bool got_e = n_steps == 0 || (ok && !abort_sh && wait_bar_warp(bar(B_ODONE + st), 0));
-        if (ok) {
-            xch[0][st][hh][r] = l;
-            if (pair_any(!got_e)) ok = false;
-        }
+        if (ok && n_steps > 0) ok = !abort_sh && wait_bar_warp(bar(B_ODONE + st), 0);
         if (!ok) abort_sh = 1;
-        if (ok) l = xch[0][st][0][r] + xch[0][st][1][r];
-        // Partial tile of (kv head, m tile, split).
-        const uint64_t row = ((uint64_t)Gr.part0 + ((uint64_t)kvh * Gr.m_tiles + mt) * Gr.splits + split) * 128u + r;
-        float wA = 1.f;
+        const bool took = F32 && n_steps > kTake;
+        const float w_taken = fast_exp2(m_taken - m);
         const float *ob = reinterpret_cast<const float *>(gsm + T_K * kTile);  // stream 1's O, [128 columns][128 rows]
-        if (hh == 0) {
-            xch[1][st][0][r] = m;
-            xch[1][st][1][r] = l;
-        }
-        asm volatile("bar.sync 9, 512;" ::: "memory");  // both streams' MMAs are done: the K and V tiles are free
+        float wA = 1.f;
+        ml_sh[st][r] = make_float2(m, l);
+        asm volatile("bar.sync 9, 256;" ::: "memory");  // both streams' MMAs are done: the K and V tiles are free
+        fence_after();
         if (solo) {
-            // Join the streams: stream 1 leaves (m, l) and its O, scaled, in the K tiles.
-            const float m0 = xch[1][0][0][r], m1 = xch[1][1][0][r], l0 = xch[1][0][1][r], l1 = xch[1][1][1][r];
-            const float mj = fmaxf(m0, m1);
-            wA = m0 == -INFINITY ? (l0 == 0.f ? 0.f : 1.f) : fast_exp2(m0 - mj);
-            const float wB = m1 == -INFINITY ? (l1 == 0.f ? 0.f : 1.f) : fast_exp2(m1 - mj);
-            if (st == 1 && n_steps > 0 && !abort_sh) {
-                fence_after();
+            // Join the streams: stream 1 leaves its O, scaled, in the K tiles.
+            const float2 a = ml_sh[0][r], b = ml_sh[1][r];
+            m = fmaxf(a.x, b.x);
+            wA = fast_exp2(a.x - m);
+            const float wB = fast_exp2(b.x - m);
+            l = a.y * wA + b.y * wB;
+            if (st == 1 && nt > 1 && !abort_sh) {
 #pragma unroll
-                for (int q2 = 0; q2 < 2; q2++) {
+                for (int c = 0; c < 4; c++) {
                     float v[32];
-                    tmem_ld32(t_o + cb + q2 * 32u, v);
-                    tmem_wait_ld();
+                    read_o(c, took, w_taken, v);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) const_cast<float *>(ob)[(cb + q2 * 32u + i) * 128u + r] = v[i] * wB;
+                    for (int i = 0; i < 32; i++) const_cast<float *>(ob)[(c * 32u + i) * 128u + r] = v[i] * wB;
                 }
             }
-            asm volatile("bar.sync 9, 512;" ::: "memory");
-            m = mj;
-            l = l0 * wA + l1 * wB;
+            asm volatile("bar.sync 9, 256;" ::: "memory");
         }
         if (!abort_sh && (!solo || st == 0)) {
             // O goes through shared memory (16-byte chunk c of row r at c ^ (r & 31)), so that
             // the global stores are whole rows: stream 0 by the V tiles, stream 1 by the K tiles
             // (solo: stream 1's O is there until it is added).
-            fence_after();
-            uint8_t *stage = gsm + (st == 0 ? T_V : T_K) * kTile + r * 512u;
+            uint8_t *tile_sm = gsm + (st == 0 ? T_V : T_K) * kTile;
 #pragma unroll
-            for (int q2 = 0; q2 < 2; q2++) {
+            for (int c = 0; c < 4; c++) {
                 float v[32];
-                tmem_ld32(t_o + cb + q2 * 32u, v);
-                tmem_wait_ld();
+                read_o(c, took, w_taken, v);
                 if (solo) {
 #pragma unroll
                     for (int i = 0; i < 32; i++) {
                         v[i] *= wA;
-                        if (nt > 1) v[i] += ob[(cb + q2 * 32u + i) * 128u + r];
+                        if (nt > 1) v[i] += ob[(c * 32u + i) * 128u + r];
                     }
                 }
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++)
-                    *reinterpret_cast<float4 *>(stage + (((cb / 4u + q2 * 8u + i) ^ (r & 31u)) << 4)) =
+                    *reinterpret_cast<float4 *>(tile_sm + r * 512u + (((c * 8u + i) ^ lane) << 4)) =
                         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
-            pair_any(false);  // the two warps' halves of 32 rows are in place; each stores 16 of them
+            if (took) asm volatile("bar.sync 10, 128;" ::: "memory");  // (the sums of all columns are read)
+            __syncwarp();  // a warp stores its own 32 rows
             const uint32_t rows = min(T, Gr.n_seqs - mt * T) * G;  // of the tile's, those that hold a head
-            const uint32_t r0 = (warp & 3u) * 32u + hh * 16u;
-            const uint8_t *tile_sm = gsm + (st == 0 ? T_V : T_K) * kTile;
+            const uint32_t r0 = (warp & 3u) * 32u;
             float *tile_out = P.part + (row - r) * 128u;
-#pragma unroll 4
-            for (uint32_t x = r0; x < min(r0 + 16u, rows); x++)
+#pragma unroll 8
+            for (uint32_t x = r0; x < min(r0 + 32u, rows); x++)
                 *reinterpret_cast<float4 *>(tile_out + x * 128u + lane * 4u) =
                     *reinterpret_cast<const float4 *>(tile_sm + x * 512u + ((lane ^ (x & 31u)) << 4));
-            if (valid && hh == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
+            if (valid) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
         }
     }
     fence_before();
@@ -564,11 +554,11 @@ uint32_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t
     return (uint32_t)ctas;
 }
 
-// CTAs stay within units + 2 * kPlanSms, a CTA has at most two tiles, and
-// 2 * (KV heads x tile pairs) within KV heads x (m tiles + groups).
+// CTAs stay within units + 2 * kPlanSms, and a CTA has at most two tiles: two Q
+// tiles (units are KV heads x pairs of m tiles), or, in F32, one and its stream 1's sums.
 uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads) {
     const uint64_t m_tiles = n_seqs / prefix_seqs_per_tile(q_heads / kv_heads) + n_groups;
-    return (uint64_t)kv_heads * (m_tiles + n_groups) + 4u * kPlanSms;
+    return (uint64_t)kv_heads * 2u * m_tiles + 4u * kPlanSms;
 }
 
 template <bool F32, int NS>
@@ -607,13 +597,15 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
     std::copy(seqs, seqs + n_seqs, P.seq);
     P.part = part;
     P.ml = ml;
+    const PrefixGroup &last = groups[n - 1];
+    P.take0 = last.part0 + kv_heads * last.m_tiles * last.splits;
     P.n_groups = n;
     P.heads_per_kv = q_heads / kv_heads;
     P.kv_heads = kv_heads;
     P.tpt = prefix_seqs_per_tile(P.heads_per_kv);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(576);
+    cfg.blockDim = dim3(320);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute at[1];

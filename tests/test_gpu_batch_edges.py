@@ -206,3 +206,47 @@ def test_a_padded_batch_leaves_the_rest_alone():
     assert (out[used:] == 5).all() and torch.isfinite(out[:used]).all()
     assert torch.equal(raw_k[used:], before[0][used:]) and torch.equal(raw_v[used:], before[1][used:])
     assert not torch.equal(raw_k[:used], before[0][:used])
+
+
+@pytest.mark.parametrize("group", [8, 12])
+def test_f32_sums_over_long_splits(group):
+    # 48 sequences over one cache of 20000 rows: a warp takes hundreds of blocks, O is taken out of the tensor core's
+    # truncating sums every 32 of them.  Each MMA drops at most 2^-23 of O: 32 * 2^-23 = 3.8e-6 of the output, and the
+    # scores' and weights' parts (bound() without its rows) of the weighted magnitude.
+    n, cap, heads = 48, 20000, 8
+    raw_k, kx = fill_i8(1, cap, heads, 1)
+    raw_v, vx = fill_i8(1, cap, heads, 2)
+    q = rows(3, n, group * heads)
+    out = torch.full_like(q, float("nan"))
+    d = kv.decode_seqs_desc([raw_k[0]] * n, [raw_v[0]] * n, cap, [cap - 1 - i for i in range(n)], q, out)
+    kv.decode_i8(d, group * heads, heads, D, q.dtype, workspace(kv.decode_i8_workspace(n, group * heads, heads)))
+    for i in range(0, n, 7):
+        want, mag, reach = attend(q[i], kx[0][:cap - i], vx[0][:cap - i], None)
+        assert torch.isfinite(out[i]).all()
+        err = (out[i].double() - want).norm() / want.norm()
+        limit = 3.8e-6 + 2 * (0.6932 * reach.max().item() * 2.0 ** -21 + 2.0 ** -21)
+        assert err <= limit, f"sequence {i}: {err:.3g}"
+
+
+def test_f32_sums_over_a_long_prefix():
+    # few splits of many tiles: the prefix kernel takes O into memory between them
+    n, plen, heads, group = 80, 9000, 8, 12
+    qh = heads * group
+    pk, pv = rows(1, plen, heads).half(), rows(2, plen, heads).half()
+    ko, vo = rows(3, n, 4, heads).half(), rows(4, n, 4, heads).half()
+    q = rows(5, n, qh, scale=1.5)
+    out = torch.full_like(q, float("nan"))
+    d = kv.decode_seqs_desc(ko, vo, 4, [plen + i % 4 for i in range(n)], q, out)
+    ws = workspace(kv.decode_shared_workspace(1, n, qh, heads))
+    for _ in range(2):
+        kv.decode_shared(kv.shared_groups_desc([dict(k_cache=pk, v_cache=pv, prefix_len=plen, seqs=d)]), qh, heads, D, kv.F16,
+                         q.dtype, ws)
+    for i in range(0, n, 9):
+        own = i % 4 + 1
+        at = torch.arange(plen, plen + own, device="cuda") % 4
+        k, v = torch.cat([pk.double(), ko[i][at].double()]), torch.cat([pv.double(), vo[i][at].double()])
+        want, mag, reach = attend(q[i], k, v, None)
+        check(out[i], want, bound(want, mag, reach, plen, q.dtype, False), f"sequence {i}")
+        # 256 MMAs of at most 2^-23 each between two of them, and the scores' 16
+        assert (out[i].double() - want).norm() <= (256 + 16 * 0.6932 * reach.max().item()) * 2.0 ** -23 * want.norm()
+    assert kv.device_error() == 0
