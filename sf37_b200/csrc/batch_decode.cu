@@ -835,8 +835,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Batch
     const uint32_t tid = threadIdx.x, G = P.group;
     const uint32_t lo = blockIdx.x / P.kv_heads, kvh = blockIdx.x - lo * P.kv_heads;
     const SeqDev &J = P.seq[lo];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
+    after_previous();
     if (J.pre_splits == 0) return;
     const uint32_t stride = part_stride(G), n_src = J.n_splits + J.pre_splits;
     const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;
@@ -1024,35 +1023,18 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchPar
     P.counters = head.counters;
     P.pre_part = head.pre_part;
     P.pre_ml = head.pre_ml;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(slots * head.kv_heads);
-    cfg.blockDim = dim3(Sh::kThreads);
-    cfg.dynamicSmemBytes = Sh::kSmem;
-    cfg.stream = stream;
     // After a prefix launch the CTAs start on the SMs that it leaves, and stream their own
     // rows meanwhile; every CTA waits for that launch before it reads its
-    // partials.  Otherwise they start as the kernel before drains, and wait for it.  What follows
-    // may start early too: sf37kv_decode, whose kernels read some caches before they wait, is told.
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    stream_record_drop(stream);
+    // partials.  Otherwise they start as the kernel before drains, and wait for it.
     P.after_prefix = after_prefix;
     P.join = after_prefix && !WIDE;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, batch_decode_kernel<MODE, I8, WIDE, NJ>, P);
-    if (e == cudaSuccess) e = cudaGetLastError();
     g_launches++;
-    if (e == cudaSuccess && P.join) {
-        cfg.gridDim = dim3(n * head.kv_heads);
-        cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = 0;
-        e = cudaLaunchKernelEx(&cfg, join_kernel<NJ>, P);
-        if (e == cudaSuccess) e = cudaGetLastError();
-        g_launches++;
-    }
-    return check_cuda(e, "decode launch");
+    if (int rc = launch_early("decode launch", batch_decode_kernel<MODE, I8, WIDE, NJ>, dim3(slots * head.kv_heads),
+                              Sh::kThreads, Sh::kSmem, stream, P))
+        return rc;
+    if (!P.join) return SF37KV_OK;
+    g_launches++;
+    return launch_early("join launch", join_kernel<NJ>, dim3(n * head.kv_heads), 256, 0, stream, P);
 }
 
 template <int MODE, bool I8>

@@ -33,6 +33,34 @@ static inline int check_cache(const char *what, uint32_t i, const sf37kv_cache &
     return SF37KV_OK;
 }
 
+// Launches a kernel that starts while the one before it on the stream drains
+// (programmatic dependent launch) and so calls after_previous() before it touches
+// memory.  sf37kv_decode, whose kernels read some caches before they wait, is
+// told that its successor's start is no longer ordered behind this one's end.
+template <typename Kernel, typename Params>
+static int launch_early(const char *what, Kernel kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+                        const Params &params) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    stream_record_drop(stream);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, params);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return check_cuda(e, what);
+}
+// Waits for the kernel before, then lets the next one start.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+}
+
 __device__ __forceinline__ uint32_t h2_bits(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);

@@ -51,6 +51,7 @@ __device__ __forceinline__ uint32_t job_of(const Begin &begin, uint32_t n, uint3
 // 8 heads, bf16: @APPEND@.
 template <bool BF16>
 __global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
+    after_previous();
     const uint32_t lane8 = threadIdx.x & 7u, unit = blockIdx.x * 32u + (threadIdx.x >> 3);
     const uint32_t row = unit / P.heads, head = unit - row * P.heads;
     const bool live = row < P.row_begin[P.n_jobs];
@@ -133,6 +134,7 @@ constexpr uint32_t kReadRows = 16;
 template <bool F16>
 __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ ReadI8Params P) {
     constexpr uint32_t E = F16 ? 8u : 4u, kAtOnce = 4;  // elements a thread and step, steps at once
+    after_previous();
     const uint32_t j = job_of(P.blk_begin, P.n_jobs, P.blks_each, blockIdx.x);
     const ReadI8Job &J = P.job[j];
     const uint32_t r0 = (blockIdx.x - P.blk_begin[j]) * kReadRows;
@@ -249,10 +251,10 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
             }
             P.row_begin[P.n_jobs] = (uint32_t)rows;
             const unsigned grid = (unsigned)((rows * kv_heads + 31u) / 32u);
-            if (bf16) append_i8_kernel<true><<<grid, 256, 0, s>>>(P);
-            else append_i8_kernel<false><<<grid, 256, 0, s>>>(P);
             g_launches++;
-            if (int rc = check_cuda(cudaGetLastError(), "append_i8 launch")) return rc;
+            if (int rc = launch_early("append_i8 launch", bf16 ? append_i8_kernel<true> : append_i8_kernel<false>, grid, 256, 0,
+                                      s, P))
+                return rc;
         }
     }
     return SF37KV_OK;
@@ -299,11 +301,10 @@ extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_lay
         base = i;
         if (P.n_jobs == 0) continue;
         P.blk_begin[P.n_jobs] = (uint32_t)blks;
-        const dim3 grid((unsigned)blks, 2);
-        if (dst_dtype == SF37KV_F16) read_i8_kernel<true><<<grid, 256, 0, s>>>(P);
-        else read_i8_kernel<false><<<grid, 256, 0, s>>>(P);
         g_launches++;
-        if (int rc = check_cuda(cudaGetLastError(), "read_i8 launch")) return rc;
+        if (int rc = launch_early("read_i8 launch", dst_dtype == SF37KV_F16 ? read_i8_kernel<true> : read_i8_kernel<false>,
+                                  dim3((unsigned)blks, 2), 256, 0, s, P))
+            return rc;
     }
     return SF37KV_OK;
 }

@@ -172,11 +172,8 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // The kernel before (which may still drain: programmatic dependent launch) is
-    // waited for; then the next one, which reads this kernel's partials after a
-    // wait of its own, may start as SMs become free.
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
+    // (the next kernel reads this one's partials after a wait of its own)
+    after_previous();
 
     // The sequences' table is read by generic loads: lane-divergent constant loads replay.
     const PrefixSeq *tab = P.seq;
@@ -603,20 +600,8 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
     P.heads_per_kv = q_heads / kv_heads;
     P.kv_heads = kv_heads;
     P.tpt = prefix_seqs_per_tile(P.heads_per_kv);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(320);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_tc05_kernel<F32, NS>, P);
-    if (e == cudaSuccess) e = cudaGetLastError();
     g_launches++;
-    return check_cuda(e, "prefix launch");
+    return launch_early("prefix launch", prefix_tc05_kernel<F32, NS>, dim3(ctas), 320, smem, stream, P);
 }
 
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
