@@ -11,15 +11,20 @@
 // keys need no conversion; value codes become f16, exactly.
 //
 // One CTA serves one KV head of one sequence over a run of rows (a split), so
-// each K/V byte is read once for all G query heads.  Four warps stream
+// each K/V byte is read once for all G query heads.  Its warps stream
 // interleaved 16-row blocks through private rings of cp.async stages; S = qK^T
-// and O += PV are mma.sync m16n8k16 tiles on fragments that the lanes load
-// straight from the stage.  The bytes bound it, not the products: 16 rows of I8
-// are 4224 bytes and about 270 warp instructions, and an SM receives those
-// bytes in 180 cycles, in which it could issue 720.  The CTAs of a (sequence,
-// KV head) leave unnormalised partials; the last one to finish (an atomic
-// counter) joins them, and the shared prefix's, in a fixed order, so results do
-// not depend on which CTA is last.
+// and O += PV are mma.sync tiles on fragments that the lanes load
+// straight from the stage.  The bytes bound it, not the products (tcgen05 would need
+// 128 rows of queries): 16 rows of I8 are 4224 bytes and about 330 warp instructions, and an
+// SM receives those bytes in 180 cycles, in which it can issue 720.  The CTAs of a
+// (sequence, KV head) leave unnormalised partials; the last one to finish (an
+// atomic counter) or join_kernel joins them, and the shared prefix's, in a fixed
+// order, so results do not depend on which CTA is last.
+//
+// Measured (one B200, graph replay; of the measured copy rate): 48 layers x 32769 rows of I8, 8
+// KV heads, f32: 540-600 us (0.85-0.94); 64 sequences of 1 to 8192 rows, bf16: 89 us (0.96);
+// one of 131072: 46 us (0.92); 128 windows of 512 rows, 96 query heads: 40 us (0.53: a CTA's
+// start and end are as long as its 512 rows); one of 2049: 9.3 us.
 //
 // Sixteen M rows of a tile hold, by MODE:
 //   kPair  G <= 8, f32: eight heads twice, f16 "hi" and remainder "lo" of the weights
@@ -48,7 +53,6 @@ constexpr uint32_t kTake = 32;
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
 constexpr uint32_t kMapped = 1024;     // slots with a direct map to their sequence
-constexpr uint32_t kMergePass = 32;    // partials joined per pass
 // Range of the weights' power of two (kernel below): the ratio of two is finite.
 constexpr int kFMin = -86, kFMax = 40;
 
@@ -119,9 +123,6 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) { return unbias(prmt(w,
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint64_t pol) {
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol) : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -168,6 +169,51 @@ __device__ __forceinline__ float4 normalise(float4 a, float l, float g) {
     return make_float4(a.x / l * g, a.y / l * g, a.z / l * g, a.w / l * g);
 }
 
+// One float4 (index idx of [G][128], head h) of the partials of a (sequence, KV
+// head): n_own of its own, `step` floats apart, then n_pre of the prefix's, a 128-row tile
+// apart, always in this order.  Eight partials' values and (m, l) pairs are loaded at once:
+// a trip to L2 for each eight, and no barrier.
+struct Joined {
+    float4 o;
+    float l;
+};
+__device__ __forceinline__ Joined join_one(const float *own, uint64_t step, uint32_t n_own, const float *pre,
+                                           const float *pre_ml, uint64_t row, uint32_t n_pre, uint32_t G, uint32_t h,
+                                           uint32_t idx) {
+    Joined r;
+    r.o = make_float4(0.f, 0.f, 0.f, 0.f);
+    r.l = 0.f;
+    float M = kNone;
+    const uint32_t n = n_own + n_pre;
+    for (uint32_t s = 0; s < n; s += 8u) {
+        float4 x[8];
+        float2 ml[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t k = s + i;
+            ml[i] = make_float2(-INFINITY, 0.f);
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n) {
+                const bool mine = k < n_own;
+                const float *po = mine ? own + k * step : pre + (row + (uint64_t)(k - n_own) * 128u) * 128u;
+                const float *pm = mine ? po + G * 128u : pre_ml + (row + (uint64_t)(k - n_own) * 128u) * 2u;
+                x[i] = __ldcg(reinterpret_cast<const float4 *>(po) + idx);
+                ml[i] = __ldcg(reinterpret_cast<const float2 *>(pm) + h);
+            }
+        }
+        float mn = M;
+#pragma unroll
+        for (int i = 0; i < 8; i++) mn = fmaxf(mn, ml[i].x);
+        const float sc = fast_exp2(M - mn);
+        M = mn;
+        r.l *= sc;
+        r.o = make_float4(r.o.x * sc, r.o.y * sc, r.o.z * sc, r.o.w * sc);
+#pragma unroll
+        for (int i = 0; i < 8; i++) fold(r.o, r.l, x[i], ml[i].y, fast_exp2(ml[i].x - mn));
+    }
+    return r;
+}
+
 }  // namespace bd
 
 // ------------------------------------------------------------ the stage
@@ -201,8 +247,9 @@ struct Stage {
 };
 
 // Warps of a CTA, CTAs of an SM and stages of a warp.  An SM runs 12 warps (8 in
-// kTwo, for their registers, and with f32 outputs over f16 caches, for the sums' memory), either as CTAs of four, which hide each other's
-// starts and ends, or as one wide CTA, which leaves fewer partials to join.
+// kTwo, for their registers, and with f32 outputs over f16 caches, for the sums'
+// memory), either as CTAs of four, which hide each other's starts and ends, or
+// as one wide CTA, which leaves fewer partials to join.
 // More stages only lengthen the queue to HBM, and with it every other access:
 // 8 layers x 32769 rows of I8 took 95 us with three stages, 100 with four, 102
 // with two; f16 rows 76 us with two stages of 12 warps, 80 with three of 8.
@@ -760,149 +807,46 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     if (tid == 0) *ctr = 0u;  // ready for the next call
 
     // ---- the last CTA joins all partials of (sequence, KV head) ----
-    const uint32_t n_src = J.n_splits + J.pre_splits;
+    const uint64_t row_pre = ((uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh) * 128u + J.pre_row;
     const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;
-    const uint64_t tile0 = (uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh;
-    // the partials land in the stages, their (m, l) pairs where q was
-    const uint32_t land = (uint32_t)__cvta_generic_to_shared(smem), ml_land = (uint32_t)__cvta_generic_to_shared(Qs);
-    const float *ml_s = reinterpret_cast<const float *>(Qs);
-    static_assert(kMergePass * 32 * 4 <= 8 * 32 * 16, "(m, l) pairs of a pass");
-    const uint32_t per = min(kMergePass, Sh::kArea / (G * 512u));
-    constexpr int kPer = (16 * 32 + kThreads - 1) / kThreads;  // float4 outputs of a thread, G <= 16
-    float4 acc[kPer];
-    float M[kPer], L[kPer];
-#pragma unroll
-    for (int k = 0; k < kPer; k++) {
-        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        M[k] = kNone;
-        L[k] = 0.f;
-    }
-    for (uint32_t s0 = 0; s0 < n_src; s0 += per) {
-        const uint32_t cnt = min(per, n_src - s0);
-        for (uint32_t s = 0; s < cnt; s++) {
-            const uint32_t x = s0 + s;
-            const float *po, *pm;
-            if (x < J.n_splits) {
-                po = own + (uint64_t)x * P.kv_heads * stride;
-                pm = po + G * 128u;
-            } else {
-                const uint64_t row = (tile0 + (x - J.n_splits)) * 128u + J.pre_row;
-                po = P.pre_part + row * 128u;
-                pm = P.pre_ml + row * 2u;
-            }
-            for (uint32_t idx = tid; idx < G * 32u; idx += kThreads) cp16(land + s * G * 512u + idx * 16u, po + idx * 4u);
-            if (tid < 2u * G) cp4(ml_land + (s * 32u + tid) * 4u, pm + tid);
-        }
-        cp_commit();
-        cp_wait<0>();
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kPer; k++) {
-            const uint32_t idx = tid + (uint32_t)k * kThreads;
-            if (idx < G * 32u) {
-                const float2 *ml = reinterpret_cast<const float2 *>(ml_s) + (idx >> 5);
-                float mn = M[k];
-#pragma unroll 4
-                for (uint32_t s = 0; s < cnt; s++) mn = fmaxf(mn, ml[s * 16u].x);
-                const float sc = fast_exp2(M[k] - mn);
-                M[k] = mn;
-                L[k] *= sc;
-                acc[k] = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
-#pragma unroll 4
-                for (uint32_t s = 0; s < cnt; s++) {
-                    const float2 x = ml[s * 16u];
-                    fold(acc[k], L[k], *reinterpret_cast<const float4 *>(smem + (s * G * 32u + idx) * 16u), x.y,
-                         fast_exp2(x.x - mn));
-                }
-            }
-        }
-        __syncthreads();
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; k++) {
-        const uint32_t idx = tid + (uint32_t)k * kThreads;
-        if (idx < G * 32u) store_out4(J.out, out0 + idx * 4u, normalise(acc[k], L[k], gate_s[idx >> 5]), P.bf16);
+    for (uint32_t idx = tid; idx < G * 32u; idx += kThreads) {
+        const uint32_t h = idx >> 5;
+        const Joined x = join_one(own, (uint64_t)P.kv_heads * stride, J.n_splits, P.pre_part, P.pre_ml, row_pre, J.pre_splits, G,
+                                  h, idx);
+        store_out4(J.out, out0 + idx * 4u, normalise(x.o, x.l, gate_s[h]), P.bf16);
     }
 }
 
 // ------------------------------------------------------------ join
 // One CTA per (sequence, KV head) with a shared prefix: its own partials and the
-// prefix's, in that order.  Bound by L2: (splits of both) * G * 520 bytes a CTA.
+// prefix's, in that order.  Bound by trips to L2: one for every eight partials.
 template <int NJ>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ BatchParams<NJ> P) {
     using namespace bd;
-    __shared__ float2 ml_s[32][16];
     const uint32_t tid = threadIdx.x, G = P.group;
     const uint32_t lo = blockIdx.x / P.kv_heads, kvh = blockIdx.x - lo * P.kv_heads;
     const SeqDev &J = P.seq[lo];
     after_previous();
     if (J.pre_splits == 0) return;
-    const uint32_t stride = part_stride(G), n_src = J.n_splits + J.pre_splits;
+    const uint32_t stride = part_stride(G);
     const float *own = P.part + ((uint64_t)J.slot * P.kv_heads + kvh) * stride;
-    const uint64_t row0 = ((uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh) * 128u + J.pre_row;
-    auto source = [&](uint32_t x) {
-        return x < J.n_splits ? own + (uint64_t)x * P.kv_heads * stride
-                              : P.pre_part + (row0 + (uint64_t)(x - J.n_splits) * 128u) * 128u;
-    };
-    float4 acc[2];
-    float M[2], L[2];
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        M[k] = kNone;
-        L[k] = 0.f;
-    }
-    for (uint32_t s0 = 0; s0 < n_src; s0 += 32u) {
-        const uint32_t cnt = min(32u, n_src - s0);
-        __syncthreads();
-        for (uint32_t i = tid; i < cnt * 16u; i += 256u) {
-            const uint32_t x = s0 + (i >> 4), h = i & 15u;
-            if (h < G)
-                ml_s[i >> 4][h] = __ldcg(x < J.n_splits
-                                             ? reinterpret_cast<const float2 *>(source(x) + G * 128u) + h
-                                             : reinterpret_cast<const float2 *>(P.pre_ml) + row0 +
-                                                   (uint64_t)(x - J.n_splits) * 128u + h);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const uint32_t idx = tid + (uint32_t)k * 256u, h = idx >> 5;
-            if (idx < G * 32u) {
-                float mn = M[k];
-                for (uint32_t s = 0; s < cnt; s++) mn = fmaxf(mn, ml_s[s][h].x);
-                const float sc = fast_exp2(M[k] - mn);
-                M[k] = mn;
-                L[k] *= sc;
-                acc[k] = make_float4(acc[k].x * sc, acc[k].y * sc, acc[k].z * sc, acc[k].w * sc);
-                for (uint32_t s = 0; s < cnt; s += 8u) {
-                    float4 x[8];
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; i++)
-                        if (s + i < cnt) x[i] = __ldcg(reinterpret_cast<const float4 *>(source(s0 + s + i)) + idx);
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; i++)
-                        if (s + i < cnt) {
-                            const float2 ml = ml_s[s + i][h];
-                            fold(acc[k], L[k], x[i], ml.y, fast_exp2(ml.x - mn));
-                        }
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const uint32_t idx = tid + (uint32_t)k * 256u, h = idx >> 5;
-        if (idx < G * 32u)
-            store_out4(J.out, (uint64_t)kvh * G * 128u + idx * 4u,
-                       normalise(acc[k], L[k], J.gate ? sigmoid_dev(J.gate[kvh * G + h]) : 1.f), P.bf16);
+    const uint64_t row_pre = ((uint64_t)J.pre_tile + (uint64_t)kvh * J.pre_kvh) * 128u + J.pre_row;
+    for (uint32_t idx = tid; idx < G * 32u; idx += 256u) {
+        const uint32_t h = idx >> 5;
+        const float gate = J.gate ? J.gate[kvh * G + h] : 0.f;
+        const Joined x = join_one(own, (uint64_t)P.kv_heads * stride, J.n_splits, P.pre_part, P.pre_ml, row_pre, J.pre_splits, G,
+                                  h, idx);
+        store_out4(J.out, (uint64_t)kvh * G * 128u + idx * 4u, normalise(x.o, x.l, J.gate ? sigmoid_dev(gate) : 1.f), P.bf16);
     }
 }
 
 // ------------------------------------------------------------ planning
 // Rows of a split.  Few pairs (sequence, KV head): one wave of wide CTAs, with
-// as many splits as fill it.  More pairs: the split whose CTAs, in whole waves of
-// `resident`, cost least, a CTA's start and end counting as kFixedRows rows; a
-// pair's splits are even, and a short pair is one.
+// as many splits as fill it (131072 rows, 8 KV heads: 56 us, 119 in CTAs of four).
+// More pairs: the split whose CTAs, in whole waves of `resident`, cost least, a CTA's
+// start and end counting as kFixedRows rows; a pair's splits are even, and a
+// short pair is one (8 layers x 32769 rows: 101 us with 13 splits, 1.9 waves, 113 with 17, 2.5
+// waves, 123 with 7, 1.01).
 constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256, kWaves = 4;
 
 struct Plan {

@@ -47,8 +47,9 @@ __device__ __forceinline__ uint32_t job_of(const Begin &begin, uint32_t n, uint3
 }
 
 // Eight lanes per head of one row, K and V together: 16 elements a lane in
-// 128-byte runs, all loads first; a head's maximum is three shuffles.  8192 rows of
-// 8 heads, bf16: @APPEND@.
+// 128-byte runs, all loads first; a head's maximum is three shuffles, and a code
+// six instructions.  8192 rows of 8 heads, bf16: 16 us, 3.2 TB/s (a warp a head with
+// integer conversions took 30 us).  Latency bounds it: 50 MB are 8 us of HBM.
 template <bool BF16>
 __global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
     after_previous();
@@ -128,7 +129,7 @@ struct ReadI8Params {
 // writes 16 bytes at a time, so stores are coalesced and loads are 4 (f32) or
 // 8 (f16) contiguous codes; 32 or 16 neighbouring threads share a scale.  A
 // code becomes f32 as the low bits of 2^23 + c + 128, less 2^23 + 128.  32768 rows of 8
-// heads to f16: @READ@.
+// heads to f16: 36 us, 5.6 TB/s (0.86 of the measured copy rate).
 constexpr uint32_t kReadRows = 16;
 
 template <bool F16>

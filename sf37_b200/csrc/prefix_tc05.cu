@@ -23,6 +23,13 @@
 // Weights are 2^(x - m) with the reference m 7 below a running row maximum,
 // raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
 // the largest.  S and O accumulate in f32 (TMEM), m and l in f32 registers.
+//
+// Bound by the tensor pipe and the softmax's latency: a step (S and PV of one stream and key
+// tile) is 1024 cycles of MMA, issues in 1400-1550 (8 MMAs and their commits take 600 on an
+// idle SM) and takes 2200, since two streams do not hide each other's softmax wholly.
+// 64 sequences x 64 heads over 32768 rows, bf16: 85 us on 144 SMs, 0.81 PFLOP/s (0.48 of
+// the measured bf16 rate); of that 15 us are a CTA's start and end (8 KB of q and the
+// first tiles, a 128 KB partial out).
 #include <algorithm>
 #include <type_traits>
 
