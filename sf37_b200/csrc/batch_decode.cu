@@ -36,6 +36,7 @@
 //   kTwo   G <= 16 and f32: two kPair tiles on the same K/V fragments.
 #include <algorithm>
 #include <climits>
+#include <cstring>
 
 #include "batch_internal.cuh"
 
@@ -852,6 +853,7 @@ constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256, kWaves = 4;
 struct Plan {
     bool wide;
     uint32_t slots;
+    uint8_t order[kMaxSeqs];  // of the sequences' slots
 };
 static uint64_t plan_ctas(const SeqDev *seqs, uint32_t n, uint64_t rows) {
     const uint32_t r = (uint32_t)std::min<uint64_t>(rows, kMaxPos);
@@ -909,11 +911,15 @@ static Plan plan_splits(SeqDev *seqs, uint32_t n, uint32_t kv_heads, uint32_t wi
         J.split_rows = (uint32_t)std::max<uint64_t>(u, ((len + J.n_splits - 1) / J.n_splits + u - 1) / u * u);
     }
     // The longest first: the short ones even out the end.
-    if (!plan.wide) std::sort(seqs, seqs + n, [](const SeqDev &a, const SeqDev &b) { return a.split_rows > b.split_rows; });
+    uint64_t key[kMaxSeqs];
+    for (uint32_t i = 0; i < n; i++) key[i] = (uint64_t)(plan.wide ? 0u : ~seqs[i].split_rows) << 32 | i;
+    if (!std::is_sorted(key, key + n)) std::sort(key, key + n);
     plan.slots = 0;
     for (uint32_t i = 0; i < n; i++) {
-        seqs[i].slot = plan.slots;
-        plan.slots += seqs[i].n_splits;
+        plan.order[i] = (uint8_t)key[i];
+        SeqDev &J = seqs[plan.order[i]];
+        J.slot = plan.slots;
+        plan.slots += J.n_splits;
     }
     return plan;
 }
@@ -941,7 +947,7 @@ static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint3
 
 // ------------------------------------------------------------ launches
 template <int MODE, bool I8, bool WIDE, int NJ>
-static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchParams<1> &head, bool after_prefix,
+static int launch(const SeqDev *seqs, uint32_t n, const Plan &plan, const BatchParams<1> &head, bool after_prefix,
                   cudaStream_t stream) {
     using Sh = Shape<MODE, I8, WIDE>;
     static bool ready[64];
@@ -955,10 +961,11 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchPar
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
     BatchParams<NJ> P;
-    std::copy(seqs, seqs + n, P.seq);
-    for (uint32_t i = 0; i < n && slots <= kMapped; i++)
-        std::fill(P.seq_of + seqs[i].slot, P.seq_of + seqs[i].slot + seqs[i].n_splits, (uint8_t)i);
-    P.slots = slots;
+    for (uint32_t i = 0; i < n; i++) {
+        const SeqDev &J = P.seq[i] = seqs[plan.order[i]];
+        if (plan.slots <= kMapped) std::memset(P.seq_of + J.slot, (int)i, J.n_splits);
+    }
+    P.slots = plan.slots;
     P.n = n;
     P.group = head.group;
     P.kv_heads = head.kv_heads;
@@ -973,7 +980,7 @@ static int launch(const SeqDev *seqs, uint32_t n, uint32_t slots, const BatchPar
     P.after_prefix = after_prefix;
     P.join = after_prefix && !WIDE;
     g_launches++;
-    if (int rc = launch_early("decode launch", batch_decode_kernel<MODE, I8, WIDE, NJ>, dim3(slots * head.kv_heads),
+    if (int rc = launch_early("decode launch", batch_decode_kernel<MODE, I8, WIDE, NJ>, dim3(plan.slots * head.kv_heads),
                               Sh::kThreads, Sh::kSmem, stream, P))
         return rc;
     if (!P.join) return SF37KV_OK;
@@ -990,10 +997,10 @@ static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32
     const bool after_prefix = prefix_ctas > 0;
     // The descriptors travel as kernel parameters; a small launch carries few.
     const bool few = n <= kSmallSeqs;
-    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
-    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
-    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
-    return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan.slots, head, after_prefix, stream);
+    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
+    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan, head, after_prefix, stream);
+    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
+    return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan, head, after_prefix, stream);
 }
 
 template <bool I8>
@@ -1044,6 +1051,10 @@ static bool append_conflict(const sf37kv_decode_seq *const *seqs, uint32_t n) {
         items[2 * i + 1] = Item{seqs[i]->cache.v_cache, w};
     }
     if (!any) return false;
+    // Caches in one allocation, as a rule: in order, K apart from V.
+    bool ordered = true;
+    for (uint32_t i = 2; i < 2 * n && ordered; i++) ordered = items[i - 2].p < items[i].p;
+    if (ordered && (items[2 * n - 2].p < items[1].p || items[2 * n - 1].p < items[0].p)) return false;
     std::sort(items, items + 2 * n, [](const Item &a, const Item &b) { return a.p != b.p ? a.p < b.p : a.writes > b.writes; });
     for (uint32_t i = 1; i < 2 * n; i++)
         if (items[i].p == items[i - 1].p && items[i - 1].writes) return true;

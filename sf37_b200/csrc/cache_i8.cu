@@ -182,8 +182,12 @@ __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ Re
     }
 }
 
-// Whether two of n pointers are equal (n <= kMaxJobs).
+// Whether two of the caches (K and V in turn, n in all) are one.
 static bool any_twice(const void **p, uint32_t n) {
+    // In one allocation, as a rule: in order, K apart from V.
+    bool ordered = true;
+    for (uint32_t i = 2; i < n && ordered; i++) ordered = p[i - 2] < p[i];
+    if (ordered && (p[n - 2] < p[1] || p[n - 1] < p[0])) return false;
     std::sort(p, p + n);
     return std::adjacent_find(p, p + n) != p + n;
 }
