@@ -13,18 +13,19 @@
 // One CTA serves one KV head of one sequence over a run of rows (a split), so
 // each K/V byte is read once for all G query heads.  Its warps stream
 // interleaved 16-row blocks through private rings of cp.async stages; S = qK^T
-// and O += PV are mma.sync tiles on fragments that the lanes load
-// straight from the stage.  The bytes bound it, not the products (tcgen05 would need
-// 128 rows of queries): 16 rows of I8 are 4224 bytes and about 330 warp instructions, and an
-// SM receives those bytes in 180 cycles, in which it can issue 720.  The CTAs of a
-// (sequence, KV head) leave unnormalised partials; the last one to finish (an
-// atomic counter) or join_kernel joins them, and the shared prefix's, in a fixed
-// order, so results do not depend on which CTA is last.
+// and O += PV are mma.sync tiles on fragments that the lanes load straight from
+// the stage.  The bytes bound it, not the products (tcgen05 would need 64 rows of
+// queries or more): 16 rows of I8 are 4224 bytes and about 330 warp instructions,
+// and an SM receives those bytes in 180 cycles, in which it can issue 720.  The
+// CTAs of a (sequence, KV head) leave unnormalised partials; the last one to
+// finish (an atomic counter) or join_kernel joins them, and the shared prefix's,
+// in a fixed order, so results do not depend on which CTA is last.
 //
-// Measured (one B200, graph replay; of the measured copy rate): 48 layers x 32769 rows of I8, 8
-// KV heads, f32: 540-600 us (0.85-0.94); 64 sequences of 1 to 8192 rows, bf16: 89 us (0.96);
-// one of 131072: 46 us (0.92); 128 windows of 512 rows, 96 query heads: 40 us (0.53: a CTA's
-// start and end are as long as its 512 rows); one of 2049: 9.3 us.
+// Measured (one B200, graph replay; of the measured copy rate): 48 layers x 32769
+// rows of I8, 8 KV heads, f32: 540-600 us (0.85-0.94); 64 sequences of 1 to 8192
+// rows, bf16: 89 us (0.96); one of 131072: 46 us (0.92); 128 windows of 512 rows,
+// 96 query heads: 40 us (0.53: a CTA's start and end are as long as its 512
+// rows); one of 2049: 9.3 us.
 //
 // Sixteen M rows of a tile hold, by MODE:
 //   kPair  G <= 8, f32: eight heads twice, f16 "hi" and remainder "lo" of the weights
@@ -48,8 +49,9 @@ enum { kPair = 0, kHalf = 1, kWide = 2, kTwo = 3 };
 
 constexpr float kSlack = 8.0f;
 constexpr float kNone = -1e30f;  // reference of a state without rows
-// The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each block (measured),
-// 9e-6 over 512 of them.  f32 outputs take O into sums of their own after this many.
+// The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each block
+// (measured), 9e-6 over 512 of them.  f32 outputs take O into sums of their own
+// after this many.
 constexpr uint32_t kTake = 32;
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
@@ -843,11 +845,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Batch
 
 // ------------------------------------------------------------ planning
 // Rows of a split.  Few pairs (sequence, KV head): one wave of wide CTAs, with
-// as many splits as fill it (131072 rows, 8 KV heads: 56 us, 119 in CTAs of four).
-// More pairs: the split whose CTAs, in whole waves of `resident`, cost least, a CTA's
-// start and end counting as kFixedRows rows; a pair's splits are even, and a
-// short pair is one (8 layers x 32769 rows: 101 us with 13 splits, 1.9 waves, 113 with 17, 2.5
-// waves, 123 with 7, 1.01).
+// as many splits as fill it (131072 rows, 8 KV heads: 56 us when this was chosen,
+// 119 in CTAs of four warps).  More pairs: the split whose CTAs, in whole waves of
+// `resident`, cost least, a CTA's start and end counting as kFixedRows rows; a
+// pair's splits are even, and a short pair is one (8 layers x 32769 rows: 101 us
+// with 13 splits, 1.9 waves, 113 with 17, 2.5 waves, 123 with 7, 1.01).
 constexpr uint32_t kMaxCtas = 4096, kFixedRows = 256, kWaves = 4;
 
 struct Plan {

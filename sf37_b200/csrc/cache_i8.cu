@@ -48,8 +48,8 @@ __device__ __forceinline__ uint32_t job_of(const Begin &begin, uint32_t n, uint3
 
 // Eight lanes per head of one row, K and V together: 16 elements a lane in
 // 128-byte runs, all loads first; a head's maximum is three shuffles, and a code
-// six instructions.  8192 rows of 8 heads, bf16: 16 us, 3.2 TB/s (a warp a head with
-// integer conversions took 30 us).  Latency bounds it: 50 MB are 8 us of HBM.
+// six instructions.  8192 rows of 8 heads, bf16: 16 us, 3.2 TB/s (a warp a head
+// with integer conversions took 30 us).  Latency bounds it: 50 MB are 8 us of HBM.
 template <bool BF16>
 __global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
     after_previous();

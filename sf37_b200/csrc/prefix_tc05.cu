@@ -14,22 +14,23 @@
 // Q tile and are joined through shared memory at the end.
 //
 // Warps 0-3 and 4-7 are the softmax of stream 0 and 1, one row a thread (two
-// threads a row, as in prefill_tc05.cu, were as fast in bf16, but left F32 no registers); warp 8
-// issues the MMAs, warp 9 the TMA loads.  TMEM: S_0, S_1, O_0, O_1 (128 columns each); P
-// (f16) overwrites its S.  F32 (f32 queries and outputs): q and P are two
-// f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits: twice the MMAs; P_lo
-// takes the second half of S's columns.
+// threads a row, as in prefill_tc05.cu, were as fast in bf16, but left F32 no
+// registers); warp 8 issues the MMAs, warp 9 the TMA loads.  TMEM: S_0, S_1, O_0,
+// O_1 (128 columns each); P (f16) overwrites its S.  F32 (f32 queries and
+// outputs): q and P are two f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits:
+// twice the MMAs; P_lo takes the second half of S's columns.
 //
 // Weights are 2^(x - m) with the reference m 7 below a running row maximum,
 // raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
 // the largest.  S and O accumulate in f32 (TMEM), m and l in f32 registers.
 //
-// Bound by the tensor pipe and the softmax's latency: a step (S and PV of one stream and key
-// tile) is 1024 cycles of MMA, issues in 1400-1550 (8 MMAs and their commits take 600 on an
-// idle SM) and takes 2200, since two streams do not hide each other's softmax wholly.
-// 64 sequences x 64 heads over 32768 rows, bf16: 85 us on 144 SMs, 0.81 PFLOP/s (0.48 of
-// the measured bf16 rate); of that 15 us are a CTA's start and end (8 KB of q and the
-// first tiles, a 128 KB partial out).
+// Bound by the tensor pipe and the softmax's latency: a step (S and PV of one
+// stream and key tile) is 1024 cycles of MMA, issues in 1400-1550 (8 MMAs and
+// their commits take 600 on an idle SM) and takes 2200, since two streams do not
+// hide each other's softmax wholly.  64 sequences x 64 heads over 32768 rows,
+// bf16: 85 us on 144 SMs, 0.81 PFLOP/s (0.48 of the measured burst bf16 rate); of
+// that 15 us are a CTA's start and end (64 KB of q and the first tiles, a 128 KB
+// partial out).
 #include <algorithm>
 #include <type_traits>
 
@@ -58,8 +59,8 @@ struct PrefixParams {
 constexpr float kHead = 7.0f, kRaise = 15.0f;
 constexpr float kNone = -1e30f;  // reference of a row without keys
 // The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each MMA (measured).
-// F32 takes O into sums in memory after this many key tiles of a stream (256 MMAs, 4e-6; 16000
-// keys, 40 sequences: 99 us with half as many, 85 with none).
+// F32 takes O into sums in memory after this many key tiles of a stream (256 MMAs,
+// 4e-6; 16000 keys, 40 sequences: 99 us with half as many, 85 with none).
 constexpr uint32_t kTake = 16;
 
 // Q tiles: scaled by a power of two for each row so that its largest element is
@@ -68,10 +69,10 @@ constexpr uint32_t kTake = 16;
 // thread, 32 lines a load, this took 8 us.  `rows` is 128 or 256 (two tiles).
 template <bool F32>
 __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, uint32_t mt0, uint32_t rows, uint32_t kvh,
-                                    uint32_t G, uint32_t T, uint8_t *tiles, float *qscale) {
+                                       uint32_t G, uint32_t T, uint8_t *tiles, float *qscale) {
     using namespace tc05;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-            constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
+    constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
     const uint32_t c = lane % kLanes;
     for (uint32_t x0 = warp * (rows / 8u); x0 < (warp + 1u) * (rows / 8u); x0 += 8u * kAtOnce) {
         uint4 raw[8];
