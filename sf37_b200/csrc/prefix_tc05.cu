@@ -13,12 +13,14 @@
 // K/V tile; with one (solo) the streams take alternate K/V tiles of the same
 // Q tile and are joined through shared memory at the end.
 //
-// Warps 0-3 and 4-7 are the softmax of stream 0 and 1, one row a thread (two
-// threads a row, as in prefill_tc05.cu, were as fast in bf16, but left F32 no
-// registers); warp 8 issues the MMAs, warp 9 the TMA loads.  TMEM: S_0, S_1, O_0,
-// O_1 (128 columns each); P (f16) overwrites its S.  F32 (f32 queries and
-// outputs): q and P are two f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits:
-// twice the MMAs; P_lo takes the second half of S's columns.
+// The first 16 warps are the softmax, eight for each stream and two threads for
+// each row; they weigh a tile in one pass, with the reference of the tiles
+// before it (one thread a row and two passes over S took 108 us where this takes
+// 101, below).  F32 has 8 and one thread a row: two leave it no registers.  Then
+// one warp issues the MMAs and one the TMA loads.  TMEM: S_0, S_1, O_0, O_1 (128
+// columns each); P (f16) overwrites its S.  F32 (f32 queries and outputs): q and P
+// are two f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits: twice the MMAs;
+// P_lo takes the second half of S's columns.
 //
 // Weights are 2^(x - m) with the reference m 7 below a running row maximum,
 // raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
@@ -63,6 +65,10 @@ constexpr float kNone = -1e30f;  // reference of a row without keys
 // 4e-6; 16000 keys, 40 sequences: 99 us with half as many, 85 with none).
 constexpr uint32_t kTake = 16;
 
+// Threads of a row in the softmax, and its warps.
+constexpr uint32_t row_threads(bool f32) { return f32 ? 1 : 2; }
+constexpr uint32_t soft_warps(bool f32) { return 8 * row_threads(f32); }
+
 // Q tiles: scaled by a power of two for each row so that its largest element is
 // in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.  Of the
 // 8 warps each reads whole rows, 16 lanes (bf16) or 32 (f32) each: with a row a
@@ -73,12 +79,15 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
     using namespace tc05;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     constexpr uint32_t kLanes = F32 ? 32 : 16, kAtOnce = 32 / kLanes;
-    const uint32_t c = lane % kLanes;
-    for (uint32_t x0 = warp * (rows / 8u); x0 < (warp + 1u) * (rows / 8u); x0 += 8u * kAtOnce) {
+    constexpr uint32_t kWarps = soft_warps(F32);
+    const uint32_t c = lane % kLanes, n = rows / (kWarps * kAtOnce);  // trips of a warp
+    for (uint32_t i0 = 0; i0 < n; i0 += 8u) {
+        const uint32_t x0 = (warp * n + i0) * kAtOnce;
         uint4 raw[8];
         float scale[8];
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
+            if (i0 + i >= n) break;
             const uint32_t x = x0 + i * kAtOnce + lane / kLanes;  // row of both tiles
             const uint32_t sl = (x & 127u) / G, hl = (x & 127u) - sl * G;
             const PrefixSeq q = tab[min((mt0 + (x >> 7)) * T + sl, n_seqs - 1u)];
@@ -86,6 +95,7 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
+            if (i0 + i >= n) break;
             const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
             float top = 0.f;
 #pragma unroll
@@ -98,6 +108,7 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
+            if (i0 + i >= n) break;
             const uint32_t x = x0 + i * kAtOnce + lane / kLanes, r = x & 127u;
             const int e = max(-126, min(126, (int)((__float_as_uint(scale[i]) >> 23) & 255u) - 127));
             const float f = __int_as_float((127 - e) << 23);
@@ -128,8 +139,19 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
     fence_async_smem();
 }
 
+// Whether any thread of two warps (named barrier `id`), or of all softmax warps, says so.
+__device__ __forceinline__ bool bar_any(uint32_t id, uint32_t threads, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r) : "r"((uint32_t)x), "r"(id), "r"(threads) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ bool pair_any(uint32_t id, bool x) { return bar_any(id, 64, x); }
+__device__ __forceinline__ bool soft_any(uint32_t threads, bool x) { return bar_any(9, threads, x); }
+
 template <bool F32, int NS>
-__global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
+__global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
     using namespace tc05;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     enum { B_KFULL = 0, B_KEMPTY = 3, B_VFULL = 6, B_VEMPTY = 8, B_SFULL = 10, B_PFULL = 12, B_ODONE = 14, N_BARS = 16 };
@@ -137,7 +159,9 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
     __shared__ __align__(8) uint64_t bars[N_BARS];
     __shared__ uint32_t tmem_base_sh;
     __shared__ volatile int abort_sh;
-    __shared__ float2 ml_sh[2][128];  // [stream][row] (m, l)
+    constexpr uint32_t H = row_threads(F32), kSoft = soft_warps(F32);
+    __shared__ float2 ml_sh[2][H][128];  // [stream][half][row] (m, l)
+    __shared__ float top_sh[2][H][128];
     __shared__ float qscale_sh[2][128];
 
     const uint32_t sraw = (uint32_t)__cvta_generic_to_shared(smem_raw);
@@ -169,7 +193,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
             bar_init(bar(B_VFULL + t), 1);
             bar_init(bar(B_VEMPTY + t), 1);
             bar_init(bar(B_SFULL + t), 1);
-            bar_init(bar(B_PFULL + t), 128);
+            bar_init(bar(B_PFULL + t), 128 * H);
             bar_init(bar(B_ODONE + t), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;");
@@ -186,9 +210,9 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
     // The sequences' table is read by generic loads: lane-divergent constant loads replay.
     const PrefixSeq *tab = P.seq;
     asm volatile("" : "+l"(tab));
-    if (warp < 8)
+    if (warp < kSoft)
         load_q<F32>(tab + Gr.seq0, Gr.n_seqs, mt0, solo ? 128u : 256u, kvh, G, T, gsm + T_Q * kTile, &qscale_sh[0][0]);
-    const uint32_t st = warp >> 2;  // stream of a softmax warp
+    const uint32_t st = warp / (4u * H), half = (warp >> 2) % H;  // of a softmax warp
     const uint32_t r = ((warp & 3u) << 5) | lane;
     const uint32_t sl = r / G;
     const uint32_t mt = solo ? mt0 : mt0 + (st & 1u);
@@ -200,7 +224,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
     fence_after();
     const uint32_t tmem = tmem_base_sh;
 
-    if (warp == 9) {
+    if (warp == kSoft + 1) {
         // ---------------- TMA loader: a ring of K tiles and one of V tiles ----------------
         auto loader = [&](auto kind) {
             constexpr uint32_t kRing = decltype(kind)::value && !F32 ? 3 : 2, kTile0 = kRing == 3 ? 1 : T_K;
@@ -230,7 +254,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
             if (solo) loader(std::true_type());
             else loader(std::false_type());
         }
-    } else if (warp == 8) {
+    } else if (warp == kSoft) {
         // ---------------- MMA issuer ----------------
         // Step i belongs to stream i & 1 and takes key tile i (solo) or i / 2 (pair).  S
         // of step i + 2 overwrites the columns from which PV of step i reads P: MMAs
@@ -294,7 +318,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
         };
         if (lane == 0 && !(solo ? issuer(std::true_type()) : issuer(std::false_type()))) abort_sh = 1;
     } else {
-        // ---------------- softmax of stream st, one row a thread ----------------
+        // ---------------- softmax of stream st, H threads a row ----------------
         const uint32_t lane_off = ((warp & 3u) * 32u) << 16;
         const uint32_t t_s = tmem + st * 128u + lane_off, t_o = tmem + 256u + st * 128u + lane_off;
         const uint32_t s_row = max(first, kbeg);
@@ -308,7 +332,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
         float *sums = P.part + (st == 0 ? row - r : ((uint64_t)P.take0 + blockIdx.x) * 128u) * 128u + r;  // [column][row]
         float m_taken = kNone;
         // 32 columns of O and of the sums
-        auto read_o = [&](int c, bool add, float scale, float (&v)[32]) {
+        auto read_o = [&](uint32_t c, bool add, float scale, float (&v)[32]) {
             tmem_ld32(t_o + c * 32u, v);
             tmem_wait_ld();
             if (add) {
@@ -320,7 +344,7 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
             const uint32_t k0 = kbeg + (solo ? 2u * s + st : s) * 128u;
             __syncwarp();
             ok = !abort_sh && wait_bar_warp(bar(B_SFULL + st), s & 1u);
-            if (!ok) break;
+            if (H == 1 && !ok) break;
             fence_after();
             if (F32 && s > 0 && s % kTake == 0) {  // PV of this step starts O anew
                 const float scale = fast_exp2(m_taken - m);
@@ -335,11 +359,11 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
             }
             const bool edge = __any_sync(0xffffffffu, k0 < s_row || k0 + 128u > kend);
             // scores 32c .. 32c+31, -inf outside the row's keys
-            auto mask = [&](int c, float (&x)[32]) {
+            auto mask = [&](uint32_t c, float (&x)[32]) {
                 if (edge)
 #pragma unroll
                     for (int i = 0; i < 32; i++)
-                        if (k0 + 32u * c + i < s_row || k0 + 32u * c + i >= kend) x[i] = -INFINITY;
+                        if (k0 + 32u * c + (uint32_t)i < s_row || k0 + 32u * c + (uint32_t)i >= kend) x[i] = -INFINITY;
             };
             auto top_of = [&](const float (&x)[32]) {
                 float a = x[0], b = x[1];
@@ -350,65 +374,138 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
                 }
                 return fmaxf(a, b);
             };
-            // The first half is read twice, the second half stays in registers.
-            float v[2][32], u[2][32];
-            tmem_ld32(t_s, u[0]);
-            tmem_ld32(t_s + 32u, u[1]);
-            tmem_wait_ld();
-            tmem_ld32(t_s + 64u, v[0]);
-            tmem_ld32(t_s + 96u, v[1]);
-            mask(0, u[0]);
-            mask(1, u[1]);
-            float mx = fmaxf(top_of(u[0]), top_of(u[1]));
-            tmem_wait_ld();
-            tmem_ld32(t_s, u[0]);
-            mask(2, v[0]);
-            mask(3, v[1]);
-            const float top = fmaxf(mx, fmaxf(top_of(v[0]), top_of(v[1]))) * qs;
-            const bool raise = top - m > kRaise;
-            if (__any_sync(0xffffffffu, raise)) {
-                const float mn = raise ? top - kHead : m, alpha = fast_exp2(m - mn);
-                if (s > 0) {
-#pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float o[32];
-                        tmem_ld32(t_o + c * 32u, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] *= alpha;
-                        tmem_st32(t_o + c * 32u, o);
-                    }
-                }
-                l *= alpha;
-                m = mn;
-            }
-            // P over S: keys 32c .. 32c+31 in columns 16c .. 16c+15 (remainders 64 columns on)
             float la = 0.f, lb = 0.f;
-            auto weigh = [&](int c, const float (&x)[32]) {
-                uint32_t w[16], wl[16];
+            if constexpr (H == 1) {
+                // The first half is read twice, the second half stays in registers.
+                float v[2][32], u[2][32];
+                tmem_ld32(t_s, u[0]);
+                tmem_ld32(t_s + 32u, u[1]);
+                tmem_wait_ld();
+                tmem_ld32(t_s + 64u, v[0]);
+                tmem_ld32(t_s + 96u, v[1]);
+                mask(0, u[0]);
+                mask(1, u[1]);
+                float mx = fmaxf(top_of(u[0]), top_of(u[1]));
+                tmem_wait_ld();
+                tmem_ld32(t_s, u[0]);
+                mask(2, v[0]);
+                mask(3, v[1]);
+                const float top = fmaxf(mx, fmaxf(top_of(v[0]), top_of(v[1]))) * qs;
+                const bool raise = top - m > kRaise;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float mn = raise ? top - kHead : m, alpha = fast_exp2(m - mn);
+                    if (s > 0) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
-                    la += p0;
-                    lb += p1;
-                    w[i] = pack_h2(p0, p1);
-                    if (F32) {
-                        const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-                        wl[i] = pack_h2(p0 - h.x, p1 - h.y);
+                        for (int c = 0; c < 4; c++) {
+                            float o[32];
+                            tmem_ld32(t_o + c * 32u, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] *= alpha;
+                            tmem_st32(t_o + c * 32u, o);
+                        }
                     }
+                    l *= alpha;
+                    m = mn;
                 }
-                tmem_st16u(t_s + c * 16u, w);
-                if (F32) tmem_st16u(t_s + 64u + c * 16u, wl);
-            };
-            tmem_wait_ld();
-            mask(0, u[0]);
-            weigh(0, u[0]);
-            tmem_ld32(t_s + 32u, u[1]);
-            tmem_wait_ld();
-            mask(1, u[1]);
-            weigh(1, u[1]);
-            weigh(2, v[0]);
-            weigh(3, v[1]);
+                // P over S: keys 32c .. 32c+31 in columns 16c .. 16c+15 (remainders 64 columns on)
+                auto weigh = [&](int c, const float (&x)[32]) {
+                    uint32_t w[16], wl[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
+                        la += p0;
+                        lb += p1;
+                        w[i] = pack_h2(p0, p1);
+                        if (F32) {
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                            wl[i] = pack_h2(p0 - h.x, p1 - h.y);
+                        }
+                    }
+                    tmem_st16u(t_s + c * 16u, w);
+                    if (F32) tmem_st16u(t_s + 64u + c * 16u, wl);
+                };
+                tmem_wait_ld();
+                mask(0, u[0]);
+                weigh(0, u[0]);
+                tmem_ld32(t_s + 32u, u[1]);
+                tmem_wait_ld();
+                mask(1, u[1]);
+                weigh(1, u[1]);
+                weigh(2, v[0]);
+                weigh(3, v[1]);
+            } else {
+                // Columns 64 * half on.  The weights are taken with the reference of the tiles
+                // before, which holds as a rule; where a row's does not, both threads of
+                // every row of the warp pair begin again (P is not written yet).
+                uint32_t w[32];
+                auto weigh = [&](int c, const float (&x)[32]) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
+                        la += p0;
+                        lb += p1;
+                        w[16 * c + i] = pack_h2(p0, p1);
+                    }
+                };
+                const uint32_t t_h = t_s + 64u * half;
+                bool raise = false;
+                float top = 0.f;
+                if (ok) {
+                    float v[32], u[32];
+                    tmem_ld32(t_h, v);
+                    tmem_wait_ld();
+                    tmem_ld32(t_h + 32u, u);
+                    mask(2 * half, v);
+                    top = top_of(v);
+                    weigh(0, v);
+                    tmem_wait_ld();
+                    mask(2 * half + 1, u);
+                    top = fmaxf(top, top_of(u)) * qs;
+                    weigh(1, u);
+                    raise = top - m > kRaise;
+                }
+                const uint32_t pair = 1u + st * 4u + (warp & 3u);
+                fence_before();
+                if (pair_any(pair, raise || !ok)) {
+                    fence_after();
+                    top_sh[st][half][r] = top;
+                    if (pair_any(pair, !ok)) {
+                        ok = false;
+                        break;
+                    }
+                    top = fmaxf(top, top_sh[st][half ^ 1u][r]);
+                    raise = top - m > kRaise;
+                    const float mn = raise ? top - kHead : m, alpha = fast_exp2(m - mn);
+                    if (s > 0) {
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            float o[32];
+                            tmem_ld32(t_o + 64u * half + c * 32u, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] *= alpha;
+                            tmem_st32(t_o + 64u * half + c * 32u, o);
+                        }
+                    }
+                    l *= alpha;
+                    m = mn;
+                    la = lb = 0.f;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        float v[32];
+                        tmem_ld32(t_h + c * 32u, v);
+                        tmem_wait_ld();
+                        mask(2 * half + c, v);
+                        weigh(c, v);
+                    }
+                    fence_before();
+                    pair_any(pair, false);
+                }
+                fence_after();
+#pragma unroll
+                for (int c = 0; c < 2; c++) tmem_st16u(t_s + 32u * half + c * 16u, *reinterpret_cast<uint32_t(*)[16]>(&w[16 * c]));
+            }
             l += la + lb;
             tmem_wait_st();
             fence_before();
@@ -420,34 +517,42 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
         const float w_taken = fast_exp2(m_taken - m);
         const float *ob = reinterpret_cast<const float *>(gsm + T_K * kTile);  // stream 1's O, [128 columns][128 rows]
         float wA = 1.f;
-        ml_sh[st][r] = make_float2(m, l);
-        asm volatile("bar.sync 9, 256;" ::: "memory");  // both streams' MMAs are done: the K and V tiles are free
+        ml_sh[st][half][r] = make_float2(m, l);
+        // Both streams' MMAs are done: the K and V tiles are free.  All go on, or none.
+        ok = !soft_any(kSoft * 32u, abort_sh);
         fence_after();
+        if (H == 2) l = ml_sh[st][0][r].y + ml_sh[st][H - 1][r].y;
         if (solo) {
             // Join the streams: stream 1 leaves its O, scaled, in the K tiles.
-            const float2 a = ml_sh[0][r], b = ml_sh[1][r];
+            float2 a = ml_sh[0][0][r], b = ml_sh[1][0][r];
+            if (H == 2) {
+                a.y += ml_sh[0][H - 1][r].y;
+                b.y += ml_sh[1][H - 1][r].y;
+            }
             m = fmaxf(a.x, b.x);
             wA = fast_exp2(a.x - m);
             const float wB = fast_exp2(b.x - m);
             l = a.y * wA + b.y * wB;
-            if (st == 1 && nt > 1 && !abort_sh) {
+            if (st == 1 && nt > 1 && ok) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (uint32_t k = 0; k < 4 / H; k++) {
+                    const uint32_t c = half * (4 / H) + k;
                     float v[32];
                     read_o(c, took, w_taken, v);
 #pragma unroll
                     for (int i = 0; i < 32; i++) const_cast<float *>(ob)[(c * 32u + i) * 128u + r] = v[i] * wB;
                 }
             }
-            asm volatile("bar.sync 9, 256;" ::: "memory");
+            soft_any(kSoft * 32u, false);
         }
-        if (!abort_sh && (!solo || st == 0)) {
+        if (ok && (!solo || st == 0)) {
             // O goes through shared memory (16-byte chunk c of row r at c ^ (r & 31)), so that
             // the global stores are whole rows: stream 0 by the V tiles, stream 1 by the K tiles
             // (solo: stream 1's O is there until it is added).
             uint8_t *tile_sm = gsm + (st == 0 ? T_V : T_K) * kTile;
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
+            for (uint32_t k = 0; k < 4 / H; k++) {
+                const uint32_t c = half * (4 / H) + k;
                 float v[32];
                 read_o(c, took, w_taken, v);
                 if (solo) {
@@ -463,15 +568,17 @@ __global__ void __launch_bounds__(320, 1) prefix_tc05_kernel(const __grid_consta
                         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
             if (took) asm volatile("bar.sync 10, 128;" ::: "memory");  // (the sums of all columns are read)
-            __syncwarp();  // a warp stores its own 32 rows
+            // a warp stores its own 32 rows, two that share them half of them each
+            if (H == 1) __syncwarp();
+            else pair_any(1u + st * 4u + (warp & 3u), false);
             const uint32_t rows = min(T, Gr.n_seqs - mt * T) * G;  // of the tile's, those that hold a head
-            const uint32_t r0 = (warp & 3u) * 32u;
+            const uint32_t r0 = (warp & 3u) * 32u + half * (32u / H);
             float *tile_out = P.part + (row - r) * 128u;
 #pragma unroll 8
-            for (uint32_t x = r0; x < min(r0 + 32u, rows); x++)
+            for (uint32_t x = r0; x < min(r0 + 32u / H, rows); x++)
                 *reinterpret_cast<float4 *>(tile_out + x * 128u + lane * 4u) =
                     *reinterpret_cast<const float4 *>(tile_sm + x * 512u + ((lane ^ (x & 31u)) << 4));
-            if (valid) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
+            if (valid && half == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
         }
     }
     fence_before();
@@ -609,7 +716,7 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
     P.kv_heads = kv_heads;
     P.tpt = prefix_seqs_per_tile(P.heads_per_kv);
     g_launches++;
-    return launch_early("prefix launch", prefix_tc05_kernel<F32, NS>, dim3(ctas), 320, smem, stream, P);
+    return launch_early("prefix launch", prefix_tc05_kernel<F32, NS>, dim3(ctas), soft_warps(F32) * 32 + 64, smem, stream, P);
 }
 
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
