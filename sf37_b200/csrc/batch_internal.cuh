@@ -108,6 +108,19 @@ __device__ __forceinline__ uint32_t i8_pack(float x, float y, float z, float w, 
     const uint32_t b = __byte_perm(i8_byte(z, s, inv), i8_byte(w, s, inv), 0x0040);
     return __byte_perm(a, b, 0x5410);
 }
+// The same without the decision; `worst` becomes the largest |remainder|.  The
+// codes are right if that is below s / 2 (all but those within 2^-16 of a tie).
+__device__ __forceinline__ uint32_t i8_pack_near(const float *x, float s, float inv, float &worst) {
+    constexpr float kMagic = 12582912.0f + 128.0f;
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float t = fmaf(x[i], inv, kMagic);
+        b[i] = __float_as_uint(t);
+        worst = fmaxf(worst, fabsf(fmaf(kMagic - t, s, x[i])));
+    }
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
 constexpr uint32_t kI8Zero = 0x80808080u;  // four zeros: also the codes of a NaN scale
 
 // Quantises one head (four elements a lane, all 32 lanes) and stores its codes

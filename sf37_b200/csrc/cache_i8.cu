@@ -48,12 +48,15 @@ __device__ __forceinline__ uint32_t job_of(const Begin &begin, uint32_t n, uint3
 
 // Eight lanes per head of one row, K and V together: 16 elements a lane in
 // 128-byte runs, all loads first; a head's maximum is three shuffles, and a code
-// six instructions.  8192 rows of 8 heads, bf16: 16 us, 3.2 TB/s (a warp a head
-// with integer conversions took 30 us).  Latency bounds it: 50 MB are 8 us of HBM.
+// four instructions, with one test of a lane's 16 remainders for a tie.  8192 rows of
+// 8 heads, bf16: 14 us, 3.6 TB/s (a warp a head with integer conversions took 30,
+// a test for each element 16; K and V in blocks of their own 17).  Latency and
+// instructions bound it: 50 MB are 8 us of HBM.
+constexpr uint32_t kAppendThreads = 128;
 template <bool BF16>
-__global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
+__global__ void __launch_bounds__(kAppendThreads) append_i8_kernel(const __grid_constant__ AppendI8Params P) {
     after_previous();
-    const uint32_t lane8 = threadIdx.x & 7u, unit = blockIdx.x * 32u + (threadIdx.x >> 3);
+    const uint32_t lane8 = threadIdx.x & 7u, unit = blockIdx.x * (kAppendThreads / 8u) + (threadIdx.x >> 3);
     const uint32_t row = unit / P.heads, head = unit - row * P.heads;
     const bool live = row < P.row_begin[P.n_jobs];
     const uint32_t j = live ? job_of(P.row_begin, P.n_jobs, P.rows_each, row) : 0u;
@@ -99,9 +102,14 @@ __global__ void __launch_bounds__(256) append_i8_kernel(const __grid_constant__ 
         for (int o = 4; o > 0; o >>= 1) a = max_abs_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
         const float s = i8_scale(a), inv = s > 0.f ? __frcp_rn(s) : 0.f;
         uint32_t codes[4];
+        float worst = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; q++)
-            codes[q] = s > 0.f ? i8_pack(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3], s, inv) : kI8Zero;
+        for (int q = 0; q < 4; q++) codes[q] = i8_pack_near(x + 4 * q, s, inv, worst);
+        if (!(worst + worst < s)) {  // a tie or one off, or a scale of 0 or NaN
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                codes[q] = s > 0.f ? i8_pack(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3], s, inv) : kI8Zero;
+        }
         if (!live) continue;
         uint8_t *cache = which ? J.v_cache : J.k_cache, *dst = cache + slot * kv_dim + head * 128u;
 #pragma unroll
@@ -255,9 +263,10 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
                 continue;
             }
             P.row_begin[P.n_jobs] = (uint32_t)rows;
-            const unsigned grid = (unsigned)((rows * kv_heads + 31u) / 32u);
+            const unsigned grid = (unsigned)((rows * kv_heads + kAppendThreads / 8u - 1u) / (kAppendThreads / 8u));
             g_launches++;
-            if (int rc = launch_early("append_i8 launch", bf16 ? append_i8_kernel<true> : append_i8_kernel<false>, grid, 256, 0,
+            if (int rc = launch_early("append_i8 launch", bf16 ? append_i8_kernel<true> : append_i8_kernel<false>, grid,
+                                      kAppendThreads, 0,
                                       s, P))
                 return rc;
         }
