@@ -66,8 +66,8 @@ constexpr float kNone = -1e30f;  // reference of a row without keys
 constexpr uint32_t kTake = 16;
 
 // Threads of a row in the softmax, and its warps.
-constexpr uint32_t row_threads(bool f32) { return f32 ? 1 : 2; }
-constexpr uint32_t soft_warps(bool f32) { return 8 * row_threads(f32); }
+__host__ __device__ constexpr uint32_t row_threads(bool f32) { return f32 ? 1 : 2; }
+__host__ __device__ constexpr uint32_t soft_warps(bool f32) { return 8 * row_threads(f32); }
 
 // Q tiles: scaled by a power of two for each row so that its largest element is
 // in [1, 2): f16 then holds a bf16 row exactly and hi + lo 22 bits.  Of the
