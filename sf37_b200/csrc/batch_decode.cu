@@ -54,7 +54,7 @@ constexpr float kNone = -1e30f;  // reference of a state without rows
 // after this many.
 constexpr uint32_t kTake = 32;
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
-constexpr uint32_t kSmallSeqs = 16, kMaxSeqs = 256;  // sequences per launch
+constexpr uint32_t kSmallSeqs = 16, kSomeSeqs = 64, kMaxSeqs = 256;  // sequences per launch
 constexpr uint32_t kMapped = 1024;     // slots with a direct map to their sequence
 // Range of the weights' power of two (kernel below): the ratio of two is finite.
 constexpr int kFMin = -86, kFMax = 40;
@@ -997,11 +997,15 @@ static int launch_n(SeqDev *seqs, uint32_t n, const BatchParams<1> &head, uint32
                                   Shape<MODE, I8, false>::kCtas,
                                   prefix_ctas < kPlanSms ? kPlanSms - prefix_ctas : kPlanSms);
     const bool after_prefix = prefix_ctas > 0;
-    // The descriptors travel as kernel parameters; a small launch carries few.
-    const bool few = n <= kSmallSeqs;
-    if (plan.wide && few) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
-    if (plan.wide) return launch<MODE, I8, true, kMaxSeqs>(seqs, n, plan, head, after_prefix, stream);
-    if (few) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
+    // The descriptors travel as kernel parameters (30 KB for kMaxSeqs, whose copies take
+    // the host some us); a small launch carries few, and a wide plan has few.
+    static_assert(kPlanSms / 4 <= kSomeSeqs, "sequences of a wide plan");
+    if (plan.wide) {
+        if (n <= kSmallSeqs) return launch<MODE, I8, true, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
+        return launch<MODE, I8, true, kSomeSeqs>(seqs, n, plan, head, after_prefix, stream);
+    }
+    if (n <= kSmallSeqs) return launch<MODE, I8, false, kSmallSeqs>(seqs, n, plan, head, after_prefix, stream);
+    if (n <= kSomeSeqs) return launch<MODE, I8, false, kSomeSeqs>(seqs, n, plan, head, after_prefix, stream);
     return launch<MODE, I8, false, kMaxSeqs>(seqs, n, plan, head, after_prefix, stream);
 }
 
