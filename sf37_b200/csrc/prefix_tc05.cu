@@ -26,13 +26,13 @@
 // raised when x - m passes 15: f16 holds them up to 2^15, and down to 2^-32 of
 // the largest.  S and O accumulate in f32 (TMEM), m and l in f32 registers.
 //
-// Bound by the tensor pipe and the softmax's latency: a step (S and PV of one
-// stream and key tile) is 1024 cycles of MMA, issues in 1400-1550 (8 MMAs and
-// their commits take 600 on an idle SM) and takes 2200, since two streams do not
-// hide each other's softmax wholly.  64 sequences x 64 heads over 32768 rows,
-// bf16: 85 us on 144 SMs, 0.81 PFLOP/s (0.48 of the measured burst bf16 rate); of
-// that 15 us are a CTA's start and end (64 KB of q and the first tiles, a 128 KB
-// partial out).
+// Bound by the MMA thread and the tensor pipe: a step (S and PV of one stream and
+// key tile) is 1024 cycles of MMA, issues in 1300-1500 (8 MMAs and their commits
+// take 600 on an idle SM, more beside the softmax) and takes 1850; its softmax takes
+// 1700 and is hidden by the other stream's.  64 sequences x 64 heads, bf16, no own
+// rows: 288 us over 131072 rows, 0.95 PFLOP/s (0.57 of the measured burst bf16
+// rate); 87 us over 32768, of which 15 are a CTA's start and end (64 KB of q and
+// the first tiles, a 128 KB partial out).
 #include <algorithm>
 #include <type_traits>
 
