@@ -7,7 +7,7 @@
 // one pass with a running reference m that is raised only when a score exceeds
 // it by more than 8.  I8 rows enter as their integer codes: a key's scale
 // multiplies its score, a value's scale its weight.  q . codes is a product of
-// integers (q as two or three 8-bit digits, s8 x u8 tiles, exact in s32), so
+// integers (q as three 8-bit digits, s8 x u8 tiles, exact in s32), so
 // keys need no conversion; value codes become f16, exactly.
 //
 // One CTA serves one KV head of one sequence over a run of rows (a split), so
@@ -31,12 +31,15 @@
 //
 // Sixteen M rows of a tile hold, by MODE:
 //   kPair  G <= 8, f32: eight heads twice, f16 "hi" and remainder "lo" of the weights
-//          (and of an f16 path's q), 22 bits at no extra cost; I8: q in three digits;
-//   kHalf  G <= 8, bf16: the same; I8: q in two digits, off by at most 2^-14 of the
-//          head's largest power of two (a bf16 q itself by 2^-8 of each element);
+//          (and of an f16 path's q), 22 bits at no extra cost;
+//   kHalf  G <= 8, bf16: the same without sums of their own (kTake);
 //   kWide  G <= 16 and bf16: sixteen heads, weights rounded to f16 (half a step is
-//          2^-11 of a weight; the output's own rounding has 2^-8), I8: two digits;
+//          2^-11 of a weight; the output's own rounding has 2^-8);
 //   kTwo   G <= 16 and f32: two kPair tiles on the same K/V fragments.
+// I8 takes q in three 8-bit digits throughout, off by at most 2^-22 of the head's
+// largest power of two.  Two digits (2^-14 of it) would be 7% faster with bf16 (64
+// sequences of 1 to 8192 rows 98.5 us against 105.8, one of 131072 48.0 against 52.7),
+// but a channel of 100 times the rest then puts the output off by more than its rounding.
 #include <algorithm>
 #include <climits>
 #include <cstring>
@@ -269,7 +272,7 @@ struct Shape {
     static constexpr uint32_t kArea = kWarps * kStages * Stage<I8>::kBytes;
     // q: an I8 q in kDigits digits of 8 bits, eight rows (a group) each, two groups a
     // tile of 16 rows; an f16 q in tiles of the weights' layout
-    static constexpr int kDigits = MODE == kHalf || MODE == kWide ? 2 : 3;
+    static constexpr int kDigits = 3;
     static constexpr int kGroups = kDigits * (MODE == kWide || MODE == kTwo ? 2 : 1);
     static constexpr int kQTiles = I8 ? (kGroups + 1) / 2 : MODE == kTwo ? 2 : 1;
     static constexpr uint32_t kQArea = (8 * 32 * 16) * (!I8 && MODE == kTwo ? 2 : I8 && kQTiles > 2 ? 2 : 1);
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 
     // q, scaled by a power of two for each head so that its largest element is in
     // [1, 2): as f16 (a bf16 q exactly, an f32 one in two parts), or, for I8, as
-    // integers q * 2^21 or 2^13 in signed digits of 8 bits.
+    // integers q * 2^21 in signed digits of 8 bits.
     if (warp < NH) {
         const uint32_t h = warp * 8u + g;
         float top = 0.f;
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         int e2;
         const float f = pow2_below(top, e2);
-        constexpr int kBits = ND == 3 ? 21 : 13;
+        constexpr int kBits = 21;
         if (t == 0) qfac[h] = pow2(e2) * (1.4426950408889634f * 0.08838834764831845f) * (I8 ? 1.f / (1 << kBits) : 1.f);
         uint32_t *Q32 = reinterpret_cast<uint32_t *>(Qs);
         if (I8) {
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                     const float x = (e == 0 ? qx[kk].x : e == 1 ? qx[kk].y : e == 2 ? qx[kk].z : qx[kk].w) * f;
                     finite = finite && fabsf(x) < 2.f;
                     // bytes of v + 0x80..80 are the digits of v plus 128
-                    const uint32_t v = (uint32_t)(__float2int_rn(x * (float)(1 << kBits)) + (ND == 3 ? 0x808080 : 0x8080));
+                    const uint32_t v = (uint32_t)(__float2int_rn(x * (float)(1 << kBits)) + 0x808080);
 #pragma unroll
                     for (int d = 0; d < ND; d++) {  // digit 0 is the highest
                         const uint32_t byte = (v >> (8 * (ND - 1 - d))) & 255u;
@@ -572,9 +575,8 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 #pragma unroll
                     for (int h = 0; h < NH; h++) {
                         auto digit = [&](int d) { return s[(h * ND + d) >> 1][i][e + 2 * ((h * ND + d) & 1)]; };
-                        // two digits: below 2^31; a third: two f32 roundings of the sum
-                        const int top2 = digit(0) * 256 + digit(1);
-                        sc[h][i][e] = ND == 3 ? fmaf((float)top2, 256.f, (float)digit(ND - 1)) : (float)top2;
+                        // two digits: below 2^31; the third: two f32 roundings of the sum
+                        sc[h][i][e] = fmaf((float)(digit(0) * 256 + digit(1)), 256.f, (float)digit(2));
                     }
             }
         } else {
