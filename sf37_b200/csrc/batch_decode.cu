@@ -84,6 +84,7 @@ struct BatchParams {
     uint32_t after_prefix, join;  // sequences with a prefix are joined by join_kernel
     float *part;          // [cta][part_stride(G)]: O [G][128], then (m, l) [G]
     uint32_t *counters;   // [sequence][kv head]
+    PrefixSync *sync;
     const float *pre_part, *pre_ml;
 };
 
@@ -299,9 +300,10 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
 
     // Launched early (programmatic dependent launch), the CTAs wait here for the
     // kernel before, whatever it was; after a prefix launch, which has itself waited
-    // and writes partials only, they may read caches and q at once.
-    if (!P.after_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;");
+    // and writes partials only, they may read caches and q once its flag tells that.
+    if (P.after_prefix) after_published(P.sync);
+    else asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
     const uint32_t slot_id = blockIdx.x / P.kv_heads, kvh = blockIdx.x - slot_id * P.kv_heads;
     uint32_t lo = 0;
@@ -756,6 +758,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
     }
     cp_wait<0>();
     __syncthreads();  // the stages become the merge buffer
+    if (P.after_prefix && tid == 0) leave_published(P.sync);
 
     // ---- the warps' states to one ----
     float *Os = reinterpret_cast<float *>(smem);  // [warp*16 + head][128]
@@ -935,16 +938,17 @@ static uint32_t seqs_per_launch(uint32_t kv_heads) {
     return (uint32_t)std::min<uint64_t>(kMaxSeqs, kCounters / kv_heads);
 }
 
-// Workspace: counters, own partials, prefix partial tiles, their (max, sum) pairs.
+// Workspace: counters, a PrefixSync, own partials, prefix partial tiles, their (max, sum) pairs.
 struct Layout {
-    uint64_t part, pre, ml, bytes;
+    uint64_t sync, part, pre, ml, bytes;
 };
 static Layout layout(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads, bool shared) {
     const uint64_t n = std::min<uint64_t>(n_seqs, seqs_per_launch(kv_heads)), g = std::min<uint64_t>(n_groups, kPrefixGroups);
     const uint64_t ctas = n * kv_heads + kMaxCtas;
     const uint64_t tiles = shared ? prefix_tiles_bound(g, n, q_heads, kv_heads) : 0;
     Layout w;
-    w.part = kCounters * 4u;
+    w.sync = kCounters * 4u;
+    w.part = w.sync + 256u;
     w.pre = (w.part + ctas * part_stride(q_heads / kv_heads) * 4u + 255u) / 256u * 256u;
     w.ml = w.pre + tiles * 128u * 128u * 4u;
     w.bytes = w.ml + tiles * 128u * 2u * 4u;
@@ -978,6 +982,7 @@ static int launch(const SeqDev *seqs, uint32_t n, const Plan &plan, const BatchP
     P.bf16 = head.bf16;
     P.part = head.part;
     P.counters = head.counters;
+    P.sync = head.sync;
     P.pre_part = head.pre_part;
     P.pre_ml = head.pre_ml;
     // After a prefix launch the CTAs start on the SMs that it leaves, and stream their own
@@ -1112,6 +1117,7 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
     head.kv_heads = kv_heads;
     head.bf16 = io_type == SF37KV_Q_BF16;
     head.counters = (uint32_t *)ws;
+    head.sync = (PrefixSync *)(ws + W.sync);
     head.part = (float *)(ws + W.part);
     head.pre_part = (const float *)(ws + W.pre);
     head.pre_ml = (const float *)(ws + W.ml);
@@ -1177,7 +1183,7 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
             }
             if (n_pg)
                 if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
-                                              (float *)(ws + W.ml), stream))
+                                              (float *)(ws + W.ml), head.sync, stream))
                     return rc;
             const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, prefix_ctas, stream)
                                               : launch_mode<false>(sd, n, head, prefix_ctas, stream);

@@ -55,10 +55,42 @@ static int launch_early(const char *what, Kernel kernel, dim3 grid, unsigned thr
     if (e == cudaSuccess) e = cudaGetLastError();
     return check_cuda(e, what);
 }
-// Waits for the kernel before, then lets the next one start.
+// Waits for the kernel before, then lets the next one start.  What the kernel before
+// wrote is read by plain loads from here on: a kernel that starts early may not
+// read it as data that is constant for its whole run (ld.global.nc).
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
+}
+
+// Two words of a workspace, zero between calls: `ready` is set by the prefix launch once
+// all work before it is complete and visible to it, and read by the decode launch that
+// runs beside it; `done` counts that launch's CTAs, the last of which clears both.
+struct PrefixSync {
+    uint32_t ready, done;
+};
+// Of one thread, after griddepcontrol.wait.
+__device__ __forceinline__ void publish_previous(PrefixSync *sync) {
+    asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(&sync->ready) : "memory");
+}
+// Of a warp of the launch that starts while the prefix launch runs: orders what follows
+// after all work that the prefix launch waited for.  The release above and this
+// acquire do so, and as a rule the flag is there at the first look, since the launch
+// starts after it; where it is not, the warp waits for the prefix launch itself.
+__device__ __forceinline__ void after_published(const PrefixSync *sync) {
+    uint32_t seen = 0;
+    if ((threadIdx.x & 31u) == 0)
+        for (int i = 0; i < 16 && !seen; i++)
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(&sync->ready) : "memory");
+    if (!__shfl_sync(0xffffffffu, seen, 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
+    __syncwarp();
+}
+// Of one thread of each CTA of that launch, when its warps are past after_published().
+__device__ __forceinline__ void leave_published(PrefixSync *sync) {
+    uint32_t prev;
+    asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                 : "=r"(prev) : "l"(&sync->done), "r"(gridDim.x - 1u) : "memory");
+    if (prev == gridDim.x - 1u) sync->ready = 0u;
 }
 
 __device__ __forceinline__ uint32_t h2_bits(float a, float b) {
@@ -68,8 +100,8 @@ __device__ __forceinline__ uint32_t h2_bits(float a, float b) {
 
 // Four consecutive elements of an f32 or bf16 array (16- or 8-byte aligned).
 __device__ __forceinline__ float4 load_row4(const void *p, uint64_t i, bool bf16) {
-    if (!bf16) return __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i));
-    const uint2 w = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i));
+    if (!bf16) return *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
+    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(p) + i);
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                        __uint_as_float(w.y & 0xffff0000u));
 }
@@ -170,6 +202,6 @@ uint32_t prefix_plan(PrefixGroup *groups, uint32_t n, uint32_t q_heads, uint32_t
 // Partial tiles that prefix_plan() stays within.
 uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads, uint32_t kv_heads);
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
-                     uint32_t kv_heads, bool f32, float *part, float *ml, cudaStream_t stream);
+                     uint32_t kv_heads, bool f32, float *part, float *ml, PrefixSync *sync, cudaStream_t stream);
 
 }  // namespace sf37kv

@@ -71,8 +71,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_i8_kernel(const __grid_
         for (uint32_t i = 0; i < kRuns; i++) {
             const uint64_t at = src + (i * 8u + lane8) * kRun;
             const uint32_t size = BF16 ? 2u : 4u;
-            raw[0][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.k) + at * size));
-            raw[1][i] = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.v) + at * size));
+            raw[0][i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.k) + at * size);
+            raw[1][i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(J.v) + at * size);
         }
     } else {
 #pragma unroll
@@ -166,10 +166,10 @@ __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ Re
                 uint32_t a = s_src + r, b = s_dst + r;
                 if (a >= J.src_cap) a = a - J.src_cap < J.src_cap ? a - J.src_cap : a % J.src_cap;
                 if (b >= J.dst_cap) b = b - J.dst_cap < J.dst_cap ? b - J.dst_cap : b % J.dst_cap;
-                s[k] = __ldg(scales + (uint64_t)(c / (128u / E)) * J.src_cap + a);
+                s[k] = scales[(uint64_t)(c / (128u / E)) * J.src_cap + a];
                 const uint8_t *p = src + a * kv_dim + c * E;
-                if (F16) w[k] = __ldg(reinterpret_cast<const uint2 *>(p));
-                else w[k].x = __ldg(reinterpret_cast<const uint32_t *>(p));
+                if (F16) w[k] = *reinterpret_cast<const uint2 *>(p);
+                else w[k].x = *reinterpret_cast<const uint32_t *>(p);
                 to[k] = b * kv_dim + c * E;
             }
         }

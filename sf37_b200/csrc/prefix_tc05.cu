@@ -54,6 +54,7 @@ struct PrefixParams {
     PrefixDev group[kPrefixGroups];
     PrefixSeq seq[NS];
     float *part, *ml;
+    PrefixSync *sync;
     uint32_t take0;  // first of one partial tile for each CTA, for stream 1's sums (F32)
     uint32_t n_groups, heads_per_kv, kv_heads, tpt;
 };
@@ -91,7 +92,7 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
             const uint32_t x = x0 + i * kAtOnce + lane / kLanes;  // row of both tiles
             const uint32_t sl = (x & 127u) / G, hl = (x & 127u) - sl * G;
             const PrefixSeq q = tab[min((mt0 + (x >> 7)) * T + sl, n_seqs - 1u)];
-            raw[i] = __ldg(reinterpret_cast<const uint4 *>(q.q) + (uint64_t)(kvh * G + hl) * kLanes + c);
+            raw[i] = reinterpret_cast<const uint4 *>(q.q)[(uint64_t)(kvh * G + hl) * kLanes + c];
         }
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
@@ -205,8 +206,11 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    // (the next kernel reads this one's partials after a wait of its own)
-    after_previous();
+    // The next kernel reads this one's partials after a wait of its own, and what was written
+    // before this one after the flag.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == 0 && tid == 0) publish_previous(P.sync);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     auto load = [&](uint32_t full, uint32_t dst, const CUtensorMap *map, uint32_t j) {
         const int32_t x = (int32_t)(kvh * 128u), y = (int32_t)(kbeg + j * 128u);
         bar_expect_tx(full, kTile);
@@ -678,7 +682,7 @@ uint64_t prefix_tiles_bound(uint64_t n_groups, uint64_t n_seqs, uint32_t q_heads
 
 template <bool F32, int NS>
 static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
-                  uint32_t kv_heads, float *part, float *ml, cudaStream_t stream) {
+                  uint32_t kv_heads, float *part, float *ml, PrefixSync *sync, cudaStream_t stream) {
     constexpr size_t smem = 6 * tc05::kTile + 1024;
     static bool ready[64];
     int dev = 0;
@@ -712,6 +716,7 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
     std::copy(seqs, seqs + n_seqs, P.seq);
     P.part = part;
     P.ml = ml;
+    P.sync = sync;
     const PrefixGroup &last = groups[n - 1];
     P.take0 = last.part0 + kv_heads * last.m_tiles * last.splits;
     P.n_groups = n;
@@ -723,12 +728,12 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
 }
 
 int prefix_attention(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, uint32_t n_seqs, uint32_t q_heads,
-                     uint32_t kv_heads, bool f32, float *part, float *ml, cudaStream_t stream) {
+                     uint32_t kv_heads, bool f32, float *part, float *ml, PrefixSync *sync, cudaStream_t stream) {
     if (n_seqs <= 32)
-        return f32 ? launch<true, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream)
-                   : launch<false, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream);
-    return f32 ? launch<true, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream)
-               : launch<false, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, stream);
+        return f32 ? launch<true, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, sync, stream)
+                   : launch<false, 32>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, sync, stream);
+    return f32 ? launch<true, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, sync, stream)
+               : launch<false, kPrefixSeqs>(groups, n, seqs, n_seqs, q_heads, kv_heads, part, ml, sync, stream);
 }
 
 int prefix_device_error(int clear) {
