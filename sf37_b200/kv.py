@@ -218,6 +218,38 @@ def oproj(layers, in_dim, out_dim, stream=None):
 _IO = {torch.float32: Q_F32, torch.bfloat16: Q_BF16}
 
 
+class Descriptors(np.ndarray):
+    """Descriptor array.  `held` says what its tensors hold (so do slices' and copies'); the calls refuse, before
+    anything is launched, head counts and types that do not fit them."""
+
+    def __array_finalize__(self, source):
+        self.held = getattr(source, "held", None)
+
+
+class _Held:
+    """device; kv_heads, q_heads: of the rows and queries, or None; cache_heads: the most that every cache has room
+    for; dtype: of the rows, queries or destinations; cache: of the caches."""
+
+    __slots__ = ("device", "kv_heads", "q_heads", "cache_heads", "dtype", "cache")
+
+    def __init__(self, device, cache_heads, dtype, cache, kv_heads=None, q_heads=None):
+        self.device, self.cache_heads, self.dtype, self.cache = device, cache_heads, dtype, cache
+        self.kv_heads, self.q_heads = kv_heads, q_heads
+
+    def check(self, what, kv_heads, dtype, cache=None, q_heads=None):
+        if self.kv_heads not in (None, kv_heads) or kv_heads > self.cache_heads:
+            has = f"rows of {self.kv_heads}" if self.kv_heads not in (None, kv_heads) else f"room for {self.cache_heads}"
+            raise ValueError(f"{what}: kv_heads is {kv_heads}, the tensors have {has}")
+        if q_heads is not None and q_heads != self.q_heads:
+            raise ValueError(f"{what}: q_heads is {q_heads}, the queries have {self.q_heads}")
+        if dtype != self.dtype:
+            raise ValueError(f"{what}: dtype is {dtype}, the tensors are {self.dtype}")
+        if cache is not None and cache != self.cache:
+            raise ValueError(f"{what}: caches of {cache} are needed, the descriptors' are {self.cache}")
+        if self.device != torch.cuda.current_device():
+            raise ValueError(f"{what}: the tensors are on CUDA device {self.device}, which is not the current one")
+
+
 def _addresses(name, x, n, dtypes=None, inner=None):
     """Addresses of the n items of a stacked tensor or a list of tensors."""
     items = [x] if isinstance(x, torch.Tensor) else list(x)
@@ -226,6 +258,8 @@ def _addresses(name, x, n, dtypes=None, inner=None):
             raise ValueError(f"{name}: tensors on the current CUDA device are needed, got {t.device}")
         if dtypes is not None and t.dtype not in dtypes:
             raise ValueError(f"{name}: dtype {t.dtype} is not one of {dtypes}")
+        if t.dtype != items[0].dtype:
+            raise ValueError(f"{name}: tensors of one dtype are needed, got {items[0].dtype} and {t.dtype}")
     if isinstance(x, torch.Tensor):
         if x.dim() < 1 or x.shape[0] != n:
             raise ValueError(f"{name}: a leading dimension of {n} is needed, got shape {tuple(x.shape)}")
@@ -251,11 +285,47 @@ def _item(x):
     return x[0]
 
 
+def _room(name, x, cap):
+    """KV heads that every cache of x has room for at its cap (an array), 128 elements (int8: 132 bytes) each."""
+    one = isinstance(x, torch.Tensor)
+    sizes = np.array([_item(x).numel()] if one else [t.numel() for t in x], dtype=np.int64)
+    per = (132 if _item(x).dtype == torch.uint8 else 128) * np.maximum(cap.astype(np.int64), 1)
+    heads = int((sizes // per).min())
+    if heads < 1:
+        raise ValueError(f"{name}: smaller than cap rows of one head")
+    return heads
+
+
+def _row_heads(name, items, rows):
+    """KV heads of row tensors [rows][kv_heads][128], the same in all."""
+    heads = None
+    for t, r in zip(items, rows):
+        if r == 0:
+            continue
+        h, rest = divmod(t.numel(), r * 128)
+        if rest or heads not in (None, h):
+            raise ValueError(f"{name}: rows of one number of heads of 128 are needed, got shape {tuple(t.shape)}")
+        heads = h
+    return heads
+
+
 def _records(layers, dtype, name):
     """Address and length of a descriptor array."""
     if layers.dtype != dtype or layers.ndim != 1 or not layers.flags.c_contiguous:
         raise ValueError(f"a contiguous array of {name}() is needed")
     return layers.ctypes.data, len(layers)  # (__array_interface__ lists all fields first: 12 us instead of 2)
+
+
+def _checked(layers, what, *args, **kwargs):
+    held = getattr(layers, "held", None)  # a plain array of records is the caller's own
+    if held is not None:
+        held.check(what, *args, **kwargs)
+
+
+def _space(workspace):
+    if not workspace.is_cuda or workspace.get_device() != torch.cuda.current_device() or not workspace.is_contiguous():
+        raise ValueError("workspace: a contiguous tensor on the current CUDA device is needed")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def i8_cache_bytes(cap, kv_heads, head_dim=128) -> int:
@@ -265,18 +335,25 @@ def i8_cache_bytes(cap, kv_heads, head_dim=128) -> int:
 
 def append_i8_desc(k_cache, v_cache, cap, pos0, k, v):
     """k, v: [n][n_tok][kv_heads][128] f32 or bf16 (or lists of [n_tok][kv_heads][128])."""
-    n, rows = _count(k), tuple(_item(k).shape)
-    d = np.zeros(n, APPEND_I8_LAYER)
+    n, stacked = _count(k), isinstance(k, torch.Tensor)
+    d = np.zeros(n, APPEND_I8_LAYER).view(Descriptors)
     d["k_cache"], d["v_cache"] = (_addresses("k_cache", k_cache, n, (torch.uint8,)),
                                   _addresses("v_cache", v_cache, n, (torch.uint8,)))
-    d["cap"], d["pos0"], d["n_tok"] = cap, pos0, rows[0] if isinstance(k, torch.Tensor) else [t.shape[0] for t in k]
-    inner = rows if isinstance(k, torch.Tensor) else None
-    d["k"], d["v"] = _addresses("k", k, n, tuple(_IO), inner), _addresses("v", v, n, (_item(k).dtype,), inner)
+    shapes = [tuple(_item(k).shape)] if stacked else [tuple(t.shape) for t in k]
+    d["cap"], d["pos0"], d["n_tok"] = cap, pos0, shapes[0][0] if stacked else [x[0] for x in shapes]
+    d["k"], d["v"] = _addresses("k", k, n, tuple(_IO)), _addresses("v", v, n, (_item(k).dtype,))
+    if any(tuple(a.shape) != tuple(b.shape) for a, b in ([(_item(k), _item(v))] if stacked and isinstance(v, torch.Tensor)
+                                                         else zip(k, v))):
+        raise ValueError("v: rows of the same shape as k's are needed")
+    heads = _row_heads("k", [_item(k)] if stacked else k, [x[0] for x in shapes])
+    d.held = _Held(_item(k).get_device(), min(_room("k_cache", k_cache, d["cap"]), _room("v_cache", v_cache, d["cap"])),
+                   _item(k).dtype, torch.uint8, heads)
     return d
 
 
 def append_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Quantises the rows of append_i8_desc() into their caches; dtype: the rows' torch dtype."""
+    _checked(layers, "append_i8", kv_heads, dtype)
     check(lib().sf37kv_append_i8(*_records(layers, APPEND_I8_LAYER, "append_i8_desc"), kv_heads, head_dim, _IO[dtype], _sp(stream)),
           "sf37kv_append_i8")
 
@@ -284,17 +361,21 @@ def append_i8(layers, kv_heads, head_dim, dtype, stream=None):
 def read_i8_desc(k_cache, v_cache, cap, dst_k, dst_v, dst_cap, first_pos, rows):
     """dst_k, dst_v: f16 or f32 caches of dst_cap rows, [n][dst_cap][kv_heads][128]."""
     n = _count(dst_k)
-    d = np.zeros(n, READ_I8_LAYER)
+    d = np.zeros(n, READ_I8_LAYER).view(Descriptors)
     d["src_k_cache"], d["src_v_cache"] = (_addresses("k_cache", k_cache, n, (torch.uint8,)),
                                           _addresses("v_cache", v_cache, n, (torch.uint8,)))
     d["dst_k_cache"] = _addresses("dst_k", dst_k, n, tuple(_DT))
     d["dst_v_cache"] = _addresses("dst_v", dst_v, n, (_item(dst_k).dtype,))
     d["src_cap"], d["dst_cap"], d["first_pos"], d["rows"] = cap, dst_cap, first_pos, rows
+    room = min(_room(name, x, d[at]) for name, x, at in (("k_cache", k_cache, "src_cap"), ("v_cache", v_cache, "src_cap"),
+                                                        ("dst_k", dst_k, "dst_cap"), ("dst_v", dst_v, "dst_cap")))
+    d.held = _Held(_item(dst_k).get_device(), room, _item(dst_k).dtype, torch.uint8)
     return d
 
 
 def read_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Reads the rows of read_i8_desc() back; dtype: the destinations' torch dtype."""
+    _checked(layers, "read_i8", kv_heads, dtype)
     check(lib().sf37kv_read_i8(*_records(layers, READ_I8_LAYER, "read_i8_desc"), kv_heads, head_dim, _DT[dtype], _sp(stream)),
           "sf37kv_read_i8")
 
@@ -302,18 +383,14 @@ def read_i8(layers, kv_heads, head_dim, dtype, stream=None):
 def decode_seqs_desc(k_cache, v_cache, cap, pos, q, out, gate=None, k_new=None, v_new=None, sliding=False,
                      window=512):
     """q, out: [n][q_heads][128] f32 or bf16; gate: [n][q_heads] f32; k_new, v_new: [n][kv_heads][128] like q;
-    caches: uint8 (int8 caches) or f16."""
+    caches: all uint8 (int8 caches) or all f16."""
     n = _count(q)
-    d = np.zeros(n, DECODE_SEQ)
-    cache = (torch.uint8, torch.float16)
-    d["k_cache"], d["v_cache"] = _addresses("k_cache", k_cache, n, cache), _addresses("v_cache", v_cache, n, cache)
+    d = np.zeros(n, DECODE_SEQ).view(Descriptors)
+    d["k_cache"] = _addresses("k_cache", k_cache, n, (torch.uint8, torch.float16))
+    d["v_cache"] = _addresses("v_cache", v_cache, n, (_item(k_cache).dtype,))
     d["cap"], d["sliding"], d["window"], d["pos"] = cap, np.asarray(sliding, dtype=bool), window, pos
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        per_row = 132 if _item(c).dtype == torch.uint8 else 128
-        sizes = [_item(c).numel()] * n if isinstance(c, torch.Tensor) else [t.numel() for t in c]
-        if any(s < int(r) * per_row for s, r in zip(sizes, d["cap"])):
-            raise ValueError(f"{name}: smaller than cap rows of one head")
-    heads, dtype = _item(q).shape[0], (_item(q).dtype,)
+    room = min(_room("k_cache", k_cache, d["cap"]), _room("v_cache", v_cache, d["cap"]))
+    heads, dtype, kv_heads = _item(q).shape[0], (_item(q).dtype,), None
     d["q"], d["out"] = _addresses("q", q, n, tuple(_IO), (heads, 128)), _addresses("out", out, n, dtype, (heads, 128))
     if gate is not None:
         d["gate"] = _addresses("gate", gate, n, (torch.float32,), (heads,))
@@ -322,6 +399,8 @@ def decode_seqs_desc(k_cache, v_cache, cap, pos, q, out, gate=None, k_new=None, 
     if k_new is not None:
         inner = tuple(_item(k_new).shape)
         d["k_new"], d["v_new"] = _addresses("k_new", k_new, n, dtype, inner), _addresses("v_new", v_new, n, dtype, inner)
+        kv_heads = _row_heads("k_new", [_item(k_new)], [1])
+    d.held = _Held(_item(q).get_device(), room, dtype[0], _item(k_cache).dtype, kv_heads, heads)
     return d
 
 
@@ -332,8 +411,9 @@ def decode_i8_workspace(n_seqs, q_heads, kv_heads) -> int:
 
 def decode_i8(seqs, q_heads, kv_heads, head_dim, dtype, workspace, stream=None):
     """One decode step over int8 caches; dtype: torch dtype of q and out."""
+    _checked(seqs, "decode_i8", kv_heads, dtype, torch.uint8, q_heads)
     check(lib().sf37kv_decode_i8(*_records(seqs, DECODE_SEQ, "decode_seqs_desc"), q_heads, kv_heads, head_dim, _IO[dtype],
-                                 workspace.data_ptr(), workspace.numel() * workspace.element_size(), _sp(stream)),
+                                 *_space(workspace), _sp(stream)),
           "sf37kv_decode_i8")
 
 
@@ -341,22 +421,24 @@ def shared_groups_desc(groups):
     """groups: list of dicts k_cache, v_cache (f16 [cap][kv_heads][128], or None), prefix_len, seqs (an array of
     decode_seqs_desc(), which the result refers to: later changes of it count)."""
     d = np.zeros(len(groups), SHARED_GROUP)
+    prefixes = []
     for i, g in enumerate(groups):
         if g["prefix_len"]:
-            k = [g["k_cache"]]
-            d[i]["prefix_k_cache"] = _addresses("prefix k_cache", k, 1, (torch.float16,))[0]
-            d[i]["prefix_v_cache"] = _addresses("prefix v_cache", [g["v_cache"]], 1, (torch.float16,))[0]
-            d[i]["prefix_cap"] = g["k_cache"].shape[0]
+            k, v = g["k_cache"], g["v_cache"]
+            d[i]["prefix_k_cache"] = _addresses("prefix k_cache", [k], 1, (torch.float16,))[0]
+            d[i]["prefix_v_cache"] = _addresses("prefix v_cache", [v], 1, (torch.float16,), tuple(k.shape))[0]
+            d[i]["prefix_cap"] = k.shape[0]
+            prefixes.append(_row_heads("prefix k_cache", [k], [k.shape[0]]))
         d[i]["prefix_len"] = g["prefix_len"]
         d[i]["seqs"], d[i]["n_seqs"] = _records(g["seqs"], DECODE_SEQ, "decode_seqs_desc")
-    return _Groups(d, [g["seqs"] for g in groups])
+    return _Groups(d, [g["seqs"] for g in groups], prefixes)
 
 
 class _Groups:
-    """Group descriptors, and the sequence arrays that they point to."""
+    """Group descriptors, the sequence arrays that they point to, and the KV heads of the prefixes."""
 
-    def __init__(self, desc, seqs):
-        self.desc, self.seqs = desc, seqs
+    def __init__(self, desc, seqs, prefixes):
+        self.desc, self.seqs, self.prefixes = desc, seqs, prefixes
 
 
 def decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads) -> int:
@@ -367,6 +449,10 @@ def decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads) -> int:
 def decode_shared(groups, q_heads, kv_heads, head_dim, cache_dtype, dtype, workspace, stream=None):
     """One decode step of groups that share a prefix; cache_dtype: F16 or I8, of the sequences' own caches."""
     d = groups.desc
+    for seqs in groups.seqs:
+        _checked(seqs, "decode_shared", kv_heads, dtype, torch.uint8 if cache_dtype == I8 else torch.float16, q_heads)
+    if any(h != kv_heads for h in groups.prefixes):
+        raise ValueError(f"decode_shared: kv_heads is {kv_heads}, the prefixes have {groups.prefixes}")
     check(lib().sf37kv_decode_shared(d.ctypes.data, len(d), q_heads, kv_heads, head_dim, cache_dtype, _IO[dtype],
-                                     workspace.data_ptr(), workspace.numel() * workspace.element_size(), _sp(stream)),
+                                     *_space(workspace), _sp(stream)),
           "sf37kv_decode_shared")
