@@ -211,7 +211,9 @@ int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n_layers, ui
 
 /* Reads positions first_pos .. first_pos + rows - 1 of I8 caches back into
  * f16 (rounded to nearest even) or f32 caches, position p to slot p % dst.cap.
- * rows <= both caps; other slots of dst are left as they were. */
+ * rows <= both caps; other slots of dst are left as they were.  The layers of a
+ * call run side by side: rows that one writes may not be another's, in its
+ * source or in what it writes (EINVAL). */
 typedef struct {
     sf37kv_cache src;      /* I8 */
     sf37kv_cache dst;      /* dst_dtype: SF37KV_F16 or SF37KV_F32 */

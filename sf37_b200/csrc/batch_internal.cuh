@@ -2,6 +2,10 @@
 // (cache_i8.cu, batch_decode.cu, prefix_tc05.cu).
 #pragma once
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include <cuda_bf16.h>
 
 #include "kv_internal.cuh"
@@ -31,6 +35,28 @@ static inline int check_cache(const char *what, uint32_t i, const sf37kv_cache &
     if (c.cap == 0 || c.cap > kMaxPos) return set_error(SF37KV_EINVAL, "%s: cache %u has cap %u", what, i, c.cap);
     if (c.k_cache == c.v_cache) return set_error(SF37KV_EINVAL, "%s: cache %u has one buffer for K and V", what, i);
     return SF37KV_OK;
+}
+
+// Memory that one call reads or writes, kernels of the call side by side.
+struct Span {
+    uintptr_t lo, hi;
+    bool writes;
+};
+static inline Span span_of(const void *p, uint64_t bytes, bool writes) {
+    return Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, writes};
+}
+// Whether a span that is written overlaps another one.  Reorders the spans.
+static inline bool spans_conflict(std::vector<Span> &s) {
+    const auto before = [](const Span &a, const Span &b) { return a.lo < b.lo; };
+    if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
+    uintptr_t any = 0, written = 0;  // ends of the spans so far
+    for (const Span &x : s) {
+        if (x.lo >= x.hi) continue;
+        if (x.lo < written || (x.writes && x.lo < any)) return true;
+        any = std::max(any, x.hi);
+        if (x.writes) written = std::max(written, x.hi);
+    }
+    return false;
 }
 
 // Launches a kernel that starts while the one before it on the stream drains

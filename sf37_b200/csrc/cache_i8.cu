@@ -13,8 +13,6 @@
 //
 // Both kernels move bytes and compute a few operations for each; HBM bounds
 // them, at (2 or 4) + 1.03 bytes for each element in either direction.
-#include <algorithm>
-
 #include "batch_internal.cuh"
 
 namespace sf37kv {
@@ -293,6 +291,26 @@ extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_lay
         if (L.src.k_cache == L.dst.k_cache || L.src.v_cache == L.dst.v_cache || L.src.k_cache == L.dst.v_cache ||
             L.src.v_cache == L.dst.k_cache)
             return set_error(SF37KV_EINVAL, "read_i8: layer %u reads and writes the same cache", i);
+    }
+    try {
+        // Destinations by the rows that are written: layers may fill parts of one cache.
+        std::vector<Span> spans;
+        spans.reserve((size_t)n_layers * 6);
+        for (int which = 0; which < 2; which++)
+            for (uint32_t i = 0; i < n_layers; i++) {
+                const sf37kv_read_i8_layer &L = layers[i];
+                if (L.rows == 0) continue;
+                const char *dst = (const char *)(which ? L.dst.v_cache : L.dst.k_cache);
+                const uint64_t row = (uint64_t)kv_heads * 128u * (uint64_t)dst_dtype, slot = L.first_pos % L.dst.cap,
+                               head = std::min<uint64_t>(L.rows, L.dst.cap - slot);
+                spans.push_back(span_of(dst + slot * row, head * row, true));
+                spans.push_back(span_of(dst, (L.rows - head) * row, true));
+                spans.push_back(span_of(which ? L.src.v_cache : L.src.k_cache, (uint64_t)L.src.cap * kv_heads * 132u, false));
+            }
+        if (spans_conflict(spans))
+            return set_error(SF37KV_EINVAL, "read_i8: rows that one layer writes are another's, read or written");
+    } catch (const std::bad_alloc &) {
+        return set_error(SF37KV_ENOMEM, "read_i8: no memory to compare %u layers", n_layers);
     }
     for (uint32_t base = 0; base < n_layers;) {
         ReadI8Params P;

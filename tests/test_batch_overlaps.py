@@ -1,0 +1,61 @@
+"""CPU: the int8 and batched decode calls refuse memory that one part of a call writes and another one uses,
+wherever in the call the two are."""
+import numpy as np
+import pytest
+
+from sf37_b200 import _lib
+
+EINVAL = 1
+P = 1 << 24  # addresses that no refused call touches, farther apart than the caches are long
+
+
+def _refused(rc, word):
+    assert rc == EINVAL and word in _lib.last_error(), (rc, _lib.last_error())
+
+
+# ------------------------------------------------------------ read back
+ROW = 8 * 128 * 2  # bytes of a destination row: 8 heads in f16
+
+
+def _read(n):
+    d = np.zeros(n, _lib.READ_I8_LAYER)
+    i = np.arange(n, dtype=np.uint64)
+    d["src_k_cache"], d["src_v_cache"] = P * (4 * i + 1), P * (4 * i + 2)
+    d["dst_k_cache"], d["dst_v_cache"] = P * (4 * i + 3), P * (4 * i + 4)
+    d["src_cap"], d["dst_cap"], d["rows"] = 16, 16, 4
+    return d
+
+
+def _read_call(d):
+    return _lib.lib().sf37kv_read_i8(d.ctypes.data, len(d), 8, 128, 2, None)
+
+
+@pytest.mark.parametrize("n,a,b", [(2, 0, 1), (3, 2, 0), (100, 1, 99)])
+def test_read_refuses_one_destination_twice(n, a, b):
+    for x, y in (("dst_k_cache", "dst_k_cache"), ("dst_v_cache", "dst_v_cache"), ("dst_k_cache", "dst_v_cache")):
+        d = _read(n)
+        d[x][b] = d[y][a]
+        _refused(_read_call(d), "another")
+        d[x][b] += 3 * ROW  # the last of the four rows
+        _refused(_read_call(d), "another")
+
+
+@pytest.mark.parametrize("n,a,b", [(2, 0, 1), (2, 1, 0), (100, 99, 1)])
+def test_read_refuses_a_destination_that_is_another_layers_source(n, a, b):
+    for x, y in (("src_k_cache", "dst_k_cache"), ("src_v_cache", "dst_k_cache")):
+        d = _read(n)
+        d[x][b] = d[y][a]
+        _refused(_read_call(d), "another")
+
+
+def test_read_refuses_rows_that_meet_past_a_rings_end():
+    d = _read(2)
+    d["dst_k_cache"][1], d["dst_v_cache"][1] = d["dst_k_cache"][0], d["dst_v_cache"][0]
+    d["first_pos"] = [14, 17]  # slots 14, 15, 0, 1 and 1 to 4
+    _refused(_read_call(d), "another")
+
+
+def test_read_refuses_k_and_v_that_overlap():
+    d = _read(1)
+    d["dst_v_cache"] = d["dst_k_cache"] + 2 * ROW
+    _refused(_read_call(d), "another")
