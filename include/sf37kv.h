@@ -198,7 +198,7 @@ uint64_t sf37kv_i8_cache_bytes(uint32_t cap, uint32_t kv_heads, uint32_t head_di
 
 /* Quantises n_tok rows per layer into slots (pos0 + t) % cap.  row_type:
  * SF37KV_Q_F32 or SF37KV_Q_BF16.  With n_tok > cap the last cap rows stay.  A
- * cache given twice in one call is refused. */
+ * cache given twice in one call, or one that overlaps another, is refused. */
 typedef struct {
     sf37kv_cache cache;
     uint32_t pos0;

@@ -188,16 +188,6 @@ __global__ void __launch_bounds__(256) read_i8_kernel(const __grid_constant__ Re
     }
 }
 
-// Whether two of the caches (K and V in turn, n in all) are one.
-static bool any_twice(const void **p, uint32_t n) {
-    // In one allocation, as a rule: in order, K apart from V.
-    bool ordered = true;
-    for (uint32_t i = 2; i < n && ordered; i++) ordered = p[i - 2] < p[i];
-    if (ordered && (p[n - 2] < p[1] || p[n - 1] < p[0])) return false;
-    std::sort(p, p + n);
-    return std::adjacent_find(p, p + n) != p + n;
-}
-
 }  // namespace sf37kv
 
 using namespace sf37kv;
@@ -226,48 +216,51 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
         if ((uint64_t)(L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap) * kv_heads > kMaxUnits)
             return set_error(SF37KV_EINVAL, "append_i8: layer %u has too many rows for one call", i);
     }
-    // Pass 0 forms the launches and checks them, pass 1 runs them.
-    for (int pass = 0; pass < 2; pass++) {
-        for (uint32_t base = 0; base < n_layers;) {
-            AppendI8Params P;
-            P.n_jobs = 0;
-            P.heads = kv_heads;
-            const bool bf16 = row_type == SF37KV_Q_BF16;
-            P.rows_each = 0;
-            uint64_t rows = 0;
-            uint32_t i = base;
-            const void *seen[2 * kMaxJobs];
-            for (; i < n_layers && P.n_jobs < (uint32_t)kMaxJobs; i++) {
-                const sf37kv_append_i8_layer &L = layers[i];
-                if (L.n_tok == 0) continue;
-                // With n_tok > cap only the last cap rows stay, as in a sequential append.
-                const uint32_t keep = L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap, skip = L.n_tok - keep;
-                if ((rows + keep) * kv_heads > kMaxUnits) break;
-                const uint64_t off = (uint64_t)skip * kv_heads * 128u * (bf16 ? 2u : 4u);
-                P.job[P.n_jobs] = AppendI8Job{(uint8_t *)L.cache.k_cache, (uint8_t *)L.cache.v_cache,
-                                              (const char *)L.k + off, (const char *)L.v + off, L.pos0 + skip,
-                                              L.cache.cap};
-                seen[2 * P.n_jobs] = L.cache.k_cache;
-                seen[2 * P.n_jobs + 1] = L.cache.v_cache;
-                P.rows_each = P.n_jobs == 0 || P.rows_each == keep ? keep : 0u;
-                P.row_begin[P.n_jobs++] = (uint32_t)rows;
-                rows += keep;
+    try {
+        std::vector<Span> spans;
+        spans.reserve((size_t)n_layers * 2);
+        for (int which = 0; which < 2; which++)
+            for (uint32_t i = 0; i < n_layers; i++) {
+                const sf37kv_cache &c = layers[i].cache;
+                if (layers[i].n_tok)
+                    spans.push_back(span_of(which ? c.v_cache : c.k_cache, (uint64_t)c.cap * kv_heads * 132u, true));
             }
-            base = i;
-            if (P.n_jobs == 0) continue;
-            if (pass == 0) {
-                if (any_twice(seen, 2 * P.n_jobs))
-                    return set_error(SF37KV_EINVAL, "append_i8: one cache is written twice in one call");
-                continue;
-            }
-            P.row_begin[P.n_jobs] = (uint32_t)rows;
-            const unsigned grid = (unsigned)((rows * kv_heads + kAppendThreads / 8u - 1u) / (kAppendThreads / 8u));
-            g_launches++;
-            if (int rc = launch_early("append_i8 launch", bf16 ? append_i8_kernel<true> : append_i8_kernel<false>, grid,
-                                      kAppendThreads, 0,
-                                      s, P))
-                return rc;
+        if (spans_conflict(spans))
+            return set_error(SF37KV_EINVAL, "append_i8: one cache is written twice in one call, or overlaps another");
+    } catch (const std::bad_alloc &) {
+        return set_error(SF37KV_ENOMEM, "append_i8: no memory to compare %u layers", n_layers);
+    }
+    for (uint32_t base = 0; base < n_layers;) {
+        AppendI8Params P;
+        P.n_jobs = 0;
+        P.heads = kv_heads;
+        const bool bf16 = row_type == SF37KV_Q_BF16;
+        P.rows_each = 0;
+        uint64_t rows = 0;
+        uint32_t i = base;
+        for (; i < n_layers && P.n_jobs < (uint32_t)kMaxJobs; i++) {
+            const sf37kv_append_i8_layer &L = layers[i];
+            if (L.n_tok == 0) continue;
+            // With n_tok > cap only the last cap rows stay, as in a sequential append.
+            const uint32_t keep = L.n_tok < L.cache.cap ? L.n_tok : L.cache.cap, skip = L.n_tok - keep;
+            if ((rows + keep) * kv_heads > kMaxUnits) break;
+            const uint64_t off = (uint64_t)skip * kv_heads * 128u * (bf16 ? 2u : 4u);
+            P.job[P.n_jobs] = AppendI8Job{(uint8_t *)L.cache.k_cache, (uint8_t *)L.cache.v_cache,
+                                          (const char *)L.k + off, (const char *)L.v + off, L.pos0 + skip,
+                                          L.cache.cap};
+            P.rows_each = P.n_jobs == 0 || P.rows_each == keep ? keep : 0u;
+            P.row_begin[P.n_jobs++] = (uint32_t)rows;
+            rows += keep;
         }
+        base = i;
+        if (P.n_jobs == 0) continue;
+        P.row_begin[P.n_jobs] = (uint32_t)rows;
+        const unsigned grid = (unsigned)((rows * kv_heads + kAppendThreads / 8u - 1u) / (kAppendThreads / 8u));
+        g_launches++;
+        if (int rc = launch_early("append_i8 launch", bf16 ? append_i8_kernel<true> : append_i8_kernel<false>, grid,
+                                  kAppendThreads, 0,
+                                  s, P))
+            return rc;
     }
     return SF37KV_OK;
 }

@@ -59,3 +59,22 @@ def test_read_refuses_k_and_v_that_overlap():
     d = _read(1)
     d["dst_v_cache"] = d["dst_k_cache"] + 2 * ROW
     _refused(_read_call(d), "another")
+
+
+# ------------------------------------------------------------ append
+def _append(n):
+    d = np.zeros(n, _lib.APPEND_I8_LAYER)
+    i = np.arange(n, dtype=np.uint64)
+    d["k_cache"], d["v_cache"] = P * (2 * i + 1), P * (2 * i + 2)
+    d["cap"], d["n_tok"], d["k"], d["v"] = 16, 4, P, P
+    return d
+
+
+@pytest.mark.parametrize("n,a,b", [(2, 0, 1), (65, 0, 64), (200, 3, 199)])
+def test_append_refuses_one_cache_twice(n, a, b):
+    for x, y in (("k_cache", "k_cache"), ("v_cache", "v_cache"), ("k_cache", "v_cache")):
+        d = _append(n)
+        d[x][b] = d[y][a]
+        _refused(_lib.lib().sf37kv_append_i8(d.ctypes.data, n, 8, 128, 0, None), "twice")
+        d[x][b] += 16 * 8 * 132 - 32  # the last scales
+        _refused(_lib.lib().sf37kv_append_i8(d.ctypes.data, n, 8, 128, 0, None), "twice")
