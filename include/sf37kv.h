@@ -241,7 +241,7 @@ typedef struct {
  * and each query attends to its cache's rows.  A query enters as integers, off
  * by at most 2^-22 of the power of two at its head's largest element.  head_dim
  * 128, q_heads/kv_heads <= 16 and any number of sequences.  A cache that one sequence appends to
- * may not be another's in the same call.
+ * may not be, or overlap, another's in the same call.
  * workspace: device memory of sf37kv_decode_i8_workspace() bytes, 256-byte
  * aligned, zero-filled once before its first use (sf37kv_dev_alloc does) and
  * left reusable by every call.  Calls that may overlap on the GPU (other

@@ -1052,28 +1052,21 @@ static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, u
     return SF37KV_OK;
 }
 
-// A cache that is appended to and given twice, among n sequences.
-static bool append_conflict(const sf37kv_decode_seq *const *seqs, uint32_t n) {
-    struct Item {
-        const void *p;
-        bool writes;
-    } items[2 * kMaxSeqs];
+// Whether a cache that one sequence of a call appends to overlaps another one's.
+static bool append_conflict(const sf37kv_shared_group *groups, uint32_t n_groups, uint64_t total, uint64_t row) {
     bool any = false;
-    for (uint32_t i = 0; i < n; i++) {
-        const bool w = seqs[i]->k_new != nullptr;
-        any |= w;
-        items[2 * i] = Item{seqs[i]->cache.k_cache, w};
-        items[2 * i + 1] = Item{seqs[i]->cache.v_cache, w};
-    }
+    for (uint32_t i = 0; i < n_groups; i++)
+        for (uint32_t k = 0; k < groups[i].n_seqs; k++) any |= groups[i].seqs[k].k_new != nullptr;
     if (!any) return false;
-    // Caches in one allocation, as a rule: in order, K apart from V.
-    bool ordered = true;
-    for (uint32_t i = 2; i < 2 * n && ordered; i++) ordered = items[i - 2].p < items[i].p;
-    if (ordered && (items[2 * n - 2].p < items[1].p || items[2 * n - 1].p < items[0].p)) return false;
-    std::sort(items, items + 2 * n, [](const Item &a, const Item &b) { return a.p != b.p ? a.p < b.p : a.writes > b.writes; });
-    for (uint32_t i = 1; i < 2 * n; i++)
-        if (items[i].p == items[i - 1].p && items[i - 1].writes) return true;
-    return false;
+    std::vector<Span> spans;
+    spans.reserve((size_t)total * 2u);
+    for (int which = 0; which < 2; which++)
+        for (uint32_t i = 0; i < n_groups; i++)
+            for (uint32_t k = 0; k < groups[i].n_seqs; k++) {
+                const sf37kv_decode_seq &L = groups[i].seqs[k];
+                spans.push_back(span_of(which ? L.cache.v_cache : L.cache.k_cache, L.cache.cap * row, L.k_new != nullptr));
+            }
+    return spans_conflict(spans);
 }
 
 // Decode of all groups; ring_clamp (sf37kv_decode_i8): no prefixes, and a full cache's
@@ -1107,6 +1100,12 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
         total += Gr.n_seqs;
     }
     if (total == 0) return SF37KV_OK;
+    try {
+        if (append_conflict(groups, n_groups, total, (uint64_t)kv_heads * (dtype == SF37KV_I8 ? 132u : 256u)))
+            return set_error(SF37KV_EINVAL, "%s: a cache that one sequence appends to is given twice, or overlaps another", what);
+    } catch (const std::bad_alloc &) {
+        return set_error(SF37KV_ENOMEM, "%s: no memory to compare %llu sequences", what, (unsigned long long)total);
+    }
     const Layout W = layout(n_groups, total, q_heads, kv_heads, !ring_clamp);
     if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < W.bytes)
         return set_error(SF37KV_EINVAL, "%s: the workspace must be 256-byte aligned and hold %llu bytes", what,
@@ -1122,73 +1121,63 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
     head.pre_part = (const float *)(ws + W.pre);
     head.pre_ml = (const float *)(ws + W.ml);
     const uint32_t most = seqs_per_launch(kv_heads), T = prefix_seqs_per_tile(head.group);
-    // Pass 0 forms the launches and checks them, pass 1 runs them.
-    for (int pass = 0; pass < 2; pass++) {
-        uint32_t gi = 0, k0 = 0;  // next group, and its next sequence
-        while (gi < n_groups) {
-            PrefixGroup pg[kPrefixGroups];
-            PrefixSeq ps[kMaxSeqs];
-            SeqDev sd[kMaxSeqs];
-            const sf37kv_decode_seq *src[kMaxSeqs];
-            uint32_t owner[kMaxSeqs];  // the sequence's prefix group, or n_pg
-            uint32_t n = 0, n_pg = 0;
-            while (gi < n_groups && n < most && n_pg < (uint32_t)kPrefixGroups) {
-                const sf37kv_shared_group &Gr = groups[gi];
-                const uint32_t take = std::min(Gr.n_seqs - k0, most - n);
-                PrefixGroup &X = pg[n_pg];
-                X = PrefixGroup{Gr.prefix.k_cache, Gr.prefix.v_cache, Gr.prefix_len, Gr.prefix_len, Gr.prefix.cap, n, take};
-                for (uint32_t k = 0; k < take; k++, n++) {
-                    const sf37kv_decode_seq &L = Gr.seqs[k0 + k];
-                    const uint32_t have = L.pos + 1u;
-                    uint32_t first = L.cache.sliding && have > L.cache.window ? have - L.cache.window : 0u;
-                    if (ring_clamp) first = start_at(L.pos, L.cache.cap, (int)L.cache.sliding, L.cache.window);
-                    ps[n] = PrefixSeq{L.q, std::min(first, Gr.prefix_len), 0};
-                    X.lo = std::min(X.lo, ps[n].start);
-                    SeqDev &J = sd[n];
-                    J = SeqDev{L.cache.k_cache, L.cache.v_cache, L.q, L.gate, L.out, L.k_new, L.v_new};
-                    J.start = std::min(std::max(first, Gr.prefix_len), have);
-                    J.end = have;
-                    J.cap = L.cache.cap;
-                    src[n] = &L;
-                    owner[n] = n_pg;
-                }
-                if (X.lo < X.len) n_pg++;
-                else for (uint32_t k = n - take; k < n; k++) owner[k] = UINT32_MAX;
-                k0 += take;
-                if (k0 == Gr.n_seqs) {
-                    gi++;
-                    k0 = 0;
-                }
+    uint32_t gi = 0, k0 = 0;  // next group, and its next sequence
+    while (gi < n_groups) {
+        PrefixGroup pg[kPrefixGroups];
+        PrefixSeq ps[kMaxSeqs];
+        SeqDev sd[kMaxSeqs];
+        uint32_t owner[kMaxSeqs];  // the sequence's prefix group, or n_pg
+        uint32_t n = 0, n_pg = 0;
+        while (gi < n_groups && n < most && n_pg < (uint32_t)kPrefixGroups) {
+            const sf37kv_shared_group &Gr = groups[gi];
+            const uint32_t take = std::min(Gr.n_seqs - k0, most - n);
+            PrefixGroup &X = pg[n_pg];
+            X = PrefixGroup{Gr.prefix.k_cache, Gr.prefix.v_cache, Gr.prefix_len, Gr.prefix_len, Gr.prefix.cap, n, take};
+            for (uint32_t k = 0; k < take; k++, n++) {
+                const sf37kv_decode_seq &L = Gr.seqs[k0 + k];
+                const uint32_t have = L.pos + 1u;
+                uint32_t first = L.cache.sliding && have > L.cache.window ? have - L.cache.window : 0u;
+                if (ring_clamp) first = start_at(L.pos, L.cache.cap, (int)L.cache.sliding, L.cache.window);
+                ps[n] = PrefixSeq{L.q, std::min(first, Gr.prefix_len), 0};
+                X.lo = std::min(X.lo, ps[n].start);
+                SeqDev &J = sd[n];
+                J = SeqDev{L.cache.k_cache, L.cache.v_cache, L.q, L.gate, L.out, L.k_new, L.v_new};
+                J.start = std::min(std::max(first, Gr.prefix_len), have);
+                J.end = have;
+                J.cap = L.cache.cap;
+                owner[n] = n_pg;
             }
-            if (n == 0) continue;
-            if (pass == 0) {
-                if (append_conflict(src, n))
-                    return set_error(SF37KV_EINVAL, "%s: a cache that one sequence appends to is given twice", what);
-                continue;
+            if (X.lo < X.len) n_pg++;
+            else for (uint32_t k = n - take; k < n; k++) owner[k] = UINT32_MAX;
+            k0 += take;
+            if (k0 == Gr.n_seqs) {
+                gi++;
+                k0 = 0;
             }
-            uint64_t own = 0;  // rows
-            for (uint32_t k = 0; k < n; k++) own += sd[k].end - sd[k].start;
-            const uint32_t prefix_ctas =
-                n_pg ? prefix_plan(pg, n_pg, q_heads, kv_heads, !head.bf16, own, dtype == SF37KV_I8) : 0;
-            for (uint32_t k = 0; k < n; k++) {
-                SeqDev &J = sd[k];
-                J.pre_tile = J.pre_kvh = J.pre_splits = J.pre_row = 0;
-                if (owner[k] == UINT32_MAX || ps[k].start >= pg[owner[k]].len) continue;
-                const PrefixGroup &X = pg[owner[k]];
-                const uint32_t i = k - X.seq0;
-                J.pre_tile = X.part0 + i / T * X.splits;
-                J.pre_kvh = X.m_tiles * X.splits;
-                J.pre_splits = X.splits;
-                J.pre_row = i % T * head.group;
-            }
-            if (n_pg)
-                if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
-                                              (float *)(ws + W.ml), head.sync, stream))
-                    return rc;
-            const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, prefix_ctas, stream)
-                                              : launch_mode<false>(sd, n, head, prefix_ctas, stream);
-            if (rc) return rc;
         }
+        if (n == 0) continue;
+        uint64_t own = 0;  // rows
+        for (uint32_t k = 0; k < n; k++) own += sd[k].end - sd[k].start;
+        const uint32_t prefix_ctas =
+            n_pg ? prefix_plan(pg, n_pg, q_heads, kv_heads, !head.bf16, own, dtype == SF37KV_I8) : 0;
+        for (uint32_t k = 0; k < n; k++) {
+            SeqDev &J = sd[k];
+            J.pre_tile = J.pre_kvh = J.pre_splits = J.pre_row = 0;
+            if (owner[k] == UINT32_MAX || ps[k].start >= pg[owner[k]].len) continue;
+            const PrefixGroup &X = pg[owner[k]];
+            const uint32_t i = k - X.seq0;
+            J.pre_tile = X.part0 + i / T * X.splits;
+            J.pre_kvh = X.m_tiles * X.splits;
+            J.pre_splits = X.splits;
+            J.pre_row = i % T * head.group;
+        }
+        if (n_pg)
+            if (int rc = prefix_attention(pg, n_pg, ps, n, q_heads, kv_heads, !head.bf16, (float *)(ws + W.pre),
+                                          (float *)(ws + W.ml), head.sync, stream))
+                return rc;
+        const int rc = dtype == SF37KV_I8 ? launch_mode<true>(sd, n, head, prefix_ctas, stream)
+                                          : launch_mode<false>(sd, n, head, prefix_ctas, stream);
+        if (rc) return rc;
     }
     return SF37KV_OK;
 }

@@ -78,3 +78,44 @@ def test_append_refuses_one_cache_twice(n, a, b):
         _refused(_lib.lib().sf37kv_append_i8(d.ctypes.data, n, 8, 128, 0, None), "twice")
         d[x][b] += 16 * 8 * 132 - 32  # the last scales
         _refused(_lib.lib().sf37kv_append_i8(d.ctypes.data, n, 8, 128, 0, None), "twice")
+
+
+# ------------------------------------------------------------ decode
+def _seqs(n):
+    d = np.zeros(n, _lib.DECODE_SEQ)
+    i = np.arange(n, dtype=np.uint64)
+    d["k_cache"], d["v_cache"] = P * (2 * i + 1), P * (2 * i + 2)
+    d["cap"], d["pos"], d["q"], d["out"] = 64, 20, P, P
+    return d
+
+
+def _decode(d):
+    return _lib.lib().sf37kv_decode_i8(d.ctypes.data, len(d), 64, 8, 128, 0, P, 1 << 40, None)
+
+
+def _shared(arrays, prefix_len=0, dtype=2):
+    g = np.zeros(len(arrays), _lib.SHARED_GROUP)
+    for i, d in enumerate(arrays):
+        g[i] = (P * (10001 + 2 * i), P * (10002 + 2 * i), 32, 0, 0, 0, prefix_len, len(d), d.ctypes.data)
+    return _lib.lib().sf37kv_decode_shared(g.ctypes.data, len(g), 64, 8, 128, dtype, 0, P, 1 << 40, None)
+
+
+@pytest.mark.parametrize("n,a,b", [(2, 0, 1), (2, 1, 0), (257, 0, 256), (600, 599, 1)])
+def test_decode_refuses_an_appended_cache_that_is_anothers(n, a, b):
+    for x, y in (("k_cache", "k_cache"), ("v_cache", "v_cache"), ("k_cache", "v_cache")):
+        for off in (0, 63 * 8 * 128 - 32):  # the same cache, or one that begins in its last codes
+            d = _seqs(n)
+            d["k_new"][a] = d["v_new"][a] = P
+            d[x][b] = d[y][a] + off
+            _refused(_decode(d), "twice")
+            _refused(_shared([d]), "twice")
+            _refused(_shared([d], dtype=1), "twice")
+
+
+def test_shared_refuses_an_appended_cache_of_another_groups_sequence():
+    one, two = _seqs(300), _seqs(300)
+    for c in ("k_cache", "v_cache"):
+        two[c] += 5000 * P
+    one["k_new"][0] = one["v_new"][0] = P
+    two["v_cache"][299] = one["v_cache"][0]
+    _refused(_shared([one, two]), "twice")
