@@ -1052,20 +1052,26 @@ static int check_seq(const char *what, uint32_t i, const sf37kv_decode_seq &L, u
     return SF37KV_OK;
 }
 
-// Whether a cache that one sequence of a call appends to overlaps another one's.
-static bool append_conflict(const sf37kv_shared_group *groups, uint32_t n_groups, uint64_t total, uint64_t row) {
+// Whether a cache that one sequence of a call appends to overlaps another one's (rows of
+// `row` bytes), or any group's prefix, which is read beside the appends.
+static bool append_conflict(const sf37kv_shared_group *groups, uint32_t n_groups, uint64_t total, uint64_t row,
+                            uint64_t prefix_row) {
     bool any = false;
     for (uint32_t i = 0; i < n_groups; i++)
         for (uint32_t k = 0; k < groups[i].n_seqs; k++) any |= groups[i].seqs[k].k_new != nullptr;
     if (!any) return false;
     std::vector<Span> spans;
-    spans.reserve((size_t)total * 2u);
+    spans.reserve((size_t)(total + n_groups) * 2u);
     for (int which = 0; which < 2; which++)
-        for (uint32_t i = 0; i < n_groups; i++)
+        for (uint32_t i = 0; i < n_groups; i++) {
+            const sf37kv_cache &prefix = groups[i].prefix;
+            if (groups[i].n_seqs && groups[i].prefix_len)
+                spans.push_back(span_of(which ? prefix.v_cache : prefix.k_cache, groups[i].prefix_len * prefix_row, false));
             for (uint32_t k = 0; k < groups[i].n_seqs; k++) {
                 const sf37kv_decode_seq &L = groups[i].seqs[k];
                 spans.push_back(span_of(which ? L.cache.v_cache : L.cache.k_cache, L.cache.cap * row, L.k_new != nullptr));
             }
+        }
     return spans_conflict(spans);
 }
 
@@ -1101,8 +1107,10 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
     }
     if (total == 0) return SF37KV_OK;
     try {
-        if (append_conflict(groups, n_groups, total, (uint64_t)kv_heads * (dtype == SF37KV_I8 ? 132u : 256u)))
-            return set_error(SF37KV_EINVAL, "%s: a cache that one sequence appends to is given twice, or overlaps another", what);
+        if (append_conflict(groups, n_groups, total, (uint64_t)kv_heads * (dtype == SF37KV_I8 ? 132u : 256u), kv_heads * 256ull))
+            return set_error(SF37KV_EINVAL,
+                             "%s: a cache that one sequence appends to is given twice, or overlaps another or a group's prefix",
+                             what);
     } catch (const std::bad_alloc &) {
         return set_error(SF37KV_ENOMEM, "%s: no memory to compare %llu sequences", what, (unsigned long long)total);
     }

@@ -119,3 +119,18 @@ def test_shared_refuses_an_appended_cache_of_another_groups_sequence():
     one["k_new"][0] = one["v_new"][0] = P
     two["v_cache"][299] = one["v_cache"][0]
     _refused(_shared([one, two]), "twice")
+
+
+@pytest.mark.parametrize("dtype,row", [(1, 132), (2, 256)])
+def test_shared_refuses_an_append_to_another_groups_prefix(dtype, row):
+    one, two = _seqs(3), _seqs(3)
+    for c in ("k_cache", "v_cache"):
+        two[c] += 5000 * P
+    one["k_new"][2] = one["v_new"][2] = P
+    for c in ("k_cache", "v_cache"):
+        for prefix in (P * 10003, P * 10004):  # K and V of the second group's prefix of 8 rows
+            keep = one[c][2]
+            for at in (prefix, prefix + 7 * 8 * 256, prefix - 64 * 8 * row + 32):
+                one[c][2] = at
+                _refused(_shared([one, two], 8, dtype), "prefix")
+            one[c][2] = keep
