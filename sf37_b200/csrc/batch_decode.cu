@@ -173,8 +173,10 @@ __device__ __forceinline__ void fold(float4 &a, float &l, const float4 &x, float
     a.w = fmaf(x.w, w, a.w);
     l = fmaf(lx, w, l);
 }
-__device__ __forceinline__ float4 normalise(float4 a, float l, float g) {
-    if (l == 0.f) return make_float4(0.f, 0.f, 0.f, 0.f);  // no row attended to
+// Of a head with the sum l of its weights; a sequence without rows gets zeros, one
+// whose scores are all -inf NaN (0 / 0).
+__device__ __forceinline__ float4 normalise(float4 a, float l, float g, bool no_rows) {
+    if (no_rows) return make_float4(0.f, 0.f, 0.f, 0.f);
     return make_float4(a.x / l * g, a.y / l * g, a.z / l * g, a.w / l * g);
 }
 
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
             const float2 ml = MLs[s * 16 + h];
             fold(a, L, *reinterpret_cast<const float4 *>(Os + os_at(s * 16u + h, d4)), ml.y, fast_exp2(ml.x - M));
         }
-        if (single) store_out4(J.out, out0 + idx * 4u, normalise(a, L, gate_s[h]), P.bf16);
+        if (single) store_out4(J.out, out0 + idx * 4u, normalise(a, L, gate_s[h], J.start == J.end), P.bf16);
         else __stcg(reinterpret_cast<float4 *>(part + idx * 4u), a);
         if (!single && (idx & 31u) == 0) __stcg(reinterpret_cast<float2 *>(part + G * 128u + 2u * h), make_float2(M, L));
     }
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         const uint32_t h = idx >> 5;
         const Joined x = join_one(own, (uint64_t)P.kv_heads * stride, J.n_splits, P.pre_part, P.pre_ml, row_pre, J.pre_splits, G,
                                   h, idx);
-        store_out4(J.out, out0 + idx * 4u, normalise(x.o, x.l, gate_s[h]), P.bf16);
+        store_out4(J.out, out0 + idx * 4u, normalise(x.o, x.l, gate_s[h], false), P.bf16);
     }
 }
 
@@ -846,7 +848,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Batch
         const float gate = J.gate ? J.gate[kvh * G + h] : 0.f;
         const Joined x = join_one(own, (uint64_t)P.kv_heads * stride, J.n_splits, P.pre_part, P.pre_ml, row_pre, J.pre_splits, G,
                                   h, idx);
-        store_out4(J.out, (uint64_t)kvh * G * 128u + idx * 4u, normalise(x.o, x.l, J.gate ? sigmoid_dev(gate) : 1.f), P.bf16);
+        store_out4(J.out, (uint64_t)kvh * G * 128u + idx * 4u, normalise(x.o, x.l, J.gate ? sigmoid_dev(gate) : 1.f, false),
+                   P.bf16);
     }
 }
 
