@@ -53,7 +53,7 @@ extern unsigned long long g_launches;
 enum { kPair = 0, kHalf = 1, kWide = 2, kTwo = 3 };
 
 constexpr float kSlack = 8.0f;
-constexpr float kNone = -1e30f;  // reference of a state without rows
+constexpr float kNone = -3.402823466e38f;  // reference of a state without rows: no finite score is below it
 // The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each block
 // (measured), 9e-6 over 512 of them.  f32 outputs take O into sums of their own
 // after this many.

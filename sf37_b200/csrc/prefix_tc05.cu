@@ -60,7 +60,10 @@ struct PrefixParams {
 };
 
 constexpr float kHead = 7.0f, kRaise = 15.0f;
-constexpr float kNone = -1e30f;  // reference of a row without keys
+// x * qs - m as one fma keeps the product's last bits, which m's rounding lacks: 0.125 at
+// references up to this, beyond which product and difference are rounded one by one.
+constexpr float kFused = 2097152.0f;
+constexpr float kNone = -3.402823466e38f;  // reference of a row without keys: no finite score is below it
 // The tensor core truncates its f32 sums: O loses 1.7e-8 of itself with each MMA (measured).
 // F32 takes O into sums in memory after this many key tiles of a stream (256 MMAs,
 // 4e-6; 16000 keys, 40 sequences: 99 us with half as many, 85 with none).
@@ -138,6 +141,12 @@ __device__ __forceinline__ void load_q(const PrefixSeq *tab, uint32_t n_seqs, ui
         }
     }
     fence_async_smem();
+}
+
+// The weight of a raw score x under the reference m.
+template <bool FUSED>
+__device__ __forceinline__ float weight(float x, float qs, float m) {
+    return fast_exp2(FUSED ? fmaf(x, qs, -m) : __fsub_rn(__fmul_rn(x, qs), m));
 }
 
 // Whether any thread of two warps (named barrier `id`), or of all softmax warps, says so.
@@ -420,7 +429,7 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
                     uint32_t w[16], wl[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
+                        const float p0 = weight<false>(x[2 * i], qs, m), p1 = weight<false>(x[2 * i + 1], qs, m);
                         la += p0;
                         lb += p1;
                         w[i] = pack_h2(p0, p1);
@@ -443,13 +452,14 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
                 weigh(3, v[1]);
             } else {
                 // Columns 64 * half on.  The weights are taken with the reference of the tiles
-                // before, which holds as a rule; where a row's does not, both threads of
-                // every row of the warp pair begin again (P is not written yet).
+                // before, which holds as a rule; where a row's does not, or is beyond kFused, both
+                // threads of every row of the warp pair begin again (P is not written yet).
                 uint32_t w[32];
-                auto weigh = [&](int c, const float (&x)[32]) {
+                auto weigh = [&](auto fused, int c, const float (&x)[32]) {
+                    constexpr bool kF = decltype(fused)::value;
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const float p0 = fast_exp2(fmaf(x[2 * i], qs, -m)), p1 = fast_exp2(fmaf(x[2 * i + 1], qs, -m));
+                        const float p0 = weight<kF>(x[2 * i], qs, m), p1 = weight<kF>(x[2 * i + 1], qs, m);
                         la += p0;
                         lb += p1;
                         w[16 * c + i] = pack_h2(p0, p1);
@@ -465,12 +475,12 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
                     tmem_ld32(t_h + 32u, u);
                     mask(2 * half, v);
                     top = top_of(v);
-                    weigh(0, v);
+                    weigh(std::true_type(), 0, v);
                     tmem_wait_ld();
                     mask(2 * half + 1, u);
                     top = fmaxf(top, top_of(u)) * qs;
-                    weigh(1, u);
-                    raise = top - m > kRaise;
+                    weigh(std::true_type(), 1, u);
+                    raise = top - m > kRaise || (fabsf(m) > kFused && m != kNone);
                 }
                 const uint32_t pair = 1u + st * 4u + (warp & 3u);
                 fence_before();
@@ -504,7 +514,7 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
                         tmem_ld32(t_h + c * 32u, v);
                         tmem_wait_ld();
                         mask(2 * half + c, v);
-                        weigh(c, v);
+                        weigh(std::false_type(), c, v);
                     }
                     fence_before();
                     pair_any(pair, false);

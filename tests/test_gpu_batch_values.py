@@ -43,3 +43,36 @@ def test_rows_that_all_score_minus_infinity(group, dtype):
     assert torch.isnan(out[0, 3]).all()
     out[0, 3] = 0
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", IO)
+@pytest.mark.parametrize("group", [8, 12])
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+@pytest.mark.parametrize("power", [22, 60, 102])
+def test_scores_of_any_size(power, cache, group, dtype):
+    # scores of -1e7 to -1e9, and up to -1e31 to -1e33: the largest one takes all the weight.  Rows are multiples of one row (powers of two, exact
+    # in f16 and in int8 scales), so the attended row with the smallest multiple wins by far more than any rounding.
+    heads, cap, n = 2, 5, 2
+    size = torch.tensor([8.0, 4.0, 1.0, 2.0, 16.0], device="cuda").view(1, cap, 1, 1)
+    base = torch.full((n, 1, heads, D), -0.25, device="cuda")
+    k, v = base * size, rows(2, n, cap, heads)
+    q = (rows(3, n, heads * group).abs() + 1) * 2.0 ** power
+    q = q.to(dtype)
+    prefix = (base[0] * 64).half().expand(3, heads, D).contiguous(), rows(4, 3, heads).half()
+    if cache == "i8":
+        raw = i8_cache(n, cap, heads), i8_cache(n, cap, heads)
+        kv.append_i8(kv.append_i8_desc(raw[0], raw[1], cap, 0, k, v), heads, D, k.dtype)
+        own, v = (raw[0], raw[1], cap), values(raw[1], cap, heads)
+    else:
+        own, v = (k.half(), v.half()), v.half().double()
+    for got, best in ((_shared(prefix, own, [7, 7], q, heads, kv.I8 if cache == "i8" else kv.F16), v[:, 2]),
+                      (_shared(None, own, [1, 4], q, heads, kv.I8 if cache == "i8" else kv.F16), torch.stack([v[0, 1], v[1, 2]]))):
+        want = best.repeat_interleave(group, 1)
+        assert torch.isfinite(got).all()
+        # one weight of 1: the value, a product and a division (2^-21 each at most), and the output's rounding
+        assert ((got.double() - want).abs() <= want.abs() * (2.0 ** -20 + (2.0 ** -8 if dtype == torch.bfloat16 else 0))).all()
+    # over the prefix alone, equal scores: the mean of its rows
+    got = _shared(prefix, own, [2, 2], q, heads, kv.I8 if cache == "i8" else kv.F16)
+    want = prefix[1].double().mean(0).repeat_interleave(group, 0).expand(n, -1, -1)
+    mag = prefix[1].double().abs().mean(0).repeat_interleave(group, 0)
+    assert ((got.double() - want).abs() <= mag * 2.0 ** -18 + (want.abs() * 2.0 ** -8 if dtype == torch.bfloat16 else 0)).all()
