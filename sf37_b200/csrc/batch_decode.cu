@@ -61,8 +61,8 @@ constexpr uint32_t kTake = 32;
 constexpr uint64_t kCounters = 16384;  // u32 counters at the start of a workspace
 constexpr uint32_t kSmallSeqs = 16, kSomeSeqs = 64, kMaxSeqs = 256;  // sequences per launch
 constexpr uint32_t kMapped = 1024;     // slots with a direct map to their sequence
-// Range of the weights' power of two (kernel below): the ratio of two is finite.
-constexpr int kFMin = -86, kFMax = 40;
+// Range of the weights' power of two (kernel below): value scales from 2^-113 to 2^121, the largest.
+constexpr int kFMin = -114, kFMax = 120;
 
 struct SeqDev {
     const void *k, *v, *q;
@@ -504,8 +504,9 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
         for (int i = 0; i < 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     // Per head: reference m, sum l, and f, a power of two that brings the
     // weights p * (value scale) into f16's range: the largest is kept in
-    // [2^7, 2^15], so weights down to 2^-32 of it are held (value scales from
-    // 2^-40 to 2^100; smaller ones lose bits, larger ones overflow).
+    // [2^7, 2^15], so weights down to 2^-32 of it are held.  When m rises, f does at most
+    // by what the weights so far lose (8 bits or more, rounded up to a whole one), so O
+    // gains less than a bit for each 8 of f's 234, and its largest weights stay in range.
     float m[NH], l[NH], f[NH];
 #pragma unroll
     for (int h = 0; h < NH; h++) {
@@ -645,7 +646,7 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                     const float x = sc[h][i][e] - m[h];
                     xm = fmaxf(xm, x);
                     p[h][i][e] = fast_exp2(x);
-                    w[h][i][e] = I8 ? p[h][i][e] * (vs[i][e] * f[h]) : p[h][i][e] * f[h];
+                    w[h][i][e] = I8 ? p[h][i][e] * vs[i][e] * f[h] : p[h][i][e] * f[h];  // (vs * f may overflow where p is 0)
                     wm = fmaxf(wm, w[h][i][e]);
                 }
             need[h] = xm > kSlack || (I8 && wm > 32768.f);
@@ -667,7 +668,8 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = nd ? fmaxf(m[h], mx) : m[h];
-                fac[h] = fast_exp2(m[h] - mn);
+                const float m_old = m[h];
+                fac[h] = fast_exp2(m_old - mn);
                 l[h] *= fac[h];
                 m[h] = mn;
                 if (I8) {
@@ -678,11 +680,13 @@ __global__ void __launch_bounds__(Shape<MODE, I8, WIDE>::kThreads, Shape<MODE, I
                         for (int e = 0; e < 2; e++) top = fmaxf(top, fast_exp2(sc[h][i][e] - mn) * vs[i][e]);
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    int e2;
-                    pow2_below(top, e2);
-                    const float fn = nd ? pow2(max(kFMin, min(kFMax, 7 - e2))) : f[h];
-                    fac[h] *= fn / f[h];
-                    f[h] = fn;
+                    int top_e, f_e;
+                    pow2_below(top, top_e);
+                    pow2_below(f[h], f_e);
+                    const int grow = (int)ceilf(fminf(mn - m_old, 256.f));  // powers of two that the weights so far lose
+                    const int fe = nd ? max(kFMin, min(min(kFMax, 7 - top_e), f_e + grow)) : f_e;
+                    fac[h] *= pow2(max(-126, min(126, fe - f_e)));
+                    f[h] = pow2(fe);
                 }
                 weigh(h);
             }

@@ -76,3 +76,51 @@ def test_scores_of_any_size(power, cache, group, dtype):
     want = prefix[1].double().mean(0).repeat_interleave(group, 0).expand(n, -1, -1)
     mag = prefix[1].double().abs().mean(0).repeat_interleave(group, 0)
     assert ((got.double() - want).abs() <= mag * 2.0 ** -18 + (want.abs() * 2.0 ** -8 if dtype == torch.bfloat16 else 0)).all()
+
+
+def _scaled_rows(heads, score, scale):
+    """An int8 cache whose row r scores score[r] (log2 units) against queries of ones, with values of size scale[r]."""
+    cap = len(score)
+    raw_k, raw_v = i8_cache(1, cap, heads, 0), fill_i8(1, cap, heads, 5)[0]
+    codes, scales = i8_views(raw_k, cap, heads)
+    codes[:] = 128
+    codes[..., 0] = 255  # c = 127 in one channel: q . K = 127 * scale
+    scales.copy_((torch.tensor(score, dtype=torch.float64) * math.sqrt(D) / math.log2(math.e) / 127).float().cuda().expand_as(scales))
+    i8_views(raw_v, cap, heads)[1].copy_(torch.tensor(scale, dtype=torch.float64).float().cuda().expand(1, heads, cap))
+    return raw_k, raw_v, cap
+
+
+@pytest.mark.parametrize("dtype", IO)
+@pytest.mark.parametrize("group", [8, 12])
+# rows whose scores rise as their values shrink, each worth as much as the others, and the reverse; a row that scores
+# little and is very large among very small ones; rows that score a little more and are very small after very large ones
+@pytest.mark.parametrize("case", ["falling", "rising", "rising by 115", "large one", "small last"])
+def test_values_of_any_size(case, group, dtype):
+    heads, n, cap = 8, 64, 768  # more pairs than run at once, so that a warp goes through many blocks
+    if case == "falling":
+        score, scale = [0.25 * x for x in range(cap)], [2.0 ** (119 - 0.25 * x) for x in range(cap)]
+    elif case == "rising":
+        score, scale = [0.25 * (cap - x) for x in range(cap)], [2.0 ** (-72 + 0.25 * x) for x in range(cap)]
+    elif case == "rising by 115":
+        score, scale = [0.15 * (cap - x) for x in range(cap)], [2.0 ** (4 + 0.15 * x) for x in range(cap)]
+    elif case == "small last":
+        score, scale = [0.0] * 500 + [9.0] * (cap - 500), [2.0 ** 100] * 500 + [2.0 ** -60] * (cap - 500)
+    else:
+        score, scale = [300.0] * cap, [2.0 ** -60] * cap
+        score[600], scale[600] = 0.0, 2.0 ** 119
+    raw_k, raw_v, cap = _scaled_rows(heads, score, scale)
+    kx, vx = values(raw_k, cap, heads)[0], values(raw_v, cap, heads)[0]
+    q = torch.ones(n, heads * group, D, device="cuda", dtype=dtype)
+    out = torch.full_like(q, float("nan"))
+    d = kv.decode_seqs_desc([raw_k[0]] * n, [raw_v[0]] * n, cap, cap - 1, q, out)
+    kv.decode_i8(d, heads * group, heads, D, dtype, workspace(kv.decode_i8_workspace(n, heads * group, heads)))
+    want, mag, reach = attend(q[0], kx, vx, None)
+    assert mag.min() > 1e-20  # far above bound()'s absolute part
+    tol = bound(want, mag, reach, cap, dtype, p_f16=group > 8 and dtype == torch.bfloat16)
+    if case == "rising":
+        # Rows that score more than 126 below the largest: their weight 2^(score - m) is below the smallest normal f32,
+        # 2^-126, for a reference m that reaches the largest score, and an f32 weight may be 0.  All that they add may be lost.
+        low = torch.tensor([x < score[0] - 126 for x in score], device="cuda")
+        tol = tol + attend(q[0], kx, vx.abs() * low.view(-1, 1, 1), None)[0]
+    check(out[0], want, tol)
+    assert all(torch.equal(x, out[0]) for x in out)
