@@ -239,9 +239,11 @@ typedef struct {
 
 /* sf37kv_decode() over I8 caches: the new rows are quantised into the caches
  * and each query attends to its cache's rows.  A query enters as integers, off
- * by at most 2^-22 of the power of two at its head's largest element.  head_dim
- * 128, q_heads/kv_heads <= 16 and any number of sequences.  A cache that one sequence appends to
- * may not be, or overlap, another's in the same call.
+ * by at most 2^-22 of the power of two at its head's largest element.  A query
+ * head or an attended row that is not finite makes the outputs that depend on it
+ * NaN or infinite, and no others.  head_dim 128, q_heads/kv_heads <= 16 and any
+ * number of sequences.  A cache that one sequence appends to may not be, or
+ * overlap, another's in the same call.
  * workspace: device memory of sf37kv_decode_i8_workspace() bytes, 256-byte
  * aligned, zero-filled once before its first use (sf37kv_dev_alloc does) and
  * left reusable by every call.  Calls that may overlap on the GPU (other

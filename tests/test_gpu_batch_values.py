@@ -124,3 +124,81 @@ def test_values_of_any_size(case, group, dtype):
         tol = tol + attend(q[0], kx, vx.abs() * low.view(-1, 1, 1), None)[0]
     check(out[0], want, tol)
     assert all(torch.equal(x, out[0]) for x in out)
+
+
+def _finite_elsewhere(got, clean, where):
+    """Not finite at `where`, a mask of outputs, and bit-equal to the call on finite inputs elsewhere."""
+    assert not torch.isfinite(got[where]).any()
+    assert torch.equal(got[~where], clean[~where])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", IO)
+@pytest.mark.parametrize("group", [8, 12])
+@pytest.mark.parametrize("cache", ["f16", "i8"])
+def test_queries_that_are_not_finite(cache, group, dtype, bad):
+    # one head of one sequence, beside others in its tiles
+    heads, n, cap, plen = 2, 5, 40, 300
+    prefix = rows(1, plen, heads).half(), rows(2, plen, heads).half()
+    if cache == "i8":
+        own = fill_i8(n, cap, heads, 3)[0], fill_i8(n, cap, heads, 4)[0], cap
+    else:
+        own = rows(3, n, cap, heads).half(), rows(4, n, cap, heads).half()
+    kind = kv.I8 if cache == "i8" else kv.F16
+    q = rows(5, n, heads * group, dtype=dtype)
+    pos = [plen + 7 * i for i in range(n)]
+    where = torch.zeros(n, heads * group, D, dtype=torch.bool, device="cuda")
+    where[2, 5] = True
+    broken = q.clone()
+    broken[2, 5, 77] = bad
+    _finite_elsewhere(_shared(prefix, own, pos, broken, heads, kind), _shared(prefix, own, pos, q, heads, kind), where)
+    pos = [7 * i for i in range(n)]
+    _finite_elsewhere(_shared(None, own, pos, broken, heads, kind), _shared(None, own, pos, q, heads, kind), where)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", IO)
+@pytest.mark.parametrize("group", [8, 12])
+def test_own_rows_that_are_not_finite(group, dtype, bad):
+    heads, n, cap, plen = 2, 5, 40, 300
+    prefix = rows(1, plen, heads).half(), rows(2, plen, heads).half()
+    k, v = rows(3, n, cap, heads).half(), rows(4, n, cap, heads).half()
+    q = rows(5, n, heads * group, dtype=dtype)
+    pos = [plen + 7 * i for i in range(n)]
+    clean = _shared(prefix, (k, v), pos, q, heads)
+    # rows that are not attended to: slots that the sequences have not reached
+    held = [[(plen + x) % cap for x in range(7 * i + 1)] for i in range(n)]
+    for i in range(n):
+        for slot in set(range(cap)) - set(held[i]):
+            k[i, slot], v[i, slot] = bad, bad
+    assert torch.equal(_shared(prefix, (k, v), pos, q, heads), clean)
+    # a key: every output of its KV head's queries (with a positive element, so that the score is not -inf)
+    where = torch.zeros(n, heads * group, D, dtype=torch.bool, device="cuda")
+    where[3, group:] = True
+    q[3, :, 50] = q[3, :, 50].abs() + 0.5
+    clean = _shared(prefix, (k, v), pos, q, heads)
+    keep = k[3, held[3][4], 1].clone()
+    k[3, held[3][4], 1, 50] = bad
+    _finite_elsewhere(_shared(prefix, (k, v), pos, q, heads), clean, where)
+    k[3, held[3][4], 1] = keep
+    # a value: its dimension only
+    where[:] = False
+    where[1, :group, 9] = True
+    v[1, held[1][2], 0, 9] = bad
+    _finite_elsewhere(_shared(prefix, (k, v), pos, q, heads), clean, where)
+
+
+@pytest.mark.parametrize("dtype", IO)
+def test_int8_rows_that_are_not_finite_beside_a_prefix(dtype):
+    heads, group, n, cap, plen = 2, 8, 5, 40, 300
+    prefix = rows(1, plen, heads).half(), rows(2, plen, heads).half()
+    raw_k, raw_v = fill_i8(n, cap, heads, 3)[0], fill_i8(n, cap, heads, 4)[0]
+    q = rows(5, n, heads * group, dtype=dtype)
+    pos = [plen + 7 * i for i in range(n)]
+    clean = _shared(prefix, (raw_k, raw_v, cap), pos, q, heads, kv.I8)
+    i8_views(raw_k, cap, heads)[1][4, 0, (plen + 30) % cap] = math.nan  # not reached
+    assert torch.equal(_shared(prefix, (raw_k, raw_v, cap), pos, q, heads, kv.I8), clean)
+    where = torch.zeros(n, heads * group, D, dtype=torch.bool, device="cuda")
+    where[3, group:] = True
+    i8_views(raw_v, cap, heads)[1][3, 1, (plen + 11) % cap] = math.nan
+    _finite_elsewhere(_shared(prefix, (raw_k, raw_v, cap), pos, q, heads, kv.I8), clean, where)
