@@ -262,9 +262,9 @@ int sf37kv_decode_i8(const sf37kv_decode_seq *seqs, uint32_t n_seqs, uint32_t q_
  * computed for all sequences of the group at once, on the tensor cores, and
  * joined with each one's own rows; a sliding window covers both.  An own cache
  * must still hold every own row of the window and may not be appended to when it
- * overlaps the prefix rows of any group of the call (else EINVAL), and prefix rows
- * that any sequence of the group attends to must be finite.  prefix_len may be 0.  An I8 prefix is read
- * back once with sf37kv_read_i8.
+ * overlaps the prefix rows of any group of the call (else EINVAL).  A prefix row
+ * that is not finite shows in the sequences that attend to it only.  prefix_len
+ * may be 0.  An I8 prefix is read back once with sf37kv_read_i8.
  * io_type F32 keeps queries and weights in two f16 parts (outputs are a few
  * 1e-6 off, by the tensor cores' truncating sums); BF16 rounds the weights to
  * f16, which its output's rounding covers.

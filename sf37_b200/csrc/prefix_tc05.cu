@@ -47,6 +47,7 @@ static __device__ int g_prefix_error;  // 1: a bounded wait gave up
 
 struct PrefixDev {
     CUtensorMap kmap, vmap;  // rows [0, len): later rows read as zeros
+    const __half *k, *v;
     uint32_t lo, len, seq0, n_seqs, m_tiles, splits, tps, part0, cta0, pairs;
 };
 template <int NS>
@@ -159,6 +160,62 @@ __device__ __forceinline__ bool bar_any(uint32_t id, uint32_t threads, bool x) {
 }
 __device__ __forceinline__ bool pair_any(uint32_t id, bool x) { return bar_any(id, 64, x); }
 __device__ __forceinline__ bool soft_any(uint32_t threads, bool x) { return bar_any(9, threads, x); }
+
+__device__ __forceinline__ bool all_finite(const float4 &x) {
+    return fmaf(x.x, 0.f, x.y * 0.f) + fmaf(x.z, 0.f, x.w * 0.f) == 0.f;
+}
+
+// One row of a partial tile again, by a warp: query head q [128] over the keys
+// [first, end) of K and V (`stride` elements a row).  PV multiplies every V row of a
+// tile by every weight, and 0 times a V that is not finite is NaN for sequences that do
+// not attend to it; so is q_hi K + q_lo K where K is infinite.  A row of O that is not
+// finite is therefore taken again by the formula, unless its query is the reason.
+__device__ __noinline__ void redo_row(const void *q, bool bf16, const __half *k, const __half *v, uint64_t stride,
+                                      uint32_t first, uint32_t end, float *o, float *ml) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const float4 x = load_row4(q, lane * 4u, bf16);
+    if (__any_sync(0xffffffffu, !all_finite(x))) return;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = kNone, l = 0.f;
+    auto row4 = [&](const __half *base, uint32_t r) {
+        const uint2 w = *reinterpret_cast<const uint2 *>(base + r * stride + lane * 4u);
+        const float2 lo = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)),
+                     hi = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+    };
+    for (uint32_t r = first; r < end; r += 4u) {
+        float s[4];
+        float4 y[4];
+        float mn = m;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t at = min(r + i, end - 1u);
+            const float4 z = row4(k, at);
+            y[i] = row4(v, at);
+            s[i] = fmaf(x.x, z.x, fmaf(x.y, z.y, fmaf(x.z, z.z, x.w * z.w)));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+            s[i] *= 1.4426950408889634f * 0.08838834764831845f;
+            mn = fmaxf(mn, s[i]);
+        }
+        const float f = fast_exp2(m - mn);
+        m = mn;
+        l *= f;
+        a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            if (r + i >= end) break;
+            const float p = fast_exp2(s[i] - m);
+            l += p;
+            a = make_float4(fmaf(p, y[i].x, a.x), fmaf(p, y[i].y, a.y), fmaf(p, y[i].z, a.z), fmaf(p, y[i].w, a.w));
+        }
+    }
+    *reinterpret_cast<float4 *>(o + lane * 4u) = a;
+    if (lane == 0) *reinterpret_cast<float2 *>(ml) = make_float2(m, l);
+}
 
 template <bool F32, int NS>
 __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
@@ -584,6 +641,7 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
                     *reinterpret_cast<float4 *>(tile_sm + r * 512u + (((c * 8u + i) ^ lane) << 4)) =
                         make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
+            if (valid && half == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
             if (took) asm volatile("bar.sync 10, 128;" ::: "memory");  // (the sums of all columns are read)
             // a warp stores its own 32 rows, two that share them half of them each
             if (H == 1) __syncwarp();
@@ -591,11 +649,21 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
             const uint32_t rows = min(T, Gr.n_seqs - mt * T) * G;  // of the tile's, those that hold a head
             const uint32_t r0 = (warp & 3u) * 32u + half * (32u / H);
             float *tile_out = P.part + (row - r) * 128u;
+            uint32_t bad = 0;  // rows with an element that is not finite
 #pragma unroll 8
-            for (uint32_t x = r0; x < min(r0 + 32u / H, rows); x++)
-                *reinterpret_cast<float4 *>(tile_out + x * 128u + lane * 4u) =
-                    *reinterpret_cast<const float4 *>(tile_sm + x * 512u + ((lane ^ (x & 31u)) << 4));
-            if (valid && half == 0) *reinterpret_cast<float2 *>(P.ml + row * 2u) = make_float2(m, l);
+            for (uint32_t x = r0; x < min(r0 + 32u / H, rows); x++) {
+                const float4 y = *reinterpret_cast<const float4 *>(tile_sm + x * 512u + ((lane ^ (x & 31u)) << 4));
+                *reinterpret_cast<float4 *>(tile_out + x * 128u + lane * 4u) = y;
+                if (!all_finite(y)) bad |= 1u << (x - r0);
+            }
+            bad = __reduce_or_sync(0xffffffffu, bad);
+            for (; bad; bad &= bad - 1u) {
+                const uint32_t x = r0 + (uint32_t)__ffs((int)bad) - 1u, hl = x % G;
+                const PrefixSeq sq = tab[Gr.seq0 + mt * T + x / G];
+                const uint64_t at = (uint64_t)kvh * 128u;
+                redo_row(reinterpret_cast<const char *>(sq.q) + (uint64_t)(kvh * G + hl) * (F32 ? 512u : 256u), !F32, Gr.k + at,
+                         Gr.v + at, (uint64_t)P.kv_heads * 128u, max(sq.start, kbeg), kend, tile_out + x * 128u, P.ml + (row - r + x) * 2u);
+            }
         }
     }
     fence_before();
@@ -711,6 +779,8 @@ static int launch(const PrefixGroup *groups, uint32_t n, const PrefixSeq *seqs, 
         PrefixDev &D = P.group[i];
         if (!tc05::make_map(&D.kmap, X.k, kv_heads * 128u, X.len) || !tc05::make_map(&D.vmap, X.v, kv_heads * 128u, X.len))
             return set_error(SF37KV_ECUDA, "prefix: tensor map encoding failed");
+        D.k = (const __half *)X.k;
+        D.v = (const __half *)X.v;
         D.lo = X.lo;
         D.len = X.len;
         D.seq0 = X.seq0;

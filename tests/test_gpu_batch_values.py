@@ -202,3 +202,37 @@ def test_int8_rows_that_are_not_finite_beside_a_prefix(dtype):
     where[3, group:] = True
     i8_views(raw_v, cap, heads)[1][3, 1, (plen + 11) % cap] = math.nan
     _finite_elsewhere(_shared(prefix, (raw_k, raw_v, cap), pos, q, heads, kv.I8), clean, where)
+
+
+@pytest.mark.parametrize("dtype", IO)
+# heads a KV head, sequences, prefix rows: one Q tile and two, one split and several
+@pytest.mark.parametrize("group,n,plen", [(8, 6, 400), (12, 25, 300), (8, 40, 5000), (16, 9, 2000)])
+def test_prefix_rows_that_are_not_finite(group, n, plen, dtype):
+    # rows that some sequences' windows leave out: their outputs are those of the rows that they attend to
+    heads, cap = 2, 20
+    prefix = rows(1, plen, heads).half(), rows(2, plen, heads).half()
+    k, v = rows(3, n, cap, heads).half(), rows(4, n, cap, heads).half()
+    q = rows(5, n, heads * group, dtype=dtype)
+    window = [0 if i % 4 == 0 else 1 + (plen + 10) * (i % 4) // 4 for i in range(n)]
+    pos = [plen + 2 + i % 9 for i in range(n)]
+    first = [p + 1 - w if w else 0 for p, w in zip(pos, window)]
+    bad = [0, plen // 3, plen // 3 + 1, plen // 2 - 40]
+    for j, row in enumerate(bad):
+        prefix[0][row, j % 2, 5] = (math.nan, math.inf)[j // 2]
+        prefix[1][row, :, 7] = (math.inf, math.nan, -math.inf, math.nan)[j]
+    out = torch.full_like(q, 5.0)
+    d = kv.decode_seqs_desc(k, v, cap, pos, q, out, sliding=[w > 0 for w in window], window=window)
+    g = kv.shared_groups_desc([dict(k_cache=prefix[0], v_cache=prefix[1], prefix_len=plen, seqs=d)])
+    kv.decode_shared(g, heads * group, heads, D, kv.F16, dtype, workspace(kv.decode_shared_workspace(1, n, heads * group, heads)))
+    finite = 0
+    for i in range(n):
+        own = torch.arange(max(plen, first[i]), pos[i] + 1, device="cuda") % cap
+        ki, vi = (torch.cat([x[min(first[i], plen):], y[i][own]]).double() for x, y in zip(prefix, (k, v)))
+        want, mag, reach = attend(q[i], ki, vi, None)
+        tol = bound(want, mag, reach, ki.shape[0], dtype, p_f16=dtype == torch.bfloat16)
+        ok = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(out[i]), ok), f"sequence {i}"
+        if ok.any():
+            check(out[i][ok], want[ok], tol[ok], f"sequence {i}")
+            finite += 1
+    assert 0 < finite < n and kv.device_error() == 0
