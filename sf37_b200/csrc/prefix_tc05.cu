@@ -221,7 +221,7 @@ template <bool F32, int NS>
 __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kernel(const __grid_constant__ PrefixParams<NS> P) {
     using namespace tc05;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    enum { B_KFULL = 0, B_KEMPTY = 3, B_VFULL = 6, B_VEMPTY = 8, B_SFULL = 10, B_PFULL = 12, B_ODONE = 14, N_BARS = 16 };
+    enum { B_KFULL = 0, B_KEMPTY = 3, B_VFULL = 6, B_VEMPTY = 8, B_SFULL = 10, B_PFULL = 12, B_ODONE = 14, B_DRAIN = 16, N_BARS = 17 };
     enum { T_Q = 0, T_K = 2, T_V = 4 };  // 32 KB tiles; Q: two tiles (pair) or hi and lo (F32), else a third K tile
     __shared__ __align__(8) uint64_t bars[N_BARS];
     __shared__ uint32_t tmem_base_sh;
@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
             bar_init(bar(B_PFULL + t), 128 * H);
             bar_init(bar(B_ODONE + t), 1);
         }
+        bar_init(bar(B_DRAIN), 1);
         asm volatile("fence.mbarrier_init.release.cluster;");
         abort_sh = 0;
     }
@@ -304,12 +305,21 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
     fence_after();
     const uint32_t tmem = tmem_base_sh;
 
+    uint32_t k_loads = 0, v_loads = 0;  // issued, of the thread that does
+
     if (warp == kSoft + 1) {
         // ---------------- TMA loader: a ring of K tiles and one of V tiles ----------------
         auto loader = [&](auto kind) {
             constexpr uint32_t kRing = decltype(kind)::value && !F32 ? 3 : 2, kTile0 = kRing == 3 ? 1 : T_K;
-            auto load_k = [&](uint32_t j) { load(bar(B_KFULL + j % kRing), tile(kTile0 + j % kRing), &Gr.kmap, j); };
-            auto load_v = [&](uint32_t j) { load(bar(B_VFULL + (j & 1u)), tile(T_V + (j & 1u)), &Gr.vmap, j); };
+            auto load_k = [&](uint32_t j) {
+                load(bar(B_KFULL + j % kRing), tile(kTile0 + j % kRing), &Gr.kmap, j);
+                k_loads = j + 1u;
+            };
+            auto load_v = [&](uint32_t j) {
+                load(bar(B_VFULL + (j & 1u)), tile(T_V + (j & 1u)), &Gr.vmap, j);
+                v_loads = j + 1u;
+            };
+            k_loads = 1u;
             for (uint32_t j = 0; j < kRing && j < nt; j++) {
                 if (j > 0) load_k(j);
                 if (j < 2) load_v(j);
@@ -668,7 +678,23 @@ __global__ void __launch_bounds__(soft_warps(F32) * 32 + 64, 1) prefix_tc05_kern
     }
     fence_before();
     __syncthreads();
-    if (abort_sh && tid == 0) atomicExch(&g_prefix_error, 1);
+    if (abort_sh) {
+        // The loads and MMAs in flight end before the shared memory and TMEM go, as far as
+        // another bounded wait for each tells.
+        if (loads) {
+            const uint32_t ring = solo && !F32 ? 3u : 2u;
+#pragma unroll 1
+            for (uint32_t t = 0; t < ring && t < k_loads; t++) (void)wait_bar(bar(B_KFULL + t), ((k_loads - 1u - t) / ring) & 1u);
+#pragma unroll 1
+            for (uint32_t t = 0; t < 2u && t < v_loads; t++) (void)wait_bar(bar(B_VFULL + t), ((v_loads - 1u - t) / 2u) & 1u);
+        }
+        if (warp == kSoft && lane == 0) {
+            commit(bar(B_DRAIN));
+            (void)wait_bar(bar(B_DRAIN), 0);
+        }
+        __syncthreads();
+        if (tid == 0) atomicExch(&g_prefix_error, 1);
+    }
     fence_after();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
