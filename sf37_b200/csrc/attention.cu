@@ -1220,11 +1220,12 @@ static const size_t kSmemF16 = smem_pipe(4, 3), kSmemF16Wide = smem_pipe(8, 3), 
 // the same stream may start while one is still running; a job of the new
 // launch may stream its rows before griddepcontrol.wait only if the running
 // kernel cannot write them, i.e. it appended to neither of the job's caches
-// (sf37kv_decode_noalloc's kernel records its appends here too).  Kernels
-// that this file does not launch (other libraries', this library's appends
-// and prefills) trigger no early start, so a decode that follows one of them
-// starts after it has completed whatever the record says; with no record for
-// a stream, no job streams early.
+// (sf37kv_decode_noalloc's kernel records its appends here too).  The int8
+// and shared-prefix kernels, which write caches and trigger early too, drop the
+// record (launch_early); other kernels that this file does not launch (other
+// libraries', this library's f16/f32 appends and prefills) trigger no early
+// start, so a decode that follows one of them starts after it has completed
+// whatever the record says.  With no record for a stream, no job streams early.
 struct StreamRecord {
     cudaStream_t stream;
     bool used;
