@@ -1147,7 +1147,7 @@ static int decode_groups(const char *what, const sf37kv_shared_group *groups, ui
             const sf37kv_shared_group &Gr = groups[gi];
             const uint32_t take = std::min(Gr.n_seqs - k0, most - n);
             PrefixGroup &X = pg[n_pg];
-            X = PrefixGroup{Gr.prefix.k_cache, Gr.prefix.v_cache, Gr.prefix_len, Gr.prefix_len, Gr.prefix.cap, n, take};
+            X = PrefixGroup{Gr.prefix.k_cache, Gr.prefix.v_cache, Gr.prefix_len, Gr.prefix_len, n, take};
             for (uint32_t k = 0; k < take; k++, n++) {
                 const sf37kv_decode_seq &L = Gr.seqs[k0 + k];
                 const uint32_t have = L.pos + 1u;

@@ -208,11 +208,10 @@ struct PrefixSeq {
 // One group: all sequences over the rows [lo, len) of one f16 prefix cache.
 struct PrefixGroup {
     const void *k, *v;
-    uint32_t lo, len, cap;
+    uint32_t lo, len;
     uint32_t seq0, n_seqs;      // its sequences in the launch's list
     // filled by prefix_plan()
     uint32_t m_tiles, splits, tiles_per_split;
-    uint32_t unit0;             // first (kv head, m tile) unit of the group
     uint32_t part0;             // first partial tile of the group
 };
 
