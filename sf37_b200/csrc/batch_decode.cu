@@ -1067,19 +1067,19 @@ static bool append_conflict(const sf37kv_shared_group *groups, uint32_t n_groups
     for (uint32_t i = 0; i < n_groups; i++)
         for (uint32_t k = 0; k < groups[i].n_seqs; k++) any |= groups[i].seqs[k].k_new != nullptr;
     if (!any) return false;
-    std::vector<Span> spans;
-    spans.reserve((size_t)(total + n_groups) * 2u);
-    for (int which = 0; which < 2; which++)
+    return parts_conflict((size_t)(total + n_groups) * 2u, [&](const auto &add) {
         for (uint32_t i = 0; i < n_groups; i++) {
-            const sf37kv_cache &prefix = groups[i].prefix;
-            if (groups[i].n_seqs && groups[i].prefix_len)
-                spans.push_back(span_of(which ? prefix.v_cache : prefix.k_cache, groups[i].prefix_len * prefix_row, false));
-            for (uint32_t k = 0; k < groups[i].n_seqs; k++) {
-                const sf37kv_decode_seq &L = groups[i].seqs[k];
-                spans.push_back(span_of(which ? L.cache.v_cache : L.cache.k_cache, L.cache.cap * row, L.k_new != nullptr));
+            const sf37kv_shared_group &Gr = groups[i];
+            const uint64_t bytes = Gr.n_seqs ? Gr.prefix_len * prefix_row : 0u;
+            add(2, Gr.prefix.k_cache, bytes, false);
+            add(3, Gr.prefix.v_cache, bytes, false);
+            for (uint32_t k = 0; k < Gr.n_seqs; k++) {
+                const sf37kv_decode_seq &L = Gr.seqs[k];
+                add(0, L.cache.k_cache, L.cache.cap * row, L.k_new != nullptr);
+                add(1, L.cache.v_cache, L.cache.cap * row, L.k_new != nullptr);
             }
         }
-    return spans_conflict(spans);
+    });
 }
 
 // Decode of all groups; ring_clamp (sf37kv_decode_i8): no prefixes, and a full cache's

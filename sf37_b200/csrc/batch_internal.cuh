@@ -37,21 +37,44 @@ static inline int check_cache(const char *what, uint32_t i, const sf37kv_cache &
     return SF37KV_OK;
 }
 
-// Memory that one call reads or writes, kernels of the call side by side.
-struct Span {
-    uintptr_t lo, hi;
-    bool writes;
-};
-static inline Span span_of(const void *p, uint64_t bytes, bool writes) {
-    return Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, writes};
-}
-// Whether a span that is written overlaps another one.  Reorders the spans.
-static inline bool spans_conflict(std::vector<Span> &s) {
-    const auto before = [](const Span &a, const Span &b) { return a.lo < b.lo; };
-    if (!std::is_sorted(s.begin(), s.end(), before)) std::sort(s.begin(), s.end(), before);
+// Whether memory that one part of a call writes overlaps what another part reads or
+// writes.  each(add) calls add(list, address, bytes, writes) for every part, at most n
+// of them; `list` (below kLists) tells parts apart that lie in order, each list in a
+// range of its own, as a rule: K and V caches in one allocation each.  Then two
+// comparisons a part settle it; otherwise the parts are sorted (std::bad_alloc).
+constexpr uint32_t kLists = 4;
+template <typename Each>
+static bool parts_conflict(size_t n, const Each &each) {
+    struct Span {
+        uintptr_t lo, hi;
+        bool writes;
+    };
+    Span list[kLists] = {};  // from the lowest byte to the highest
+    bool in_order[kLists] = {true, true, true, true};
+    each([&](uint32_t i, const void *p, uint64_t bytes, bool writes) {
+        if (!bytes) return;
+        Span &x = list[i];
+        const uintptr_t lo = (uintptr_t)p, hi = lo + (uintptr_t)bytes;
+        x.writes |= writes;
+        in_order[i] &= lo >= x.hi;
+        x.lo = x.hi ? std::min(x.lo, lo) : lo;
+        x.hi = std::max(x.hi, hi);
+    });
+    bool apart = true;
+    for (uint32_t i = 0; i < kLists; i++) {
+        apart &= in_order[i] || !list[i].writes;
+        for (uint32_t k = 0; k < i; k++)
+            apart &= !(list[i].writes || list[k].writes) || list[i].hi <= list[k].lo || list[k].hi <= list[i].lo;
+    }
+    if (apart) return false;
+    std::vector<Span> s;
+    s.reserve(n);
+    each([&](uint32_t, const void *p, uint64_t bytes, bool writes) {
+        if (bytes) s.push_back(Span{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes, writes});
+    });
+    std::sort(s.begin(), s.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
     uintptr_t any = 0, written = 0;  // ends of the spans so far
     for (const Span &x : s) {
-        if (x.lo >= x.hi) continue;
         if (x.lo < written || (x.writes && x.lo < any)) return true;
         any = std::max(any, x.hi);
         if (x.writes) written = std::max(written, x.hi);

@@ -217,15 +217,14 @@ extern "C" int sf37kv_append_i8(const sf37kv_append_i8_layer *layers, uint32_t n
             return set_error(SF37KV_EINVAL, "append_i8: layer %u has too many rows for one call", i);
     }
     try {
-        std::vector<Span> spans;
-        spans.reserve((size_t)n_layers * 2);
-        for (int which = 0; which < 2; which++)
-            for (uint32_t i = 0; i < n_layers; i++) {
-                const sf37kv_cache &c = layers[i].cache;
-                if (layers[i].n_tok)
-                    spans.push_back(span_of(which ? c.v_cache : c.k_cache, (uint64_t)c.cap * kv_heads * 132u, true));
-            }
-        if (spans_conflict(spans))
+        if (parts_conflict((size_t)n_layers * 2, [&](const auto &add) {
+                for (uint32_t i = 0; i < n_layers; i++) {
+                    const sf37kv_cache &c = layers[i].cache;
+                    const uint64_t bytes = layers[i].n_tok ? (uint64_t)c.cap * kv_heads * 132u : 0u;
+                    add(0, c.k_cache, bytes, true);
+                    add(1, c.v_cache, bytes, true);
+                }
+            }))
             return set_error(SF37KV_EINVAL, "append_i8: one cache is written twice in one call, or overlaps another");
     } catch (const std::bad_alloc &) {
         return set_error(SF37KV_ENOMEM, "append_i8: no memory to compare %u layers", n_layers);
@@ -287,20 +286,21 @@ extern "C" int sf37kv_read_i8(const sf37kv_read_i8_layer *layers, uint32_t n_lay
     }
     try {
         // Destinations by the rows that are written: layers may fill parts of one cache.
-        std::vector<Span> spans;
-        spans.reserve((size_t)n_layers * 6);
-        for (int which = 0; which < 2; which++)
-            for (uint32_t i = 0; i < n_layers; i++) {
-                const sf37kv_read_i8_layer &L = layers[i];
-                if (L.rows == 0) continue;
-                const char *dst = (const char *)(which ? L.dst.v_cache : L.dst.k_cache);
-                const uint64_t row = (uint64_t)kv_heads * 128u * (uint64_t)dst_dtype, slot = L.first_pos % L.dst.cap,
-                               head = std::min<uint64_t>(L.rows, L.dst.cap - slot);
-                spans.push_back(span_of(dst + slot * row, head * row, true));
-                spans.push_back(span_of(dst, (L.rows - head) * row, true));
-                spans.push_back(span_of(which ? L.src.v_cache : L.src.k_cache, (uint64_t)L.src.cap * kv_heads * 132u, false));
-            }
-        if (spans_conflict(spans))
+        const uint64_t row = (uint64_t)kv_heads * 128u * (uint64_t)dst_dtype;
+        if (parts_conflict((size_t)n_layers * 6, [&](const auto &add) {
+                for (uint32_t i = 0; i < n_layers; i++) {
+                    const sf37kv_read_i8_layer &L = layers[i];
+                    if (L.rows == 0) continue;
+                    const uint64_t slot = L.first_pos % L.dst.cap, head = std::min<uint64_t>(L.rows, L.dst.cap - slot),
+                                   bytes = (uint64_t)L.src.cap * kv_heads * 132u;
+                    add(0, L.dst.k_cache, (L.rows - head) * row, true);
+                    add(0, (const char *)L.dst.k_cache + slot * row, head * row, true);
+                    add(1, L.dst.v_cache, (L.rows - head) * row, true);
+                    add(1, (const char *)L.dst.v_cache + slot * row, head * row, true);
+                    add(2, L.src.k_cache, bytes, false);
+                    add(3, L.src.v_cache, bytes, false);
+                }
+            }))
             return set_error(SF37KV_EINVAL, "read_i8: rows that one layer writes are another's, read or written");
     } catch (const std::bad_alloc &) {
         return set_error(SF37KV_ENOMEM, "read_i8: no memory to compare %u layers", n_layers);
