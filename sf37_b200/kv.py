@@ -224,6 +224,7 @@ class Descriptors(np.ndarray):
 
     def __array_finalize__(self, source):
         self.held = getattr(source, "held", None)
+        self.at = None  # this array's address, once asked for
 
 
 class _Held:
@@ -236,18 +237,18 @@ class _Held:
         self.device, self.cache_heads, self.dtype, self.cache = device, cache_heads, dtype, cache
         self.kv_heads, self.q_heads = kv_heads, q_heads
 
-    def check(self, what, kv_heads, dtype, cache=None, q_heads=None):
+    def check(self, what, device, kv_heads, dtype, cache, q_heads):
         if self.kv_heads not in (None, kv_heads) or kv_heads > self.cache_heads:
             has = f"rows of {self.kv_heads}" if self.kv_heads not in (None, kv_heads) else f"room for {self.cache_heads}"
             raise ValueError(f"{what}: kv_heads is {kv_heads}, the tensors have {has}")
-        if q_heads is not None and q_heads != self.q_heads:
+        if q_heads != self.q_heads:
             raise ValueError(f"{what}: q_heads is {q_heads}, the queries have {self.q_heads}")
-        if dtype != self.dtype:
+        if dtype is not self.dtype:
             raise ValueError(f"{what}: dtype is {dtype}, the tensors are {self.dtype}")
-        if cache is not None and cache != self.cache:
+        if cache is not self.cache:
             raise ValueError(f"{what}: caches of {cache} are needed, the descriptors' are {self.cache}")
-        if self.device != torch.cuda.current_device():
-            raise ValueError(f"{what}: the tensors are on CUDA device {self.device}, which is not the current one")
+        if device != self.device:
+            raise ValueError(f"{what}: the tensors are on CUDA device {self.device}, the current one is {device}")
 
 
 def _addresses(name, x, n, dtypes=None, inner=None):
@@ -313,19 +314,24 @@ def _records(layers, dtype, name):
     """Address and length of a descriptor array."""
     if layers.dtype != dtype or layers.ndim != 1 or not layers.flags.c_contiguous:
         raise ValueError(f"a contiguous array of {name}() is needed")
-    return layers.ctypes.data, len(layers)  # (__array_interface__ lists all fields first: 12 us instead of 2)
+    if type(layers) is not Descriptors:
+        return layers.ctypes.data, len(layers)
+    if layers.at is None:  # (ctypes: 1 us; __array_interface__ lists all fields first: 12)
+        layers.at = layers.ctypes.data
+    return layers.at, len(layers)
 
 
-def _checked(layers, what, *args, **kwargs):
-    held = getattr(layers, "held", None)  # a plain array of records is the caller's own
-    if held is not None:
-        held.check(what, *args, **kwargs)
+def _checked(layers, what, device, kv_heads, dtype, cache, q_heads):
+    if type(layers) is Descriptors and layers.held is not None:  # a plain array of records is the caller's own
+        layers.held.check(what, device, kv_heads, dtype, cache, q_heads)
 
 
 def _space(workspace):
-    if not workspace.is_cuda or workspace.get_device() != torch.cuda.current_device() or not workspace.is_contiguous():
+    """Device, address and bytes of a workspace."""
+    device = workspace.get_device()  # -1 on the CPU
+    if device != torch.cuda.current_device() or not workspace.is_contiguous():
         raise ValueError("workspace: a contiguous tensor on the current CUDA device is needed")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return device, workspace.data_ptr(), workspace.nbytes
 
 
 def i8_cache_bytes(cap, kv_heads, head_dim=128) -> int:
@@ -353,7 +359,7 @@ def append_i8_desc(k_cache, v_cache, cap, pos0, k, v):
 
 def append_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Quantises the rows of append_i8_desc() into their caches; dtype: the rows' torch dtype."""
-    _checked(layers, "append_i8", kv_heads, dtype)
+    _checked(layers, "append_i8", torch.cuda.current_device(), kv_heads, dtype, torch.uint8, None)
     check(lib().sf37kv_append_i8(*_records(layers, APPEND_I8_LAYER, "append_i8_desc"), kv_heads, head_dim, _IO[dtype], _sp(stream)),
           "sf37kv_append_i8")
 
@@ -375,7 +381,7 @@ def read_i8_desc(k_cache, v_cache, cap, dst_k, dst_v, dst_cap, first_pos, rows):
 
 def read_i8(layers, kv_heads, head_dim, dtype, stream=None):
     """Reads the rows of read_i8_desc() back; dtype: the destinations' torch dtype."""
-    _checked(layers, "read_i8", kv_heads, dtype)
+    _checked(layers, "read_i8", torch.cuda.current_device(), kv_heads, dtype, torch.uint8, None)
     check(lib().sf37kv_read_i8(*_records(layers, READ_I8_LAYER, "read_i8_desc"), kv_heads, head_dim, _DT[dtype], _sp(stream)),
           "sf37kv_read_i8")
 
@@ -411,9 +417,10 @@ def decode_i8_workspace(n_seqs, q_heads, kv_heads) -> int:
 
 def decode_i8(seqs, q_heads, kv_heads, head_dim, dtype, workspace, stream=None):
     """One decode step over int8 caches; dtype: torch dtype of q and out."""
-    _checked(seqs, "decode_i8", kv_heads, dtype, torch.uint8, q_heads)
+    device, at, size = _space(workspace)
+    _checked(seqs, "decode_i8", device, kv_heads, dtype, torch.uint8, q_heads)
     check(lib().sf37kv_decode_i8(*_records(seqs, DECODE_SEQ, "decode_seqs_desc"), q_heads, kv_heads, head_dim, _IO[dtype],
-                                 *_space(workspace), _sp(stream)),
+                                 at, size, _sp(stream)),
           "sf37kv_decode_i8")
 
 
@@ -438,7 +445,7 @@ class _Groups:
     """Group descriptors, the sequence arrays that they point to, and the KV heads of the prefixes."""
 
     def __init__(self, desc, seqs, prefixes):
-        self.desc, self.seqs, self.prefixes = desc, seqs, prefixes
+        self.desc, self.seqs, self.prefixes, self.at = desc, seqs, prefixes, desc.ctypes.data
 
 
 def decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads) -> int:
@@ -448,11 +455,12 @@ def decode_shared_workspace(n_groups, n_seqs, q_heads, kv_heads) -> int:
 
 def decode_shared(groups, q_heads, kv_heads, head_dim, cache_dtype, dtype, workspace, stream=None):
     """One decode step of groups that share a prefix; cache_dtype: F16 or I8, of the sequences' own caches."""
-    d = groups.desc
+    device, at, size = _space(workspace)
     for seqs in groups.seqs:
-        _checked(seqs, "decode_shared", kv_heads, dtype, torch.uint8 if cache_dtype == I8 else torch.float16, q_heads)
-    if any(h != kv_heads for h in groups.prefixes):
-        raise ValueError(f"decode_shared: kv_heads is {kv_heads}, the prefixes have {groups.prefixes}")
-    check(lib().sf37kv_decode_shared(d.ctypes.data, len(d), q_heads, kv_heads, head_dim, cache_dtype, _IO[dtype],
-                                     *_space(workspace), _sp(stream)),
+        _checked(seqs, "decode_shared", device, kv_heads, dtype, torch.uint8 if cache_dtype == I8 else torch.float16, q_heads)
+    for heads in groups.prefixes:
+        if heads != kv_heads:
+            raise ValueError(f"decode_shared: kv_heads is {kv_heads}, the prefixes have {groups.prefixes}")
+    check(lib().sf37kv_decode_shared(groups.at, len(groups.seqs), q_heads, kv_heads, head_dim, cache_dtype, _IO[dtype],
+                                     at, size, _sp(stream)),
           "sf37kv_decode_shared")

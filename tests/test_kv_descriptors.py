@@ -168,13 +168,16 @@ def test_rows_and_prefixes_of_different_shapes(calls):
 
 
 def test_workspaces_and_devices(calls, monkeypatch):
-    s = seqs()
+    s, append_0 = seqs(), append()
     for ws in (torch.zeros(1 << 10, dtype=torch.uint8), space()[::2], torch.zeros(8, dtype=torch.uint8).as_subclass(OnOther)):
         with pytest.raises(ValueError, match="workspace"):
             kv.decode_i8(s, 8, 4, D, torch.float32, ws)
         with pytest.raises(ValueError, match="workspace"):
             kv.decode_shared(groups(seqs(cache="f16")), 8, 4, D, kv.F16, torch.float32, ws)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)  # another device than when the array was made
-    with pytest.raises(ValueError, match="device 0"):
+    with pytest.raises(ValueError, match="workspace"):
         kv.decode_i8(s, 8, 4, D, torch.float32, space())
+    for call in (lambda ws: kv.decode_i8(s, 8, 4, D, torch.float32, ws), lambda ws: kv.append_i8(append_0, 4, D, torch.float32)):
+        with pytest.raises(ValueError, match="device 0"):
+            call(torch.zeros(8, dtype=torch.uint8).as_subclass(OnOther))
     assert not calls
