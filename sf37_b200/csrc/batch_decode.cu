@@ -22,12 +22,12 @@
 // in a fixed order, so results do not depend on which CTA is last.
 //
 // Measured (one B200, graph replay; of the measured copy rate): 48 layers x 32769
-// rows of I8, 8 KV heads, f32: 524-540 us (0.95-0.97); 64 sequences of 1 to 8192
-// rows, bf16: 89 us (0.96); one of 131072: 46 us (0.92); 128 windows of 512 rows,
-// 96 query heads: 40 us (0.53: a CTA's start and end are as long as its 512
-// rows); one of 2049: 9.3 us.  Under seconds of load the card's power cap lowers the
-// SMs to 1.6 GHz, and the 48 layers take 620 us (bf16 queries: 555): the integer
-// and f16 tiles of three digits then bound it.
+// rows of I8, 8 KV heads, f32: 520-560 us (0.91-0.98); 64 sequences of 1 to 8192
+// rows, bf16: 96 us (0.89); one of 131072: 47 us (0.90); 128 windows of 512 rows,
+// 96 query heads: 42 us (0.50: a CTA's start and end are as long as its 512
+// rows); one of 2049: 9.2 us.  Under seconds of load the card's power cap lowers the
+// SMs to 1.55 GHz, and the 48 layers take 660 us (bf16 queries: 648), 64 sequences
+// 112: the integer and f16 tiles then bound it.
 //
 // Sixteen M rows of a tile hold, by MODE:
 //   kPair  G <= 8, f32: eight heads twice, f16 "hi" and remainder "lo" of the weights

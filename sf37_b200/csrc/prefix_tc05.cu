@@ -15,8 +15,8 @@
 //
 // The first 16 warps are the softmax, eight for each stream and two threads for
 // each row; they weigh a tile in one pass, with the reference of the tiles
-// before it (one thread a row and two passes over S took 108 us where this takes
-// 101, below).  F32 has 8 and one thread a row: two leave it no registers.  Then
+// before it (one thread a row and two passes over S took 108 us where this took
+// 101, 64 sequences over 32768 rows).  F32 has 8 and one thread a row: two leave it no registers.  Then
 // one warp issues the MMAs and one the TMA loads.  TMEM: S_0, S_1, O_0, O_1 (128
 // columns each); P (f16) overwrites its S.  F32 (f32 queries and outputs): q and P
 // are two f16 parts each, q_hi + q_lo and P_hi + P_lo, 22 bits: twice the MMAs;
@@ -29,9 +29,9 @@
 // Bound by the MMA thread and the tensor pipe: a step (S and PV of one stream and
 // key tile) is 1024 cycles of MMA, issues in 1300-1500 (8 MMAs and their commits
 // take 600 on an idle SM, more beside the softmax) and takes 1850; its softmax takes
-// 1700 and is hidden by the other stream's.  64 sequences x 64 heads, bf16, no own
-// rows: 288 us over 131072 rows, 0.95 PFLOP/s (0.57 of the measured burst bf16
-// rate); 87 us over 32768, of which 15 are a CTA's start and end (64 KB of q and
+// 1700 and is hidden by the other stream's.  64 sequences x 64 heads, bf16: this
+// launch takes 292 us over 131072 rows, 0.94 PFLOP/s (0.56 of the measured burst
+// bf16 rate); 86 us over 32768, of which 15 are a CTA's start and end (64 KB of q and
 // the first tiles, a 128 KB partial out).
 #include <algorithm>
 #include <type_traits>
